@@ -1,0 +1,634 @@
+// Weights in 4 bits and rows in 8 bits: the products of few tokens that read them, and what makes such weights and rows.
+//
+// Weights: w[n, k] = s[n, k / G] q[n, k], q in -8..7 and s bfloat16, groups of G = 32, 64 or 128 columns.  Rows: x[t, k] =
+// a[t, k / G] p[t, k], p in -127..127 and a = max|x| / 127 of the group in float32.  maeddesg/ROCmForge's products of Q4_0 and Q4_1
+// blocks with Q8_0 rows (hip_kernels/quant/, src/gpu/quant_wrapper.rs) use the same pair, blocks of 32 and halves as scales; the layout,
+// the group sizes and the kernels here are this library's own.
+//
+// How weights are stored.  The unit is a tile of 16 rows by 64 columns, 512 bytes in a row, the tiles of 16 rows one after another along
+// K.  The 16 bytes of lane 4 g + t hold rows g and g + 8 of the columns 32 c + 8 t .. + 7, c = 0, 1, as four words (row g: c = 0, 1; row
+// g + 8: c = 0, 1); the low half of byte b of a word is column b of the eight, the high half column 4 + b.  So a lane's one 16-byte load
+// is what it feeds to two mma.m16n8k32 of 8-bit integers (or four m16n8k16 of bfloat16 numbers): halves of bytes become operands with
+// one shift and one mask, in place, and a row's 8 numbers for the same columns are one 8-byte load of the row as it lies.  The scales
+// lie beside them, [tile of rows, group, 16], row g + 8 r at 2 g + r: the two that a lane needs are one word.
+#include "common.cuh"
+#include <type_traits>
+
+#define W4_WARPS 8
+
+template <typename T> struct Quad;                       // four neighbouring numbers
+template <> struct Quad<float> {
+    static __device__ __forceinline__ void load(const float* p, float* v) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    }
+};
+template <> struct Quad<__nv_bfloat16> {
+    static __device__ __forceinline__ void load(const __nv_bfloat16* p, float* v) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
+        v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
+    }
+};
+// Columns c .. c + 3 of a row of n numbers, zeros from n on.  VEC: the row starts on an access of four and n is a multiple of four.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_quad(const T* row, int c, int n, float* v) {
+    if constexpr (VEC) {
+        if (c < n) Quad<T>::load(row + c, v);
+        else v[0] = v[1] = v[2] = v[3] = 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = c + i < n ? Cvt<T>::to_f32(row[c + i]) : 0.f;
+    }
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {           // NaN if either is
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
+// The 8-bit form of a group: G / 4 neighbouring lanes hold four numbers each; returns the lane's four bytes, and the group's scale in
+// `scale`.  A group of zeros has the scale 0, one below 2^-120 too (127 / m must stay finite); a NaN or an infinity in a group makes its
+// scale NaN, so that every product that reads it is NaN, as one of the numbers themselves would be NaN or infinite.
+template <int G>
+__device__ __forceinline__ uint32_t to_8_bits(const float* v, float& scale) {
+    float m = max_nan(max_nan(fabsf(v[0]), fabsf(v[1])), max_nan(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+    for (int o = G / 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const bool finite = m < INFINITY, some = m >= 0x1p-120f;
+    scale = !finite ? __uint_as_float(0x7fffffffu) : some ? m / 127.f : 0.f;
+    if (!finite || !some) return 0u;
+    const float inv = 127.f / m;                          // |v| inv <= 127 (1 + 2^-23): rounds to 127 at most
+    uint32_t out = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out |= (uint32_t)(__float2int_rn(v[i] * inv) & 255) << (8 * i);
+    return out;
+}
+
+// ---------------------------------------------------------------- rows to 8 bits
+// A lane has four columns; a block 1,024 columns of a row.
+template <typename T, int G, bool VEC>
+__global__ void __launch_bounds__(256) quantize_q8_kernel(const T* x, long long ldx, int8_t* __restrict__ q, float* __restrict__ scales,
+                                                          int T_, int K, int Kp) {
+    pdl_trigger();
+    pdl_wait(x);
+    const int c = 4 * (blockIdx.x * 256 + threadIdx.x);
+    for (int t = blockIdx.y; t < T_; t += gridDim.y) {
+        float v[4], s;
+        load_quad<T, VEC>(x + (size_t)t * ldx, c, K, v);
+        const uint32_t p = to_8_bits<G>(v, s);
+        if (c < Kp) {
+            *reinterpret_cast<uint32_t*>(q + (size_t)t * Kp + c) = p;
+            if (c % G == 0) scales[(size_t)t * (Kp / G) + c / G] = s;
+        }
+    }
+}
+
+// ... and the numbers that 8-bit rows stand for.
+template <typename T>
+__global__ void __launch_bounds__(256) dequantize_q8_kernel(const int8_t* q, const float* scales, T* __restrict__ y, int T_, int K, int Kp, int G) {
+    pdl_trigger();
+    pdl_wait(q, scales);
+    const int c = 4 * (blockIdx.x * 256 + threadIdx.x);
+    if (c >= K) return;
+    for (int t = blockIdx.y; t < T_; t += gridDim.y) {
+        const char4 p = *reinterpret_cast<const char4*>(q + (size_t)t * Kp + c);
+        const float s = scales[(size_t)t * (Kp / G) + c / G];
+        const float v[4] = {p.x * s, p.y * s, p.z * s, p.w * s};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < K) y[(size_t)t * K + c + i] = Cvt<T>::from_f32(v[i]);
+    }
+}
+
+// ---------------------------------------------------------------- gated unit to 8 bits
+// y[t, j] = act(gu[t, 2j]) gu[t, 2j + 1] (the fused weight's rows are interleaved), in 32 bits and from there to 8.
+template <typename T, int ACT, int G, bool VEC>
+__global__ void __launch_bounds__(256) swiglu_q8_kernel(const T* gu, int8_t* __restrict__ q, float* __restrict__ scales, int T_, int I, int Ip) {
+    pdl_trigger();
+    pdl_wait(gu);
+    const int c = 4 * (blockIdx.x * 256 + threadIdx.x);
+    for (int t = blockIdx.y; t < T_; t += gridDim.y) {
+        const T* row = gu + (size_t)t * 2 * I;
+        float a[4], b[4], v[4], s;
+        load_quad<T, VEC>(row, 2 * c, 2 * I, a);
+        load_quad<T, VEC>(row, 2 * c + 4, 2 * I, b);
+        const float g[4] = {a[0], a[2], b[0], b[2]}, u[4] = {a[1], a[3], b[1], b[3]};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float act;
+            if constexpr (ACT == 0) act = g[i] / (1.f + expf(-g[i]));
+            else if constexpr (ACT == 1) act = fmaxf(g[i], 0.f);
+            else act = 0.5f * g[i] * (1.f + tanhf(0.7978845608028654f * (g[i] + 0.044715f * g[i] * g[i] * g[i])));
+            v[i] = act * u[i];
+        }
+        const uint32_t p = to_8_bits<G>(v, s);
+        if (c < Ip) {
+            *reinterpret_cast<uint32_t*>(q + (size_t)t * Ip + c) = p;
+            if (c % G == 0) scales[(size_t)t * (Ip / G) + c / G] = s;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- add + RMSNorm to 8 bits
+// v = h[row] + sum_s pending[s][row];  y = v rsqrt(mean(v^2) + eps) w, to 8 bits from 32.  The kinds of pending and of rows are those
+// of add_rmsnorm (elementwise.cu).  A block has a row, a lane four columns at a time, in registers.
+template <typename T, int G, int NV, bool VEC>
+__global__ void __launch_bounds__(1024) add_rmsnorm_q8_kernel(float* __restrict__ h, const void* pending, int kind, int n_pending,
+                                                              size_t pstride, const void* w, int w_is_f32, float eps,
+                                                              int8_t* __restrict__ q, float* __restrict__ scales, const int* rows, int n_h, int H, int Hp) {
+    pdl_trigger();
+    __shared__ float red[34];
+    const int r = blockIdx.x;
+    const int t = rows ? min(max(rows[r], 0), n_h - 1) : r;             // (a row that is not there is never read)
+    pdl_wait(pending);
+    float* hrow = h + (size_t)t * H;
+    float v[NV][4];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = 4 * (threadIdx.x + i * blockDim.x);
+        load_quad<float, VEC>(hrow, c, H, v[i]);
+        if (kind == 1) {
+            for (int s = 0; s < n_pending; ++s) {
+                float p[4];
+                load_quad<float, VEC>(reinterpret_cast<const float*>(pending) + (size_t)s * pstride + (size_t)t * H, c, H, p);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i][j] += p[j];
+            }
+        } else if (kind == 2) {
+            float p[4];
+            load_quad<T, VEC>(reinterpret_cast<const T*>(pending) + (size_t)t * H, c, H, p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][j] += p[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ss += v[i][j] * v[i][j];
+    }
+    const float inv = rsqrtf(block_sum(ss, red) / (float)H + eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = 4 * (threadIdx.x + i * blockDim.x);
+        if (!rows && kind != 0) {
+            if constexpr (VEC) {
+                if (c < H) *reinterpret_cast<float4*>(hrow + c) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c + j < H) hrow[c + j] = v[i][j];
+            }
+        }
+        float y[4], s;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = c + j < H ? v[i][j] * inv * load_vec(w, w_is_f32, c + j) : 0.f;
+        const uint32_t p = to_8_bits<G>(y, s);
+        if (c < Hp) {
+            *reinterpret_cast<uint32_t*>(q + (size_t)r * Hp + c) = p;
+            if (c % G == 0) scales[(size_t)r * (Hp / G) + c / G] = s;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- weights to 4 bits, and back
+// The scale of a group: its largest magnitude becomes 7.5 steps (a grid of -8..7 then misses it by 3/4 of a step at most), rounded to five
+// significant bits.  s q has at most eight then, so every weight is a bfloat16 number: the products of 8-bit rows and the 16-bit products
+// of a prompt multiply the same weights, and nothing is rounded between them.  Steps of 1/16 octave between scales cost 3 % of the
+// quantisation step at most.  A NaN or an infinity makes the group's scale NaN.
+__device__ __forceinline__ float w4_scale(float m) {
+    if (!(m < INFINITY)) return __uint_as_float(0x7fc00000u);
+    if (m < 0x1p-100f) return 0.f;
+    uint32_t u = __float_as_uint(m / 7.5f);
+    u += 0x3ffffu + (u >> 19 & 1u);                      // to the nearest of five significant bits, ties to even
+    return __uint_as_float(u & 0xfff80000u);
+}
+// A warp makes the tiles of a group's columns: lane 4 g + t holds the eight columns of its two rows and two halves, 32 numbers a tile.
+template <typename T, int G>
+__global__ void __launch_bounds__(256) quantize_w4_kernel(const T* weight, long long ldw, uint4* __restrict__ packed, __nv_bfloat16* __restrict__ scales,
+                                                          int N, int K, int Kp) {
+    constexpr int TILES = G == 128 ? 2 : 1;              // tiles of 64 columns that a group spans
+    constexpr int GROUPS = G == 32 ? 2 : 1;              // groups in that many columns
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int units = Kp / (64 * TILES);
+    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (unit >= (long long)((N + 15) / 16) * units) return;
+    const int tile = (int)(unit / units), col0 = (int)(unit % units) * 64 * TILES;
+    float m[2][GROUPS] = {}, v[TILES][2][2][8];
+#pragma unroll
+    for (int b = 0; b < TILES; ++b)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int n = 16 * tile + g + 8 * r, k = col0 + 64 * b + 32 * c + 8 * t + j;
+                    v[b][r][c][j] = n < N && k < K ? Cvt<T>::to_f32(weight[(size_t)n * ldw + k]) : 0.f;
+                    m[r][GROUPS == 2 ? c : 0] = max_nan(m[r][GROUPS == 2 ? c : 0], fabsf(v[b][r][c][j]));
+                }
+    float s[2][GROUPS], inv[2][GROUPS];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < GROUPS; ++c) {
+            m[r][c] = max_nan(m[r][c], __shfl_xor_sync(0xffffffffu, m[r][c], 1));
+            m[r][c] = max_nan(m[r][c], __shfl_xor_sync(0xffffffffu, m[r][c], 2));
+            s[r][c] = w4_scale(m[r][c]);
+            inv[r][c] = s[r][c] > 0.f ? 1.f / s[r][c] : 0.f;             // (a NaN scale leaves zeros behind it)
+            if (t == 0) scales[((size_t)tile * (Kp / G) + col0 / G + c) * 16 + 2 * g + r] = __float2bfloat16_rn(s[r][c]);
+        }
+#pragma unroll
+    for (int b = 0; b < TILES; ++b) {
+        uint32_t word[4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                word[2 * r + c] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float f = inv[r][GROUPS == 2 ? c : 0];
+                    const int i = f > 0.f ? max(-8, min(7, __float2int_rn(v[b][r][c][j] * f))) : 0;
+                    word[2 * r + c] |= (uint32_t)(i & 15) << (8 * (j & 3) + 4 * (j >> 2));
+                }
+            }
+        packed[((size_t)tile * (Kp / 64) + col0 / 64 + b) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+    }
+}
+
+// The weights as numbers [N, K]: a warp writes a tile, a lane four runs of eight columns.
+template <typename T, int G>
+__global__ void __launch_bounds__(256) dequantize_w4_kernel(const uint4* packed, const __nv_bfloat16* scales, T* __restrict__ out, int N, int K, int Kp) {
+    pdl_wait(packed, scales);
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, blocks = Kp / 64;
+    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (unit >= (long long)((N + 15) / 16) * blocks) return;
+    const int tile = (int)(unit / blocks), block = (int)(unit % blocks);
+    const uint4 p = packed[(size_t)unit * 32 + lane];
+    const uint32_t word[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int n = 16 * tile + g + 8 * r, k = 64 * block + 32 * c + 8 * t;
+            if (n >= N || k >= K) continue;
+            const float s = __bfloat162float(scales[((size_t)tile * (Kp / G) + k / G) * 16 + 2 * g + r]);
+            T v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = (int)(word[2 * r + c] >> (8 * (j & 3) + 4 * (j >> 2)) & 15u);
+                v[j] = Cvt<T>::from_f32((float)((i ^ 8) - 8) * s);
+            }
+            T* to = out + (size_t)n * K + k;
+            if (K % 8 == 0) {
+#pragma unroll
+                for (int j = 0; j < 8 * (int)sizeof(T) / 16; ++j) reinterpret_cast<uint4*>(to)[j] = reinterpret_cast<const uint4*>(v)[j];
+            } else {
+                for (int j = 0; j < 8 && k + j < K; ++j) to[j] = v[j];
+            }
+        }
+}
+
+// Products stream their weights before they wait for the kernel before them, which holds for weights that were there before the step.
+// Where a kernel has just made them, this one stands between: it is launched without the early start, so what was written before it is
+// complete and visible when it begins, and the product's early part begins no sooner.
+__global__ void weights_made_kernel() {}
+
+// ---------------------------------------------------------------- products of few tokens
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+enum { W4_STORE = 0, W4_F32 = 1, W4_ADD = 2, W4_PARTIAL = 3 };
+
+struct W4Out {
+    void* out;
+    const void* bias;
+    int bias_is_f32, mode, out_is_f32, M, N;
+};
+__device__ __forceinline__ void w4_write(const W4Out& o, int split, int t, int n, float v) {
+    if (t >= o.M || n >= o.N) return;
+    if (o.mode == W4_PARTIAL) {
+        reinterpret_cast<float*>(o.out)[((size_t)split * o.M + t) * o.N + n] = v;
+        return;
+    }
+    if (o.bias != nullptr) v += load_vec(o.bias, o.bias_is_f32, n);
+    const size_t at = (size_t)t * o.N + n;
+    if (o.mode == W4_ADD) reinterpret_cast<float*>(o.out)[at] += v;
+    else if (o.out_is_f32) reinterpret_cast<float*>(o.out)[at] = v;
+    else reinterpret_cast<__nv_bfloat16*>(o.out)[at] = __float2bfloat16_rn(v);
+}
+
+// What a lane multiplies a tile of weights with: token g's numbers of the lane's columns, in the order in which they lie.
+// 8-bit rows are padded with zeros to whole tiles; 16-bit rows are the caller's, and end at K: WHOLE says that they can be read in 16
+// bytes at a time (8-number runs that lie inside or outside the row as a whole).
+template <typename X, bool WHOLE> struct RowPart;
+template <> struct RowPart<int8_t, true> {
+    uint2 v[2];
+    __device__ __forceinline__ void load(const int8_t* row, int k, int) {
+        v[0] = *reinterpret_cast<const uint2*>(row + k);
+        v[1] = *reinterpret_cast<const uint2*>(row + k + 32);
+    }
+    __device__ __forceinline__ void zero() { v[0] = v[1] = make_uint2(0u, 0u); }
+};
+template <bool WHOLE> struct RowPart<__nv_bfloat16, WHOLE> {
+    uint4 v[2];
+    static __device__ __forceinline__ uint4 eight(const __nv_bfloat16* row, int k, int K) {
+        uint4 r = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (WHOLE) {
+            if (k < K) r = *reinterpret_cast<const uint4*>(row + k);
+        } else {
+            const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
+            uint32_t two[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                two[i] = (k + 2 * i < K ? p[k + 2 * i] : 0u) | (k + 2 * i + 1 < K ? (uint32_t)p[k + 2 * i + 1] << 16 : 0u);
+            r = make_uint4(two[0], two[1], two[2], two[3]);
+        }
+        return r;
+    }
+    __device__ __forceinline__ void load(const __nv_bfloat16* row, int k, int K) {
+        v[0] = eight(row, k, K);
+        v[1] = eight(row, k + 32, K);
+    }
+    __device__ __forceinline__ void zero() { v[0] = v[1] = make_uint4(0u, 0u, 0u, 0u); }
+};
+
+// c += (rows g, g + 8; the 32 columns of half `half`) times the token's numbers.
+__device__ __forceinline__ void half_tile(int (&c)[4], uint32_t lo_row, uint32_t hi_row, const uint2& x) {
+    const uint32_t m = 0xf0f0f0f0u;                      // a half of a byte at its upper end is 16 q as a signed byte
+    mma_s8(c, lo_row << 4 & m, hi_row << 4 & m, lo_row & m, hi_row & m, x.x, x.y);
+}
+// Two halves of bytes, 16 bits apart, as bfloat16 numbers: 128 + (q + 8) in the bits of 128, less 136; both steps are exact.
+__device__ __forceinline__ uint32_t two_weights(uint32_t w) {
+    uint32_t v = (w & 0x000f000fu) ^ 0x43084308u;
+    const __nv_bfloat162 less = __float2bfloat162_rn(-136.f);
+    __nv_bfloat162 r = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&v), less);
+    return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ void half_tile(float (&c)[4], uint32_t lo_row, uint32_t hi_row, const uint4& x) {
+    // columns (0, 2), (1, 3) and (4, 6), (5, 7) of the eight are 16 bits apart in the word; the row's pairs are put together alike
+    mma_bf16(c, two_weights(lo_row), two_weights(hi_row), two_weights(lo_row >> 8), two_weights(hi_row >> 8),
+             __byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));
+    mma_bf16(c, two_weights(lo_row >> 4), two_weights(hi_row >> 4), two_weights(lo_row >> 12), two_weights(hi_row >> 12),
+             __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
+}
+
+// Eight tokens (blockIdx.z) by a tile of 16 rows: the block's warps share out the columns of its split.  A warp asks for four tiles of
+// 64 columns at a time, the next four while it multiplies; nothing passes through shared memory but the warps' sums, as no number of
+// a row is used by two warps.
+template <int G, typename X, bool WHOLE>
+__global__ void __launch_bounds__(32 * W4_WARPS) w4_eight_kernel(const uint4* __restrict__ w0, const uint32_t* __restrict__ w1, const X* x,
+                                                               const float* xs, long long ldx, int K, int blocks, W4Out o) {
+    using Sum = typename std::conditional<std::is_same<X, int8_t>::value, int, float>::type;
+    constexpr bool BYTES = std::is_same<X, int8_t>::value;
+    constexpr int D = 4;
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int slices = gridDim.y * W4_WARPS, slice = blockIdx.y * W4_WARPS + warp;
+    const int from = (int)((long long)blocks * slice / slices), to = (int)((long long)blocks * (slice + 1) / slices);
+    const uint4* wt = w0 + (size_t)blockIdx.x * blocks * 32 + lane;
+    const int groups = blocks * 64 / G;
+    const uint32_t* st = w1 + (size_t)blockIdx.x * groups * 8 + g;
+    uint4 w[D];
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+        if (from + i < to) w[i] = wt[(size_t)(from + i) * 32];
+    pdl_wait(x, xs);
+    const int tok = blockIdx.z * 8 + g, ta = blockIdx.z * 8 + 2 * t;
+    const bool mine = tok < o.M, has_a = ta < o.M, has_b = ta + 1 < o.M;
+    const X* xrow = x + (size_t)tok * ldx;
+    float acc[4] = {};
+    for (int b = from; b < to; b += D) {
+        uint4 next[D];
+        RowPart<X, WHOLE> rows[D];
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            if (b + D + i < to) next[i] = wt[(size_t)(b + D + i) * 32];
+            if (mine && b + i < to) rows[i].load(xrow, 64 * (b + i) + 8 * t, K);
+            else rows[i].zero();
+        }
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            if (b + i >= to) break;
+            Sum c[4] = {};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                half_tile(c, half ? w[i].y : w[i].x, half ? w[i].w : w[i].z, rows[i].v[half]);
+                if (G == 32 || half == 1) {
+                    const int group = (64 * (b + i) + 32 * half) / G;
+                    const uint32_t s2 = st[(size_t)group * 8];
+                    float s0 = __uint_as_float(s2 << 16), s1 = __uint_as_float(s2 & 0xffff0000u);
+                    float a0 = 1.f, a1 = 1.f;
+                    if constexpr (BYTES) {
+                        s0 *= 0.0625f; s1 *= 0.0625f;    // the products hold 16 q
+                        a0 = has_a ? xs[(size_t)ta * groups + group] : 0.f;
+                        a1 = has_b ? xs[(size_t)(ta + 1) * groups + group] : 0.f;
+                    }
+                    acc[0] += (float)c[0] * (s0 * a0);
+                    acc[1] += (float)c[1] * (s0 * a1);
+                    acc[2] += (float)c[2] * (s1 * a0);
+                    acc[3] += (float)c[3] * (s1 * a1);
+                    c[0] = c[1] = c[2] = c[3] = 0;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < D; ++i) w[i] = next[i];
+    }
+    __shared__ float part[W4_WARPS][8][17];              // [warp][token][row]
+    part[warp][2 * t][g] = acc[0];
+    part[warp][2 * t + 1][g] = acc[1];
+    part[warp][2 * t][g + 8] = acc[2];
+    part[warp][2 * t + 1][g + 8] = acc[3];
+    __syncthreads();
+    if (threadIdx.x < 128) {
+        const int token = threadIdx.x >> 4, row = threadIdx.x & 15;
+        float v = part[0][token][row];
+#pragma unroll
+        for (int i = 1; i < W4_WARPS; ++i) v += part[i][token][row];
+        w4_write(o, blockIdx.y, blockIdx.z * 8 + token, blockIdx.x * 16 + row, v);
+    }
+}
+
+// ---------------------------------------------------------------- launchers
+static bool bad_group(int G) { return G != 32 && G != 64 && G != 128; }
+static int padded(int K, int G) { const int u = G > 64 ? G : 64; return (K + u - 1) / u * u; }
+static bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// f(G as a constant)
+template <typename F>
+static void with_group(int G, F f) {
+    if (G == 32) f(std::integral_constant<int, 32>());
+    else if (G == 64) f(std::integral_constant<int, 64>());
+    else f(std::integral_constant<int, 128>());
+}
+static dim3 quad_grid(int T_, int Kp) { return dim3((Kp + 1023) / 1024, T_ < 65535 ? T_ : 65535); }
+
+template <typename T>
+static int launch_quantize_q8(const T* x, long long ldx, int8_t* q, float* s, int T_, int K, int G, cudaStream_t st) {
+    const int Kp = padded(K, G);
+    const bool vec = K % 4 == 0 && ldx % 4 == 0 && aligned(x, 4 * sizeof(T));
+    with_group(G, [&](auto gc) {
+        constexpr int GC = decltype(gc)::value;
+        if (vec) rf_launch(quantize_q8_kernel<T, GC, true>, quad_grid(T_, Kp), dim3(256), 0, st, x, ldx, q, s, T_, K, Kp);
+        else rf_launch(quantize_q8_kernel<T, GC, false>, quad_grid(T_, Kp), dim3(256), 0, st, x, ldx, q, s, T_, K, Kp);
+    });
+    RF_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T, int ACT>
+static int launch_swiglu_q8(const T* gu, int8_t* q, float* s, int T_, int I, int G, cudaStream_t st) {
+    const int Ip = padded(I, G);
+    const bool vec = I % 2 == 0 && aligned(gu, 4 * sizeof(T));
+    with_group(G, [&](auto gc) {
+        constexpr int GC = decltype(gc)::value;
+        if (vec) rf_launch(swiglu_q8_kernel<T, ACT, GC, true>, quad_grid(T_, Ip), dim3(256), 0, st, gu, q, s, T_, I, Ip);
+        else rf_launch(swiglu_q8_kernel<T, ACT, GC, false>, quad_grid(T_, Ip), dim3(256), 0, st, gu, q, s, T_, I, Ip);
+    });
+    RF_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T>
+static int launch_add_rmsnorm_q8(float* h, const void* pending, int kind, int n_pending, size_t pstride, const void* w, int w_is_f32, float eps,
+                                 int8_t* q, float* s, const int* rows, int n_rows, int n_h, int H, int G, cudaStream_t st) {
+    const int Hp = padded(H, G), quads = Hp / 4;
+    if (quads > 8 * 1024) return RF_ERR_UNSUPPORTED;
+    const bool vec = H % 4 == 0 && pstride % 4 == 0 && aligned(h, 16) && (kind == 0 || aligned(pending, kind == 1 ? 16 : 4 * sizeof(T)));
+    int threads = (quads + 31) / 32 * 32;
+    if (threads > 1024) threads = 1024;
+    const int per = (quads + threads - 1) / threads;
+    with_group(G, [&](auto gc) {
+        constexpr int GC = decltype(gc)::value;
+        auto go = [&](auto kernel) {
+            rf_launch(kernel, dim3(n_rows), dim3(threads), 0, st, h, pending, kind, n_pending, pstride, w, w_is_f32, eps, q, s, rows, n_h, H, Hp);
+        };
+        if (vec) {
+            if (per <= 1) go(add_rmsnorm_q8_kernel<T, GC, 1, true>);
+            else if (per <= 2) go(add_rmsnorm_q8_kernel<T, GC, 2, true>);
+            else go(add_rmsnorm_q8_kernel<T, GC, 8, true>);
+        } else {
+            go(add_rmsnorm_q8_kernel<T, GC, 8, false>);
+        }
+    });
+    RF_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" {
+
+// x [T, K] (rows ldx apart) -> q int8 [T, Kp], scales float32 [T, Kp / G]; Kp: K up to a multiple of 64 (128 if G is).
+int rf_quantize_q8(int dtype, const void* x, long long ldx, void* q, void* scales, int T_, int K, int G, cudaStream_t st) {
+    if (T_ < 0 || K <= 0 || bad_group(G)) return RF_ERR_BAD_ARG;
+    if (T_ == 0) return 0;
+    return dtype == 0 ? launch_quantize_q8((const float*)x, ldx, (int8_t*)q, (float*)scales, T_, K, G, st)
+                      : launch_quantize_q8((const __nv_bfloat16*)x, ldx, (int8_t*)q, (float*)scales, T_, K, G, st);
+}
+
+int rf_dequantize_q8(int dtype, const void* q, const void* scales, void* y, int T_, int K, int G, cudaStream_t st) {
+    if (T_ < 0 || K <= 0 || bad_group(G)) return RF_ERR_BAD_ARG;
+    if (T_ == 0) return 0;
+    const int Kp = padded(K, G);
+    if (dtype == 0) rf_launch(dequantize_q8_kernel<float>, quad_grid(T_, Kp), dim3(256), 0, st, (const int8_t*)q, (const float*)scales, (float*)y, T_, K, Kp, G);
+    else rf_launch(dequantize_q8_kernel<__nv_bfloat16>, quad_grid(T_, Kp), dim3(256), 0, st, (const int8_t*)q, (const float*)scales, (__nv_bfloat16*)y, T_, K, Kp, G);
+    RF_LAUNCH_CHECK();
+    return 0;
+}
+
+// act 0: silu, 1: relu, 2: gelu by tanh
+int rf_swiglu_q8(int dtype, const void* gu, int act, void* q, void* scales, int T_, int I, int G, cudaStream_t st) {
+    if (T_ < 0 || I <= 0 || bad_group(G) || act < 0 || act > 2) return RF_ERR_BAD_ARG;
+    if (T_ == 0) return 0;
+    auto go = [&](auto p) {
+        int8_t* qq = (int8_t*)q;
+        float* ss = (float*)scales;
+        return act == 0 ? launch_swiglu_q8<std::remove_cv_t<std::remove_pointer_t<decltype(p)>>, 0>(p, qq, ss, T_, I, G, st)
+             : act == 1 ? launch_swiglu_q8<std::remove_cv_t<std::remove_pointer_t<decltype(p)>>, 1>(p, qq, ss, T_, I, G, st)
+                        : launch_swiglu_q8<std::remove_cv_t<std::remove_pointer_t<decltype(p)>>, 2>(p, qq, ss, T_, I, G, st);
+    };
+    return dtype == 0 ? go((const float*)gu) : go((const __nv_bfloat16*)gu);
+}
+
+int rf_add_rmsnorm_q8(int dtype, float* h, const void* pending, int kind, int n_pending, long long pstride, const void* w, int w_is_f32, float eps,
+                      void* q, void* scales, const int* rows, int n_rows, int n_h, int H, int G, cudaStream_t st) {
+    if (n_rows < 0 || n_h < 0 || H <= 0 || bad_group(G) || kind < 0 || kind > 2 || n_pending < 0) return RF_ERR_BAD_ARG;
+    if (n_rows == 0) return 0;
+    if (n_h == 0) return RF_ERR_BAD_ARG;
+    return dtype == 0 ? launch_add_rmsnorm_q8<float>(h, pending, kind, n_pending, (size_t)pstride, w, w_is_f32, eps, (int8_t*)q, (float*)scales, rows, n_rows, n_h, H, G, st)
+                      : launch_add_rmsnorm_q8<__nv_bfloat16>(h, pending, kind, n_pending, (size_t)pstride, w, w_is_f32, eps, (int8_t*)q, (float*)scales, rows, n_rows, n_h, H, G, st);
+}
+
+// weight [N, K] (rows ldw apart) -> packed, scales (the layout above)
+int rf_quantize_w4(int dtype, const void* weight, long long ldw, void* packed, void* scales, int N, int K, int G, cudaStream_t st) {
+    if (N <= 0 || K <= 0 || bad_group(G)) return RF_ERR_BAD_ARG;
+    const int Kp = padded(K, G);
+    const long long units = (long long)((N + 15) / 16) * (Kp / (G == 128 ? 128 : 64));
+    if ((units + 7) / 8 > 0x7fffffffll) return RF_ERR_UNSUPPORTED;
+    with_group(G, [&](auto gc) {
+        constexpr int GC = decltype(gc)::value;
+        const dim3 grid((unsigned)((units + 7) / 8));
+        if (dtype == 0) quantize_w4_kernel<float, GC><<<grid, 256, 0, st>>>((const float*)weight, ldw, (uint4*)packed, (__nv_bfloat16*)scales, N, K, Kp);
+        else quantize_w4_kernel<__nv_bfloat16, GC><<<grid, 256, 0, st>>>((const __nv_bfloat16*)weight, ldw, (uint4*)packed, (__nv_bfloat16*)scales, N, K, Kp);
+    });
+    weights_made_kernel<<<1, 32, 0, st>>>();
+    RF_LAUNCH_CHECK();
+    return 0;
+}
+
+int rf_dequantize_w4(int dtype, const void* packed, const void* scales, void* out, int N, int K, int G, cudaStream_t st) {
+    if (N <= 0 || K <= 0 || bad_group(G)) return RF_ERR_BAD_ARG;
+    const int Kp = padded(K, G);
+    const long long units = (long long)((N + 15) / 16) * (Kp / 64);
+    if ((units + 7) / 8 > 0x7fffffffll) return RF_ERR_UNSUPPORTED;
+    with_group(G, [&](auto gc) {
+        constexpr int GC = decltype(gc)::value;
+        const dim3 grid((unsigned)((units + 7) / 8));
+        if (dtype == 0) rf_launch(dequantize_w4_kernel<float, GC>, grid, dim3(256), 0, st, (const uint4*)packed, (const __nv_bfloat16*)scales, (float*)out, N, K, Kp);
+        else rf_launch(dequantize_w4_kernel<__nv_bfloat16, GC>, grid, dim3(256), 0, st, (const uint4*)packed, (const __nv_bfloat16*)scales, (__nv_bfloat16*)out, N, K, Kp);
+    });
+    weights_made_kernel<<<1, 32, 0, st>>>();
+    RF_LAUNCH_CHECK();
+    return 0;
+}
+
+// Lets products that follow read weights that the stream's last kernels have made (see weights_made_kernel).
+int rf_weights_made(cudaStream_t st) {
+    weights_made_kernel<<<1, 32, 0, st>>>();
+    RF_LAUNCH_CHECK();
+    return 0;
+}
+
+// out = x w^T (+ bias): x_kind 0: 8-bit rows (x int8 [M, Kp], xs float32 [M, Kp / G]), 1: bfloat16 rows [M, K], ldx apart.  mode W4_STORE (float32 if out_is_f32, else bfloat16), W4_ADD (out float32 += ...), W4_PARTIAL (float32
+// [splits, M, N], no bias); splits > 1 with W4_PARTIAL only.
+int rf_gemm_w4(int x_kind, const void* x, const void* xs, long long ldx, const void* packed, const void* scales, const void* bias, int bias_is_f32,
+               void* out, int out_is_f32, int mode, int splits, int M, int N, int K, int G, cudaStream_t st) {
+    if (M <= 0 || N <= 0 || K <= 0 || bad_group(G) || splits < 1 || splits > 65535 || (splits > 1 && mode != W4_PARTIAL) || mode < 0 || mode > 3) return RF_ERR_BAD_ARG;
+    if ((x_kind == 0 && (!aligned(x, 8) || ldx % 8)) || !aligned(packed, 16) || !aligned(scales, 4)) return RF_ERR_BAD_ARG;
+    const bool whole = K % 8 == 0 && ldx % 8 == 0 && aligned(x, 16);
+    const int blocks = padded(K, G) / 64;
+    if ((M + 7) / 8 > 65535) return RF_ERR_UNSUPPORTED;
+    const W4Out o{out, bias, bias_is_f32, mode, out_is_f32, M, N};
+    with_group(G, [&](auto gc) {
+        constexpr int GC = decltype(gc)::value;
+        const dim3 grid((N + 15) / 16, splits, (M + 7) / 8);
+        const uint4* w0 = (const uint4*)packed;
+        const uint32_t* w1 = (const uint32_t*)scales;
+        const __nv_bfloat16* x16 = (const __nv_bfloat16*)x;
+        const float* none = nullptr;
+        const dim3 block(32 * W4_WARPS);
+        if (x_kind == 0) rf_launch(w4_eight_kernel<GC, int8_t, true>, grid, block, 0, st, w0, w1, (const int8_t*)x, (const float*)xs, ldx, K, blocks, o);
+        else if (whole) rf_launch(w4_eight_kernel<GC, __nv_bfloat16, true>, grid, block, 0, st, w0, w1, x16, none, ldx, K, blocks, o);
+        else rf_launch(w4_eight_kernel<GC, __nv_bfloat16, false>, grid, block, 0, st, w0, w1, x16, none, ldx, K, blocks, o);
+    });
+    RF_LAUNCH_CHECK();
+    return 0;
+}
+
+}  // extern "C"
