@@ -14,8 +14,6 @@
 #include "common.cuh"
 #include <type_traits>
 
-#define W4_WARPS 8
-
 template <typename T> struct Quad;                       // four neighbouring numbers
 template <> struct Quad<float> {
     static __device__ __forceinline__ void load(const float* p, float* v) {
@@ -256,35 +254,35 @@ __global__ void __launch_bounds__(256) quantize_w4_kernel(const T* weight, long 
     }
 }
 
-// The weights as numbers [N, K]: a warp writes a tile, a lane four runs of eight columns.
+// The weights as numbers, columns lo .. hi - 1 (lo a multiple of 64): a warp writes a tile, a lane four runs of eight columns.
 template <typename T, int G>
-__global__ void __launch_bounds__(256) dequantize_w4_kernel(const uint4* packed, const __nv_bfloat16* scales, T* __restrict__ out, int N, int K, int Kp) {
+__global__ void __launch_bounds__(256) dequantize_w4_kernel(const uint4* packed, const __nv_bfloat16* scales, T* __restrict__ out, int N, int Kp, int lo, int hi) {
     pdl_wait(packed, scales);
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, blocks = Kp / 64;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, blocks = (hi - lo + 63) / 64;
     const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (unit >= (long long)((N + 15) / 16) * blocks) return;
-    const int tile = (int)(unit / blocks), block = (int)(unit % blocks);
-    const uint4 p = packed[(size_t)unit * 32 + lane];
+    const int tile = (int)(unit / blocks), k0 = lo + 64 * (int)(unit % blocks), ld = hi - lo;
+    const uint4 p = packed[((size_t)tile * (Kp / 64) + k0 / 64) * 32 + lane];
     const uint32_t word[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const int n = 16 * tile + g + 8 * r, k = 64 * block + 32 * c + 8 * t;
-            if (n >= N || k >= K) continue;
+            const int n = 16 * tile + g + 8 * r, k = k0 + 32 * c + 8 * t;
+            if (n >= N || k >= hi) continue;
             const float s = __bfloat162float(scales[((size_t)tile * (Kp / G) + k / G) * 16 + 2 * g + r]);
-            T v[8];
+            alignas(16) T v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int i = (int)(word[2 * r + c] >> (8 * (j & 3) + 4 * (j >> 2)) & 15u);
                 v[j] = Cvt<T>::from_f32((float)((i ^ 8) - 8) * s);
             }
-            T* to = out + (size_t)n * K + k;
-            if (K % 8 == 0) {
+            T* to = out + (size_t)n * ld + (k - lo);
+            if (ld % 8 == 0) {
 #pragma unroll
                 for (int j = 0; j < 8 * (int)sizeof(T) / 16; ++j) reinterpret_cast<uint4*>(to)[j] = reinterpret_cast<const uint4*>(v)[j];
             } else {
-                for (int j = 0; j < 8 && k + j < K; ++j) to[j] = v[j];
+                for (int j = 0; j < 8 && k + j < hi; ++j) to[j] = v[j];
             }
         }
 }
@@ -295,72 +293,17 @@ __global__ void __launch_bounds__(256) dequantize_w4_kernel(const uint4* packed,
 __global__ void weights_made_kernel() {}
 
 // ---------------------------------------------------------------- products of few tokens
+// c += A B, A 16 rows by 32 (16) columns of weights, B as many columns by eight tokens.
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-
-enum { W4_STORE = 0, W4_F32 = 1, W4_ADD = 2, W4_PARTIAL = 3 };
-
-struct W4Out {
-    void* out;
-    const void* bias;
-    int bias_is_f32, mode, out_is_f32, M, N;
-};
-__device__ __forceinline__ void w4_write(const W4Out& o, int split, int t, int n, float v) {
-    if (t >= o.M || n >= o.N) return;
-    if (o.mode == W4_PARTIAL) {
-        reinterpret_cast<float*>(o.out)[((size_t)split * o.M + t) * o.N + n] = v;
-        return;
-    }
-    if (o.bias != nullptr) v += load_vec(o.bias, o.bias_is_f32, n);
-    const size_t at = (size_t)t * o.N + n;
-    if (o.mode == W4_ADD) reinterpret_cast<float*>(o.out)[at] += v;
-    else if (o.out_is_f32) reinterpret_cast<float*>(o.out)[at] = v;
-    else reinterpret_cast<__nv_bfloat16*>(o.out)[at] = __float2bfloat16_rn(v);
-}
-
-// What a lane multiplies a tile of weights with: token g's numbers of the lane's columns, in the order in which they lie.
-// 8-bit rows are padded with zeros to whole tiles; 16-bit rows are the caller's, and end at K: WHOLE says that they can be read in 16
-// bytes at a time (8-number runs that lie inside or outside the row as a whole).
-template <typename X, bool WHOLE> struct RowPart;
-template <> struct RowPart<int8_t, true> {
-    uint2 v[2];
-    __device__ __forceinline__ void load(const int8_t* row, int k, int) {
-        v[0] = *reinterpret_cast<const uint2*>(row + k);
-        v[1] = *reinterpret_cast<const uint2*>(row + k + 32);
-    }
-    __device__ __forceinline__ void zero() { v[0] = v[1] = make_uint2(0u, 0u); }
-};
-template <bool WHOLE> struct RowPart<__nv_bfloat16, WHOLE> {
-    uint4 v[2];
-    static __device__ __forceinline__ uint4 eight(const __nv_bfloat16* row, int k, int K) {
-        uint4 r = make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (WHOLE) {
-            if (k < K) r = *reinterpret_cast<const uint4*>(row + k);
-        } else {
-            const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
-            uint32_t two[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                two[i] = (k + 2 * i < K ? p[k + 2 * i] : 0u) | (k + 2 * i + 1 < K ? (uint32_t)p[k + 2 * i + 1] << 16 : 0u);
-            r = make_uint4(two[0], two[1], two[2], two[3]);
-        }
-        return r;
-    }
-    __device__ __forceinline__ void load(const __nv_bfloat16* row, int k, int K) {
-        v[0] = eight(row, k, K);
-        v[1] = eight(row, k + 32, K);
-    }
-    __device__ __forceinline__ void zero() { v[0] = v[1] = make_uint4(0u, 0u, 0u, 0u); }
-};
-
-// c += (rows g, g + 8; the 32 columns of half `half`) times the token's numbers.
-__device__ __forceinline__ void half_tile(int (&c)[4], uint32_t lo_row, uint32_t hi_row, const uint2& x) {
+// c += (rows g, g + 8; 32 columns) times the token's numbers: a word of four bytes a row, eight numbers.
+__device__ __forceinline__ void quarter(int (&c)[4], uint32_t lo_row, uint32_t hi_row, const uint2& x) {
     const uint32_t m = 0xf0f0f0f0u;                      // a half of a byte at its upper end is 16 q as a signed byte
     mma_s8(c, lo_row << 4 & m, hi_row << 4 & m, lo_row & m, hi_row & m, x.x, x.y);
 }
@@ -371,88 +314,274 @@ __device__ __forceinline__ uint32_t two_weights(uint32_t w) {
     __nv_bfloat162 r = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&v), less);
     return *reinterpret_cast<uint32_t*>(&r);
 }
-__device__ __forceinline__ void half_tile(float (&c)[4], uint32_t lo_row, uint32_t hi_row, const uint4& x) {
+__device__ __forceinline__ void quarter(float (&c)[4], uint32_t lo_row, uint32_t hi_row, const uint4& x) {
     // columns (0, 2), (1, 3) and (4, 6), (5, 7) of the eight are 16 bits apart in the word; the row's pairs are put together alike
     mma_bf16(c, two_weights(lo_row), two_weights(hi_row), two_weights(lo_row >> 8), two_weights(hi_row >> 8),
              __byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));
     mma_bf16(c, two_weights(lo_row >> 4), two_weights(hi_row >> 4), two_weights(lo_row >> 12), two_weights(hi_row >> 12),
              __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
 }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {       // zeros if it is not there
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ unsigned long long two(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add_two(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul_two(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma_two(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 
-// Eight tokens (blockIdx.z) by a tile of 16 rows: the block's warps share out the columns of its split.  A warp asks for four tiles of
-// 64 columns at a time, the next four while it multiplies; nothing passes through shared memory but the warps' sums, as no number of
-// a row is used by two warps.
-template <int G, typename X, bool WHOLE>
-__global__ void __launch_bounds__(32 * W4_WARPS) w4_eight_kernel(const uint4* __restrict__ w0, const uint32_t* __restrict__ w1, const X* x,
-                                                               const float* xs, long long ldx, int K, int blocks, W4Out o) {
-    using Sum = typename std::conditional<std::is_same<X, int8_t>::value, int, float>::type;
+struct W4Out {
+    void* out;               // [M, N] float32 if is_f32, else bfloat16; add: float32, added into
+    const void* bias;        // [N] or null
+    int bias_is_f32, is_f32, add, M, N;
+};
+__device__ __forceinline__ void w4_write(const W4Out& o, int t, int n, float v) {
+    if (n >= o.N) return;
+    if (o.bias != nullptr) v += load_vec(o.bias, o.bias_is_f32, n);
+    const size_t at = (size_t)t * o.N + n;
+    if (o.add) reinterpret_cast<float*>(o.out)[at] += v;
+    else if (o.is_f32) reinterpret_cast<float*>(o.out)[at] = v;
+    else reinterpret_cast<__nv_bfloat16*>(o.out)[at] = __float2bfloat16_rn(v);
+}
+
+// 8 NB tokens (blockIdx.y) by tiles of 16 rows, one block of 16 warps an SM for as long as there are tiles.  The numbers of the block's
+// tokens lie in shared memory from the start (a cluster's CTAs have a share of the columns each, so that they fit), and their scales.  A
+// warp goes through its tiles in units of 128 columns (1 KB of weights), which asynchronous copies bring into a ring of its own, DEPTH
+// units ahead and without regard to where a row of tiles ends; a lane reads back what it has copied itself (but for the scales).  No
+// warp waits for another but once a round, when `ways` warps (and the cluster's CTAs) add up what they have of a tile, and not even then
+// where a tile is one warp's.
+// A group's (at most 128 columns') exact sum is formed by the tensor cores in whole numbers and added up in 32 bits; the whole number starts
+// at 1.5 2^23 as a float's bits, so that its bits are that float plus the sum (below 2^22: 128 columns of 16 * 8 * 127), and no conversion is
+// needed.
+#define W4_WARPS 16
+#define W4_SLOT (1024 + 128)                             // a unit's weights, and its scales [group][16 rows]
+#define W4_SUMS (16 * W4_WARPS + 4)                      // pitch of the warps' sums [token][16 rows a warp]
+// Shared memory of a block: tokens' numbers (rows a pitch apart by which eight tokens' reads meet every bank once), their scales
+// [group][token], the warps' sums (two sets for a cluster), the rings.
+struct W4Shared {
+    int columns, pitch, scales, sums, ring, bytes;
+};
+__host__ __device__ constexpr int w4_depth(int nb) { return nb == 1 ? 6 : nb == 2 ? 4 : 3; }
+__host__ __device__ inline W4Shared w4_shared(int units, int splits, int G, int size, int M, int nb) {
+    W4Shared s;
+    s.columns = (units + splits - 1) / splits * 128;
+    s.pitch = s.columns * size + (size == 1 ? 32 : 64);
+    s.scales = (M < 8 * nb ? M : 8 * nb) * s.pitch;
+    s.sums = s.scales + (size == 1 ? s.columns / G * 8 * nb * 4 : 0);
+    s.ring = s.sums + (splits > 1 ? 2 : 1) * 8 * nb * W4_SUMS * 4;
+    s.bytes = s.ring + W4_WARPS * w4_depth(nb) * W4_SLOT;
+    return s;
+}
+
+template <int G, typename X, int NB>
+__global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint4* __restrict__ w0, const uint32_t* __restrict__ w1, const X* x,
+                                                                      const float* xs, long long ldx, int whole, int K, int blocks, int ways, int splits, W4Out o) {
     constexpr bool BYTES = std::is_same<X, int8_t>::value;
-    constexpr int D = 4;
+    constexpr int DEPTH = w4_depth(NB), GROUPS = 128 / G, QUARTERS = G / 32, THREADS = 32 * W4_WARPS;
+    extern __shared__ __align__(128) uint8_t smem[];
     pdl_trigger();
+    const int units = (blocks + 1) / 2, all_groups = blocks * 64 / G;
+    const W4Shared sh = w4_shared(units, splits, G, (int)sizeof(X), o.M, NB);
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int slices = gridDim.y * W4_WARPS, slice = blockIdx.y * W4_WARPS + warp;
-    const int from = (int)((long long)blocks * slice / slices), to = (int)((long long)blocks * (slice + 1) / slices);
-    const uint4* wt = w0 + (size_t)blockIdx.x * blocks * 32 + lane;
-    const int groups = blocks * 64 / G;
-    const uint32_t* st = w1 + (size_t)blockIdx.x * groups * 8 + g;
-    uint4 w[D];
-#pragma unroll
-    for (int i = 0; i < D; ++i)
-        if (from + i < to) w[i] = wt[(size_t)(from + i) * 32];
-    pdl_wait(x, xs);
-    const int tok = blockIdx.z * 8 + g, ta = blockIdx.z * 8 + 2 * t;
-    const bool mine = tok < o.M, has_a = ta < o.M, has_b = ta + 1 < o.M;
-    const X* xrow = x + (size_t)tok * ldx;
-    float acc[4] = {};
-    for (int b = from; b < to; b += D) {
-        uint4 next[D];
-        RowPart<X, WHOLE> rows[D];
-#pragma unroll
-        for (int i = 0; i < D; ++i) {
-            if (b + D + i < to) next[i] = wt[(size_t)(b + D + i) * 32];
-            if (mine && b + i < to) rows[i].load(xrow, 64 * (b + i) + 8 * t, K);
-            else rows[i].zero();
-        }
-#pragma unroll
-        for (int i = 0; i < D; ++i) {
-            if (b + i >= to) break;
-            Sum c[4] = {};
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                half_tile(c, half ? w[i].y : w[i].x, half ? w[i].w : w[i].z, rows[i].v[half]);
-                if (G == 32 || half == 1) {
-                    const int group = (64 * (b + i) + 32 * half) / G;
-                    const uint32_t s2 = st[(size_t)group * 8];
-                    float s0 = __uint_as_float(s2 << 16), s1 = __uint_as_float(s2 & 0xffff0000u);
-                    float a0 = 1.f, a1 = 1.f;
-                    if constexpr (BYTES) {
-                        s0 *= 0.0625f; s1 *= 0.0625f;    // the products hold 16 q
-                        a0 = has_a ? xs[(size_t)ta * groups + group] : 0.f;
-                        a1 = has_b ? xs[(size_t)(ta + 1) * groups + group] : 0.f;
-                    }
-                    acc[0] += (float)c[0] * (s0 * a0);
-                    acc[1] += (float)c[1] * (s0 * a1);
-                    acc[2] += (float)c[2] * (s1 * a0);
-                    acc[3] += (float)c[3] * (s1 * a1);
-                    c[0] = c[1] = c[2] = c[3] = 0;
-                }
+    const int rank = blockIdx.x % splits, cluster = blockIdx.x / splits, clusters = gridDim.x / splits;
+    const int tiles = (o.N + 15) / 16, at_once = W4_WARPS / ways, rounds = (tiles + clusters * at_once - 1) / (clusters * at_once);
+    const int tok0 = blockIdx.y * 8 * NB, live = min(8 * NB, o.M - tok0);
+    const int first = (int)((long long)units * rank / splits), count = (int)((long long)units * (rank + 1) / splits) - first;
+    const int from = first + count * (warp % ways) / ways, to = first + count * (warp % ways + 1) / ways;
+    auto tile_of = [&](int round) { return (round * clusters + cluster) * at_once + warp / ways; };
+    // the unit that is asked for next, and the ring
+    int ask_round = from < to && tile_of(0) < tiles ? 0 : rounds, ask_unit = from;
+    const uint32_t ring = base + sh.ring + warp * DEPTH * W4_SLOT;
+    int slot = 0;
+    auto ask = [&](int into) {
+        if (ask_round < rounds) {
+            const int tile = tile_of(ask_round);
+            const uint32_t to_here = ring + into * W4_SLOT;
+            const uint4* p = w0 + ((size_t)tile * blocks + 2 * ask_unit) * 32 + lane;
+            copy16(to_here + 16 * lane, p, true);
+            const bool second = 2 * ask_unit + 1 < blocks;
+            copy16(to_here + 512 + 16 * lane, second ? p + 32 : p, second);
+            if (t < GROUPS) {
+                const int group = ask_unit * GROUPS + t;
+                const uint32_t* s = w1 + (size_t)tile * all_groups * 8 + g;
+                copy4(to_here + 1024 + (8 * t + g) * 4, group < all_groups ? s + (size_t)group * 8 : s, group < all_groups);
+            }
+            if (++ask_unit == to) {
+                ask_unit = from;
+                if (tile_of(++ask_round) >= tiles) ask_round = rounds;
             }
         }
-#pragma unroll
-        for (int i = 0; i < D; ++i) w[i] = next[i];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int i = 0; i < DEPTH; ++i) ask(i);
+    pdl_wait(x, xs);
+    if (whole) {
+        constexpr int EACH = 16 / (int)sizeof(X);
+        for (int tok = warp; tok < live; tok += W4_WARPS) {
+            const X* row = x + (size_t)(tok0 + tok) * ldx;
+            for (int i = lane; i < count * 128 / EACH; i += 32) {
+                const int k = first * 128 + i * EACH;
+                const bool there = k < (BYTES ? 64 * blocks : K);       // (16-bit rows end at K, 8-bit ones are padded with zeros)
+                copy16(base + tok * sh.pitch + 16 * i, there ? row + k : x, there);
+            }
+        }
+    } else {
+        for (int tok = warp; tok < live; tok += W4_WARPS) {
+            const X* row = x + (size_t)(tok0 + tok) * ldx;
+            X* mine = reinterpret_cast<X*>(smem + tok * sh.pitch);
+            for (int i = lane; i < count * 128; i += 32) mine[i] = first * 128 + i < K ? row[first * 128 + i] : static_cast<X>(0.f);
+        }
     }
-    __shared__ float part[W4_WARPS][8][17];              // [warp][token][row]
-    part[warp][2 * t][g] = acc[0];
-    part[warp][2 * t + 1][g] = acc[1];
-    part[warp][2 * t][g + 8] = acc[2];
-    part[warp][2 * t + 1][g + 8] = acc[3];
+    if constexpr (BYTES) {
+        const int here = count * GROUPS;
+        for (int i = threadIdx.x; i < here * live; i += THREADS) {
+            const int tok = i / here, gr = i - tok * here;
+            const bool there = first * GROUPS + gr < all_groups;
+            copy4(base + sh.scales + (gr * 8 * NB + tok) * 4, there ? xs + (size_t)(tok0 + tok) * all_groups + first * GROUPS + gr : xs, there);
+        }
+    }
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    if (threadIdx.x < 128) {
-        const int token = threadIdx.x >> 4, row = threadIdx.x & 15;
-        float v = part[0][token][row];
+    float* sums = reinterpret_cast<float*>(smem + sh.sums);
+    const uint8_t* rows[NB];                             // (a token that is not there reads another's numbers: its sums are not written)
 #pragma unroll
-        for (int i = 1; i < W4_WARPS; ++i) v += part[i][token][row];
-        w4_write(o, blockIdx.y, blockIdx.z * 8 + token, blockIdx.x * 16 + row, v);
+    for (int nb = 0; nb < NB; ++nb) rows[nb] = smem + min(8 * nb + g, live - 1) * sh.pitch + 8 * t * (int)sizeof(X);
+    const float* scales = reinterpret_cast<const float*>(smem + sh.scales) + 2 * t;
+    unsigned long long acc[NB][2] = {};                  // [eight tokens][row g, g + 8] of two tokens
+
+    // a round's sums, over the warps of a tile and the CTAs of the cluster in order; every CTA writes a share
+    auto write_round = [&](int round) {
+        const float* at = sums + (splits > 1 ? round & 1 : 0) * 8 * NB * W4_SUMS;
+        const int rows_here = 16 * at_once, n0 = (round * clusters + cluster) * rows_here;
+        for (int i = rank * THREADS + threadIdx.x; i < live * rows_here; i += splits * THREADS) {
+            const int tok = i / rows_here, r = i - tok * rows_here;
+            const float* p = at + tok * W4_SUMS + r / 16 * ways * 16 + r % 16;
+            float v = 0.f;
+            if (splits == 1) {
+                for (int k = 0; k < ways; ++k) v += p[16 * k];
+            } else {
+                const uint32_t here = (uint32_t)__cvta_generic_to_shared(p);
+                for (int c = 0; c < splits; ++c) {
+                    uint32_t there;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(c));
+                    for (int k = 0; k < ways; ++k) {
+                        float f;
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there + 64 * k) : "memory");
+                        v += f;
+                    }
+                }
+            }
+            w4_write(o, tok0 + tok, n0 + r, v);
+        }
+    };
+
+    for (int round = 0; round < rounds; ++round) {
+        if (tile_of(round) < tiles)
+            for (int u = from; u < to; ++u) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+                __syncwarp();
+                const uint8_t* here = smem + sh.ring + (warp * DEPTH + slot) * W4_SLOT;
+                const uint4 wa = *reinterpret_cast<const uint4*>(here + 16 * lane), wb = *reinterpret_cast<const uint4*>(here + 512 + 16 * lane);
+                float sw[GROUPS][2];
+#pragma unroll
+                for (int p = 0; p < GROUPS; ++p) {
+                    const uint32_t s2 = *reinterpret_cast<const uint32_t*>(here + 1024 + (8 * p + g) * 4);
+                    sw[p][0] = __uint_as_float(s2 << 16); sw[p][1] = __uint_as_float(s2 & 0xffff0000u);
+                    if (BYTES) { sw[p][0] *= 0.0625f; sw[p][1] *= 0.0625f; }              // the products hold 16 q
+                }
+                __syncwarp();                            // all have read the slot
+                ask(slot);
+                slot = slot + 1 == DEPTH ? 0 : slot + 1;
+                const uint32_t lo[4] = {wa.x, wa.y, wb.x, wb.y}, hi[4] = {wa.z, wa.w, wb.z, wb.w};
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const uint8_t* row = rows[nb] + 128 * (u - first) * (int)sizeof(X);
+                    if constexpr (BYTES) {
+                        int c[GROUPS][4];
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            int (&part)[4] = c[h / QUARTERS];
+                            if (h % QUARTERS == 0) part[0] = part[1] = part[2] = part[3] = 0x4b400000;
+                            quarter(part, lo[h], hi[h], *reinterpret_cast<const uint2*>(row + 32 * h));
+                        }
+#pragma unroll
+                        for (int p = 0; p < GROUPS; ++p) {
+                            const float2 a = *reinterpret_cast<const float2*>(scales + ((u - first) * GROUPS + p) * 8 * NB + 8 * nb);
+                            const unsigned long long xa = two(a.x, a.y), less = two(-12582912.f, -12582912.f);
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                acc[nb][e] = fma_two(add_two(two(__int_as_float(c[p][2 * e]), __int_as_float(c[p][2 * e + 1])), less),
+                                                     mul_two(xa, two(sw[p][e], sw[p][e])), acc[nb][e]);
+                        }
+                    } else {
+                        float c[GROUPS][4];
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            float (&part)[4] = c[h / QUARTERS];
+                            if (h % QUARTERS == 0) part[0] = part[1] = part[2] = part[3] = 0.f;
+                            quarter(part, lo[h], hi[h], *reinterpret_cast<const uint4*>(row + 64 * h));
+                        }
+#pragma unroll
+                        for (int p = 0; p < GROUPS; ++p)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                acc[nb][e] = fma_two(two(c[p][2 * e], c[p][2 * e + 1]), two(sw[p][e], sw[p][e]), acc[nb][e]);
+                    }
+                }
+            }
+        if (splits > 1 && round > 0) {
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            write_round(round - 1);
+        }
+        if (splits == 1 && ways > 1 && round > 0) __syncthreads();              // the sums of the round before are read
+        float* to_a = sums + ((splits > 1 ? round & 1 : 0) * 8 * NB + 2 * t) * W4_SUMS + 16 * warp + g;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float a, c;
+                asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(c) : "l"(acc[nb][e]));
+                to_a[8 * nb * W4_SUMS + 8 * e] = a;
+                to_a[(8 * nb + 1) * W4_SUMS + 8 * e] = c;
+                acc[nb][e] = 0ull;
+            }
+        if (splits > 1) {
+            // two sets of sums in turn: who writes a set for the second time knows, by the barrier between, that all have read the first
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        } else if (ways > 1) {
+            __syncthreads();
+            write_round(round);
+        } else {                                         // the warp's own tile: half the warp has a token's 16 rows
+            __syncwarp();
+            const int n = tile_of(round) * 16 + lane % 16;
+            for (int tok = lane / 16; tok < live; tok += 2) w4_write(o, tok0 + tok, n, sums[tok * W4_SUMS + 16 * warp + lane % 16]);
+            __syncwarp();
+        }
+    }
+    if (splits > 1) {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        write_round(rounds - 1);
+        // a CTA's shared memory stays until its peers have read it
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
 }
 
@@ -522,6 +651,30 @@ static int launch_add_rmsnorm_q8(float* h, const void* pending, int kind, int n_
     return 0;
 }
 
+// f(group, rows, eights) with the constants and types of a product's kernel
+template <typename F>
+static void with_product(int x_kind, int G, int eights, F f) {
+    with_group(G, [&](auto gc) {
+        auto with_rows = [&](auto rows) {
+            if (eights == 1) f(gc, rows, std::integral_constant<int, 1>());
+            else if (eights == 2) f(gc, rows, std::integral_constant<int, 2>());
+            else f(gc, rows, std::integral_constant<int, 4>());
+        };
+        if (x_kind == 0) with_rows(static_cast<const int8_t*>(nullptr));
+        else with_rows(static_cast<const __nv_bfloat16*>(nullptr));
+    });
+}
+template <int G, typename X, int NB>
+static int set_shared() {                                // the kernel's limit of shared memory, once a device
+    static PerDevice<bool> set;
+    bool& done = set.here();
+    if (done) return 0;
+    const cudaError_t e = cudaFuncSetAttribute(w4_product_kernel<G, X, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    done = e == cudaSuccess;
+    return (int)e;
+}
+#define W4_MOST_SHARED (227 * 1024)
+
 extern "C" {
 
 // x [T, K] (rows ldx apart) -> q int8 [T, Kp], scales float32 [T, Kp / G]; Kp: K up to a multiple of 64 (128 if G is).
@@ -582,16 +735,16 @@ int rf_quantize_w4(int dtype, const void* weight, long long ldw, void* packed, v
     return 0;
 }
 
-int rf_dequantize_w4(int dtype, const void* packed, const void* scales, void* out, int N, int K, int G, cudaStream_t st) {
-    if (N <= 0 || K <= 0 || bad_group(G)) return RF_ERR_BAD_ARG;
+int rf_dequantize_w4(int dtype, const void* packed, const void* scales, void* out, int N, int K, int lo, int hi, int G, cudaStream_t st) {
+    if (N <= 0 || K <= 0 || bad_group(G) || lo < 0 || lo % 64 || hi <= lo || hi > K || !aligned(out, 16)) return RF_ERR_BAD_ARG;
     const int Kp = padded(K, G);
-    const long long units = (long long)((N + 15) / 16) * (Kp / 64);
+    const long long units = (long long)((N + 15) / 16) * ((hi - lo + 63) / 64);
     if ((units + 7) / 8 > 0x7fffffffll) return RF_ERR_UNSUPPORTED;
     with_group(G, [&](auto gc) {
         constexpr int GC = decltype(gc)::value;
         const dim3 grid((unsigned)((units + 7) / 8));
-        if (dtype == 0) rf_launch(dequantize_w4_kernel<float, GC>, grid, dim3(256), 0, st, (const uint4*)packed, (const __nv_bfloat16*)scales, (float*)out, N, K, Kp);
-        else rf_launch(dequantize_w4_kernel<__nv_bfloat16, GC>, grid, dim3(256), 0, st, (const uint4*)packed, (const __nv_bfloat16*)scales, (__nv_bfloat16*)out, N, K, Kp);
+        if (dtype == 0) rf_launch(dequantize_w4_kernel<float, GC>, grid, dim3(256), 0, st, (const uint4*)packed, (const __nv_bfloat16*)scales, (float*)out, N, Kp, lo, hi);
+        else rf_launch(dequantize_w4_kernel<__nv_bfloat16, GC>, grid, dim3(256), 0, st, (const uint4*)packed, (const __nv_bfloat16*)scales, (__nv_bfloat16*)out, N, Kp, lo, hi);
     });
     weights_made_kernel<<<1, 32, 0, st>>>();
     RF_LAUNCH_CHECK();
@@ -605,28 +758,56 @@ int rf_weights_made(cudaStream_t st) {
     return 0;
 }
 
-// out = x w^T (+ bias): x_kind 0: 8-bit rows (x int8 [M, Kp], xs float32 [M, Kp / G]), 1: bfloat16 rows [M, K], ldx apart.  mode W4_STORE (float32 if out_is_f32, else bfloat16), W4_ADD (out float32 += ...), W4_PARTIAL (float32
-// [splits, M, N], no bias); splits > 1 with W4_PARTIAL only.
+// Bytes of shared memory that a product's block takes with `eights` eights of tokens and a share of the columns in `splits`.
+int rf_gemm_w4_shared(int x_kind, int M, int K, int G, int eights, int splits) {
+    return w4_shared((padded(K, G) / 64 + 1) / 2, splits, G, x_kind == 0 ? 1 : 2, M, eights).bytes;
+}
+
+// Clusters of `splits` blocks, each with an SM of its own, that run at once on the current device (< 0: an error).
+int rf_gemm_w4_clusters(int splits) {
+    if (splits < 1 || splits > 8) return RF_ERR_BAD_ARG;
+    if (const int e = set_shared<128, int8_t, 1>()) return -e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits);
+    cfg.blockDim = dim3(32 * W4_WARPS);
+    cfg.dynamicSmemBytes = W4_MOST_SHARED;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, w4_product_kernel<128, int8_t, 1>, &cfg);
+    return e == cudaSuccess ? n : -(int)e;
+}
+
+// out = x w^T (+ bias): x_kind 0: 8-bit rows (x int8 [M, Kp], xs float32 [M, Kp / G]), 1: bfloat16 rows [M, K], ldx apart; out as W4Out
+// has it.  eights: eights of tokens a block (1, 2, 4); ways: warps a tile (a power of two up to 16); splits: CTAs of a cluster that share
+// out the columns (1 .. 8); clusters: of each share of tokens.
 int rf_gemm_w4(int x_kind, const void* x, const void* xs, long long ldx, const void* packed, const void* scales, const void* bias, int bias_is_f32,
-               void* out, int out_is_f32, int mode, int splits, int M, int N, int K, int G, cudaStream_t st) {
-    if (M <= 0 || N <= 0 || K <= 0 || bad_group(G) || splits < 1 || splits > 65535 || (splits > 1 && mode != W4_PARTIAL) || mode < 0 || mode > 3) return RF_ERR_BAD_ARG;
-    if ((x_kind == 0 && (!aligned(x, 8) || ldx % 8)) || !aligned(packed, 16) || !aligned(scales, 4)) return RF_ERR_BAD_ARG;
-    const bool whole = K % 8 == 0 && ldx % 8 == 0 && aligned(x, 16);
-    const int blocks = padded(K, G) / 64;
-    if ((M + 7) / 8 > 65535) return RF_ERR_UNSUPPORTED;
-    const W4Out o{out, bias, bias_is_f32, mode, out_is_f32, M, N};
-    with_group(G, [&](auto gc) {
-        constexpr int GC = decltype(gc)::value;
-        const dim3 grid((N + 15) / 16, splits, (M + 7) / 8);
-        const uint4* w0 = (const uint4*)packed;
-        const uint32_t* w1 = (const uint32_t*)scales;
-        const __nv_bfloat16* x16 = (const __nv_bfloat16*)x;
-        const float* none = nullptr;
-        const dim3 block(32 * W4_WARPS);
-        if (x_kind == 0) rf_launch(w4_eight_kernel<GC, int8_t, true>, grid, block, 0, st, w0, w1, (const int8_t*)x, (const float*)xs, ldx, K, blocks, o);
-        else if (whole) rf_launch(w4_eight_kernel<GC, __nv_bfloat16, true>, grid, block, 0, st, w0, w1, x16, none, ldx, K, blocks, o);
-        else rf_launch(w4_eight_kernel<GC, __nv_bfloat16, false>, grid, block, 0, st, w0, w1, x16, none, ldx, K, blocks, o);
+               void* out, int out_is_f32, int add, int eights, int ways, int splits, int clusters, int M, int N, int K, int G, cudaStream_t st) {
+    if (M <= 0 || N <= 0 || K <= 0 || bad_group(G) || (add && !out_is_f32)) return RF_ERR_BAD_ARG;
+    if ((x_kind == 0 && (!aligned(x, 16) || ldx % 16)) || !aligned(packed, 16) || !aligned(scales, 16)) return RF_ERR_BAD_ARG;
+    if (splits < 1 || splits > 8 || clusters < 1 || ways < 1 || ways > W4_WARPS || (ways & (ways - 1)) || (eights != 1 && eights != 2 && eights != 4)) return RF_ERR_BAD_ARG;
+    const int whole = x_kind == 0 || (K % 8 == 0 && ldx % 8 == 0 && aligned(x, 16));
+    const int blocks = padded(K, G) / 64, smem = rf_gemm_w4_shared(x_kind, M, K, G, eights, splits);
+    const long long y = (M + 8ll * eights - 1) / (8 * eights);
+    if (smem > W4_MOST_SHARED || y > 65535 || (long long)clusters * splits > 0x7fffffffll) return RF_ERR_UNSUPPORTED;
+    const W4Out o{out, bias, bias_is_f32, out_is_f32, add, M, N};
+    int bad = 0;
+    with_product(x_kind, G, eights, [&](auto gc, auto rows, auto nb) {
+        using X = std::remove_cv_t<std::remove_pointer_t<decltype(rows)>>;
+        constexpr int GC = decltype(gc)::value, NB = decltype(nb)::value;
+        bad = set_shared<GC, X, NB>();
+        if (bad) return;
+        const dim3 grid(clusters * splits, (unsigned)y), block(32 * W4_WARPS);
+        auto go = [&](auto... args) {
+            if (splits > 1) rf_launch_cluster(w4_product_kernel<GC, X, NB>, grid, block, smem, st, splits, args...);
+            else rf_launch(w4_product_kernel<GC, X, NB>, grid, block, smem, st, args...);
+        };
+        go((const uint4*)packed, (const uint32_t*)scales, (const X*)x, (const float*)xs, ldx, whole, K, blocks, ways, splits, o);
     });
+    if (bad) return bad;
     RF_LAUNCH_CHECK();
     return 0;
 }

@@ -2,6 +2,8 @@
 
 maeddesg/ROCmForge keeps its quantised weights as the GGUF file has them and multiplies Q4 blocks with Q8 rows while it decodes
 (src/gpu/ops.rs:455-747); here weights are quantised once, when a model is made, into the layout that the kernels read.
+
+The calls of a decode step are as short on the device as a launch is on the host, so the checks build no text unless they fail.
 """
 from __future__ import annotations
 
@@ -10,33 +12,57 @@ import functools
 import torch
 
 from . import tensor_core as tc
-from ._ffi import KernelError, c_float, c_int, c_ll, c_void_p, check, dtype_code, fn, need, need_cuda, ptr, stream
+from ._ffi import KernelError, c_float, c_int, c_ll, c_void_p, check, dtype_code, fn, need, need_cuda, ptr, sm_count, stream
 
 W4_GROUPS = (32, 64, 128)
-W4_STORE, W4_ADD, W4_PARTIAL = 0, 2, 3
+W4_MOST_SHARED = 227 * 1024
+_p, _i, _n = c_void_p, c_int, c_ll
+_LAUNCHERS = {
+    "rf_quantize_q8": [_i, _p, _n, _p, _p, _i, _i, _i, _p],
+    "rf_dequantize_q8": [_i, _p, _p, _p, _i, _i, _i, _p],
+    "rf_swiglu_q8": [_i, _p, _i, _p, _p, _i, _i, _i, _p],
+    "rf_add_rmsnorm_q8": [_i, _p, _p, _i, _i, _n, _p, _i, c_float, _p, _p, _p, _i, _i, _i, _i, _p],
+    "rf_quantize_w4": [_i, _p, _n, _p, _p, _i, _i, _i, _p],
+    "rf_dequantize_w4": [_i, _p, _p, _p, _i, _i, _i, _i, _i, _p],
+    "rf_weights_made": [_p],
+    "rf_gemm_w4_shared": [_i, _i, _i, _i, _i, _i],
+    "rf_gemm_w4_clusters": [_i],
+    "rf_gemm_w4": [_i, _p, _p, _n, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p],
+}
 
 
 @functools.lru_cache(None)
-def _f(name, *argtypes):
-    return fn("quantized", name, list(argtypes))
+def _f(name: str):
+    return fn("quantized", name, _LAUNCHERS[name])
 
 
 def padded_columns(K: int, group: int) -> int:
     """Columns that the stored forms of a row of ``K`` take: whole tiles of 64 and whole groups."""
-    unit = max(64, group)
+    unit = 128 if group == 128 else 64
     return (K + unit - 1) // unit * unit
 
 
 def _need_group(group, what: str) -> None:
-    need(group in W4_GROUPS, f"{what}: groups of {group} (known: {W4_GROUPS})")
+    if group not in W4_GROUPS:
+        raise KernelError(f"{what}: groups of {group} (known: {W4_GROUPS})")
+
+
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _need_here(what: str, *tensors) -> None:
     """Every tensor on the current device, whose stream the launch goes to."""
-    need_cuda(*tensors)
-    here = torch.cuda.current_device()
+    here = -2
     for t in tensors:
-        need(t is None or t.device.index == here, f"{what}: a tensor on {None if t is None else t.device}, the current device is cuda:{here}")
+        if t is None:
+            continue
+        at = t.get_device()
+        if at < 0:
+            need_cuda(t)
+        if here == -2:
+            here = _device()
+        if at != here:
+            raise KernelError(f"{what}: a tensor on cuda:{at}, the current device is cuda:{here}")
 
 
 class Q8Rows:
@@ -45,16 +71,32 @@ class Q8Rows:
     ``q`` int8 [T, padded_columns(K, group)] with zeros from column K on, ``scales`` float32 [T, padded columns / group]; ``dtype`` is that
     of the rows they stand for, in which ``materialize`` gives them back and a product's result comes."""
 
+    __slots__ = ("q", "scales", "K", "group", "dtype")
+
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, K: int, group: int, dtype: torch.dtype):
         _need_group(group, "Q8Rows")
         Kp = padded_columns(K, group)
-        need(q.dtype == torch.int8 and q.dim() == 2 and q.shape[1] == Kp and q.is_contiguous(), f"Q8Rows: q must be int8 [T, {Kp}]")
-        need(scales.dtype == torch.float32 and tuple(scales.shape) == (q.shape[0], Kp // group) and scales.is_contiguous(),
-             f"Q8Rows: scales must be float32 [T, {Kp // group}]")
-        need(q.device == scales.device, "Q8Rows: q and scales must be on one device")
+        if not (K > 0 and q.dtype == torch.int8 and q.dim() == 2 and q.shape[1] == Kp and q.is_contiguous() and q.data_ptr() % 16 == 0):
+            raise KernelError(f"Q8Rows: q must be int8 [T, {Kp}], aligned to 16 bytes")
+        if not (scales.dtype == torch.float32 and scales.shape == (q.shape[0], Kp // group) and scales.is_contiguous()):
+            raise KernelError(f"Q8Rows: scales must be float32 [T, {Kp // group}]")
+        need(q.get_device() == scales.get_device(), "Q8Rows: q and scales must be on one device")
         dtype_code(dtype)
-        self.q, self.scales, self.K, self.group, self.dtype = q, scales, int(K), int(group), dtype
-        self.shape = torch.Size((q.shape[0], int(K)))
+        self.q, self.scales, self.K, self.group, self.dtype = q, scales, K, group, dtype
+
+    @classmethod
+    def empty(cls, T: int, K: int, group: int, dtype: torch.dtype, device) -> "Q8Rows":
+        """Rows that a kernel is about to fill."""
+        Kp = padded_columns(K, group)
+        r = cls.__new__(cls)
+        r.q = torch.empty((T, Kp), dtype=torch.int8, device=device)
+        r.scales = torch.empty((T, Kp // group), dtype=torch.float32, device=device)
+        r.K, r.group, r.dtype = K, group, dtype
+        return r
+
+    @property
+    def shape(self):
+        return torch.Size((self.q.shape[0], self.K))
 
     @property
     def device(self):
@@ -62,12 +104,12 @@ class Q8Rows:
 
     def materialize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The rows as an ordinary tensor [T, K]."""
-        dtype = dtype or self.dtype
-        _need_here("Q8Rows.materialize", self.q, self.scales)
-        T, K = self.shape
-        out = torch.empty((T, K), dtype=dtype, device=self.device)
-        f = _f("rf_dequantize_q8", c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p)
-        check(f(dtype_code(dtype), ptr(self.q), ptr(self.scales), ptr(out), T, K, self.group, stream()), "Q8Rows.materialize")
+        q, dtype = self.q, dtype or self.dtype
+        _need_here("Q8Rows.materialize", q)
+        T, K = q.shape[0], self.K
+        out = torch.empty((T, K), dtype=dtype, device=q.device)
+        check(_f("rf_dequantize_q8")(dtype_code(dtype), q.data_ptr(), self.scales.data_ptr(), out.data_ptr(), T, K, self.group, stream()),
+              "Q8Rows.materialize")
         return out
 
 
@@ -79,18 +121,23 @@ class W4Weight:
     groups, 16]: entry [2 g + r] is row g + 8 r.  Rows and columns are padded with zeros.  Products read both before they wait for the
     kernel launched before them: whoever writes them with kernels of its own calls ``weights_made`` afterwards."""
 
+    __slots__ = ("packed", "scales", "N", "K", "group")
+
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, N: int, K: int, group: int):
         _need_group(group, "W4Weight")
         need(N > 0 and K > 0, "W4Weight: an empty weight")
         Kp, tiles = padded_columns(K, group), (N + 15) // 16
-        need(packed.dtype == torch.uint8 and tuple(packed.shape) == (tiles, Kp // 64, 32, 16) and packed.is_contiguous(),
-             f"W4Weight: packed must be uint8 [{tiles}, {Kp // 64}, 32, 16]")
-        need(scales.dtype == torch.bfloat16 and tuple(scales.shape) == (tiles, Kp // group, 16) and scales.is_contiguous(),
-             f"W4Weight: scales must be bfloat16 [{tiles}, {Kp // group}, 16]")
-        need(packed.device == scales.device, "W4Weight: packed and scales must be on one device")
-        need(packed.data_ptr() % 16 == 0 and scales.data_ptr() % 4 == 0, "W4Weight: packed must be aligned to 16 bytes, scales to 4")
-        self.packed, self.scales, self.N, self.K, self.group = packed, scales, int(N), int(K), int(group)
-        self.shape = torch.Size((int(N), int(K)))
+        if not (packed.dtype == torch.uint8 and packed.shape == (tiles, Kp // 64, 32, 16) and packed.is_contiguous()):
+            raise KernelError(f"W4Weight: packed must be uint8 [{tiles}, {Kp // 64}, 32, 16]")
+        if not (scales.dtype == torch.bfloat16 and scales.shape == (tiles, Kp // group, 16) and scales.is_contiguous()):
+            raise KernelError(f"W4Weight: scales must be bfloat16 [{tiles}, {Kp // group}, 16]")
+        need(packed.get_device() == scales.get_device(), "W4Weight: packed and scales must be on one device")
+        need(packed.data_ptr() % 16 == 0 and scales.data_ptr() % 16 == 0, "W4Weight: packed and scales must be aligned to 16 bytes")
+        self.packed, self.scales, self.N, self.K, self.group = packed, scales, N, K, group
+
+    @property
+    def shape(self):
+        return torch.Size((self.N, self.K))
 
     @property
     def device(self):
@@ -127,7 +174,7 @@ class W4Weight:
 
 def weights_made() -> None:
     """Products on the current stream may from here on read weights that the stream's last kernels have made."""
-    check(_f("rf_weights_made", c_void_p)(stream()), "weights_made")
+    check(_f("rf_weights_made")(stream()), "weights_made")
 
 
 def quantize_w4(weight: torch.Tensor, group: int = 128) -> W4Weight:
@@ -141,24 +188,20 @@ def quantize_w4(weight: torch.Tensor, group: int = 128) -> W4Weight:
     Kp, tiles = padded_columns(K, group), (N + 15) // 16
     packed = torch.empty((tiles, Kp // 64, 32, 16), dtype=torch.uint8, device=weight.device)
     scales = torch.empty((tiles, Kp // group, 16), dtype=torch.bfloat16, device=weight.device)
-    f = _f("rf_quantize_w4", c_int, c_void_p, c_ll, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p)
-    check(f(dtype_code(weight.dtype), ptr(weight), weight.stride(0), ptr(packed), ptr(scales), N, K, group, stream()), f"quantize_w4 ({N}x{K})")
+    check(_f("rf_quantize_w4")(dtype_code(weight.dtype), ptr(weight), weight.stride(0), ptr(packed), ptr(scales), N, K, group, stream()),
+          f"quantize_w4 ({N}x{K})")
     return W4Weight(packed, scales, N, K, group)
 
 
-def dequantize_w4(w: W4Weight, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The weights as a tensor [N, K]; products may read it at once."""
-    _need_here("dequantize_w4", w.packed, w.scales)
-    out = torch.empty(w.shape, dtype=dtype, device=w.device)
-    f = _f("rf_dequantize_w4", c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p)
-    check(f(dtype_code(dtype), ptr(w.packed), ptr(w.scales), ptr(out), w.N, w.K, w.group, stream()), f"dequantize_w4 ({w.N}x{w.K})")
+def dequantize_w4(w: W4Weight, dtype: torch.dtype = torch.bfloat16, columns: tuple[int, int] | None = None) -> torch.Tensor:
+    """The weights as a tensor [N, K], or the columns [from, to) of them, ``from`` a multiple of 64; products may read it at once."""
+    _need_here("dequantize_w4", w.packed)
+    lo, hi = columns or (0, w.K)
+    need(0 <= lo < hi <= w.K and lo % 64 == 0, "dequantize_w4: columns must lie in the weight and start at a multiple of 64")
+    out = torch.empty((w.N, hi - lo), dtype=dtype, device=w.device)
+    check(_f("rf_dequantize_w4")(dtype_code(dtype), ptr(w.packed), ptr(w.scales), ptr(out), w.N, w.K, lo, hi, w.group, stream()),
+          "dequantize_w4")
     return out
-
-
-def _new_rows(T: int, K: int, group: int, dtype, device) -> Q8Rows:
-    Kp = padded_columns(K, group)
-    return Q8Rows(torch.empty((T, Kp), dtype=torch.int8, device=device),
-                  torch.empty((T, Kp // group), dtype=torch.float32, device=device), K, group, dtype)
 
 
 def quantize_q8(x: torch.Tensor, group: int = 128) -> Q8Rows:
@@ -168,9 +211,9 @@ def quantize_q8(x: torch.Tensor, group: int = 128) -> Q8Rows:
     _need_group(group, "quantize_q8")
     need(x.dim() == 2 and x.shape[1] > 0 and x.stride(1) == 1, "quantize_q8: x must be [T, K] with unit inner stride")
     T, K = x.shape
-    y = _new_rows(T, K, group, x.dtype, x.device)
-    f = _f("rf_quantize_q8", c_int, c_void_p, c_ll, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p)
-    check(f(dtype_code(x.dtype), ptr(x), x.stride(0), ptr(y.q), ptr(y.scales), T, K, group, stream()), f"quantize_q8 ({T}x{K})")
+    code = dtype_code(x.dtype)
+    y = Q8Rows.empty(T, K, group, x.dtype, x.device)
+    check(_f("rf_quantize_q8")(code, x.data_ptr(), x.stride(0), y.q.data_ptr(), y.scales.data_ptr(), T, K, group, stream()), "quantize_q8")
     return y
 
 
@@ -185,7 +228,8 @@ def add_rmsnorm_q8(h: torch.Tensor, weight: torch.Tensor, eps: float, compute_dt
     _need_group(group, "add_rmsnorm_q8")
     need(h.dtype == torch.float32 and h.dim() == 2 and h.is_contiguous(), "add_rmsnorm_q8: h must be [T,H] float32")
     T, H = h.shape
-    need(weight.shape == (H,) and weight.dtype in (torch.float32, torch.bfloat16) and weight.is_contiguous(),
+    w_is_f32 = weight.dtype == torch.float32
+    need(weight.shape == (H,) and (w_is_f32 or weight.dtype == torch.bfloat16) and weight.is_contiguous(),
          "add_rmsnorm_q8: weight must be [H] in float32 or bfloat16")
     kind, n_pending, pstride = 0, 0, 0
     if pending is not None:
@@ -202,11 +246,10 @@ def add_rmsnorm_q8(h: torch.Tensor, weight: torch.Tensor, eps: float, compute_dt
     if rows is not None:
         need(rows.dtype == torch.int32 and rows.dim() == 1 and rows.is_contiguous(), "add_rmsnorm_q8: rows must be 1-d int32")
         n_rows = rows.shape[0]
-    y = _new_rows(n_rows, H, group, compute_dtype, h.device)
-    f = _f("rf_add_rmsnorm_q8", c_int, c_void_p, c_void_p, c_int, c_int, c_ll, c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p, c_int,
-           c_int, c_int, c_int, c_void_p)
-    check(f(dtype_code(compute_dtype), ptr(h), ptr(pending), kind, n_pending, pstride, ptr(weight), int(weight.dtype == torch.float32), float(eps),
-            ptr(y.q), ptr(y.scales), ptr(rows), n_rows, T, H, group, stream()), f"add_rmsnorm_q8 (H={H})")
+    code = dtype_code(compute_dtype)
+    y = Q8Rows.empty(n_rows, H, group, compute_dtype, h.device)
+    check(_f("rf_add_rmsnorm_q8")(code, h.data_ptr(), ptr(pending), kind, n_pending, pstride, weight.data_ptr(), w_is_f32, eps, y.q.data_ptr(),
+                                  y.scales.data_ptr(), ptr(rows), n_rows, T, H, group, stream()), "add_rmsnorm_q8")
     return y
 
 
@@ -215,69 +258,118 @@ _ACTIVATIONS = {"silu": 0, "relu": 1, "gelu_tanh": 2}
 
 def swiglu_q8(gu: torch.Tensor, group: int = 128, activation: str = "silu") -> Q8Rows:
     """``swiglu`` with its result in 8 bits: act(gu[t, 2j]) * gu[t, 2j+1], from 32 bits straight to groups of ``group`` columns."""
-    need(activation in _ACTIVATIONS, f"swiglu_q8: activation {activation!r} (known: {sorted(_ACTIVATIONS)})")
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
+        raise KernelError(f"swiglu_q8: activation {activation!r} (known: {sorted(_ACTIVATIONS)})")
     _need_here("swiglu_q8", gu)
     _need_group(group, "swiglu_q8")
     need(gu.dim() == 2 and gu.is_contiguous() and gu.shape[1] % 2 == 0 and gu.shape[1] > 0, "swiglu_q8: input must be [T, 2I]")
     T, I = gu.shape[0], gu.shape[1] // 2
-    y = _new_rows(T, I, group, gu.dtype, gu.device)
-    f = _f("rf_swiglu_q8", c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p)
-    check(f(dtype_code(gu.dtype), ptr(gu), _ACTIVATIONS[activation], ptr(y.q), ptr(y.scales), T, I, group, stream()), f"swiglu_q8 (I={I})")
+    code = dtype_code(gu.dtype)
+    y = Q8Rows.empty(T, I, group, gu.dtype, gu.device)
+    check(_f("rf_swiglu_q8")(code, gu.data_ptr(), act, y.q.data_ptr(), y.scales.data_ptr(), T, I, group, stream()), "swiglu_q8")
     return y
 
 
 W4_FEW_TOKENS = 128      # tokens that products of 16-bit rows take straight from the 4 bits; more: the weights as 16 bits, then that product
 
 
+@functools.lru_cache(None)
+def w4_clusters(splits: int, device: int) -> int:
+    """Clusters of ``splits`` blocks that run at once on a device, an SM a block."""
+    if splits == 1:
+        return sm_count(device)
+    n = _f("rf_gemm_w4_clusters")(splits)
+    need(n > 0, "gemm_w4: no clusters can be launched")
+    return n
+
+
+@functools.lru_cache(4096)
+def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
+    """(eights, ways, splits, clusters): how ``rf_gemm_w4`` shares out a product.  Chosen from sizes alone."""
+    units, tiles = (padded_columns(K, group) // 64 + 1) // 2, (N + 15) // 16
+    eights, best = 1 if M <= 8 else 2 if M <= 16 else 4, None
+    while eights and best is None:                       # fewer tokens at once where longer rows leave no room for more
+        shares = (M + 8 * eights - 1) // (8 * eights)
+        for splits in range(1, 9):
+            if _f("rf_gemm_w4_shared")(0 if q8 else 1, M, K, group, eights, splits) > W4_MOST_SHARED:
+                continue
+            clusters = max(1, clusters_of(splits) // shares)
+            for ways in (1, 2, 4, 8, 16):
+                rounds = (tiles + clusters * (16 // ways) - 1) // (clusters * (16 // ways))
+                cost = rounds * ((units + splits * ways - 1) // (splits * ways) + 1) + (splits > 1)
+                if best is None or cost < best[0]:
+                    best = cost, eights, ways, splits, min(clusters, (tiles * ways + 15) // 16)
+        eights //= 2
+    if best is None:
+        raise KernelError(f"gemm_w4: rows of {K} columns are too long")
+    return best[1:]
+
+
+@functools.lru_cache(None)
+def _clusters_on(device: int):
+    return functools.partial(w4_clusters, device=device)
+
+
 def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tensor | None = None, out_f32: bool = False,
-            accumulate: bool = False, splits: int = 0) -> torch.Tensor:
+            accumulate: bool = False) -> torch.Tensor:
     """y = x @ w.T (+ bias) with 4-bit weights, 32-bit sums.
 
     ``x``: ``Q8Rows`` of the weight's K and group (products inside a group are exact, in whole numbers), or a tensor [M, K] in bfloat16
-    or float32.  out_f32: the result is float32 whatever the rows; accumulate: added into ``out`` (float32); splits >= 1 (8-bit rows, or
-    few 16-bit ones): the float32 stack [splits, M, N] of partial sums over ranges of K (no bias)."""
-    q8 = isinstance(x, Q8Rows)
+    or float32.  out_f32: the result is float32 whatever the rows; accumulate: added into ``out`` (float32)."""
+    q8 = type(x) is Q8Rows
     need(q8 or isinstance(x, torch.Tensor), "gemm_w4: x must be Q8Rows or a tensor")
-    need(isinstance(w, W4Weight), "gemm_w4: w must be a W4Weight")
-    _need_here("gemm_w4", x.q if q8 else x, w.packed, bias, out)
+    need(type(w) is W4Weight, "gemm_w4: w must be a W4Weight")
+    rows = x.q if q8 else x
+    _need_here("gemm_w4", rows, w.packed, bias, out)
     if q8:
-        need(x.group == w.group, f"gemm_w4: rows in groups of {x.group}, the weight in groups of {w.group}")
+        if x.group != w.group:
+            raise KernelError(f"gemm_w4: rows in groups of {x.group}, the weight in groups of {w.group}")
+        K = x.K
     else:
         need(x.dim() == 2 and x.stride(1) == 1, "gemm_w4: x must be [M, K] with unit inner stride")
-    need(x.shape[1] == w.K, f"gemm_w4: inner sizes differ ({x.shape[1]} vs {w.K})")
-    M, N, dt = x.shape[0], w.N, x.dtype
+        K = x.shape[1]
+    if K != w.K:
+        raise KernelError(f"gemm_w4: inner sizes differ ({K} vs {w.K})")
+    M, N, dt = rows.shape[0], w.N, x.dtype
     dtype_code(dt)
     if bias is not None:
         need(bias.shape == (N,) and bias.dtype in (torch.float32, torch.bfloat16) and bias.is_contiguous(), "gemm_w4: bias must be [N]")
-    if splits >= 1:
-        need(not accumulate and out is None and bias is None, "gemm_w4: partial sums take no bias and no output tensor")
-        out, mode, odt = torch.empty((splits, M, N), dtype=torch.float32, device=x.device), W4_PARTIAL, torch.float32
+    odt = torch.float32 if out_f32 or accumulate else dt
+    if out is None:
+        need(not accumulate, "gemm_w4: accumulate needs an output tensor")
+        out = torch.empty((M, N), dtype=odt, device=rows.device)
     else:
-        mode, odt = W4_ADD if accumulate else W4_STORE, torch.float32 if out_f32 or accumulate else dt
-        if out is None:
-            need(not accumulate, "gemm_w4: accumulate needs an output tensor")
-            out = torch.empty((M, N), dtype=odt, device=x.device)
         need(out.shape == (M, N) and out.dtype == odt and out.is_contiguous(), "gemm_w4: output must be [M, N], contiguous, of the result's dtype")
     if M == 0:
         return out
     if not q8 and (dt == torch.float32 or M > W4_FEW_TOKENS):
-        need(mode != W4_PARTIAL, "gemm_w4: no partial sums of float32 rows or of many tokens")
-        return _gemm_through_16_bits(x, w, bias, out, mode, odt)
-    f = _f("rf_gemm_w4", c_int, c_void_p, c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
-           c_int, c_int, c_void_p)
-    check(f(0 if q8 else 1, ptr(x.q if q8 else x), ptr(x.scales if q8 else None), x.q.stride(0) if q8 else x.stride(0), ptr(w.packed), ptr(w.scales),
-            ptr(bias), int(bias is not None and bias.dtype == torch.float32), ptr(out), int(odt == torch.float32), mode,
-            max(splits, 1), M, N, w.K, w.group, stream()), f"gemm_w4 ({M}x{N}x{w.K})")
+        return _gemm_through_16_bits(x, w, bias, out, accumulate)
+    at, ld = rows.data_ptr(), rows.stride(0)
+    eights, ways, splits, clusters = w4_launch(q8, M, N, K, w.group, _clusters_on(rows.get_device()))
+    code = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales.data_ptr() if q8 else None, ld, w.packed.data_ptr(), w.scales.data_ptr(), ptr(bias),
+                            bias is not None and bias.dtype == torch.float32, out.data_ptr(), odt == torch.float32, accumulate, eights, ways, splits,
+                            clusters, M, N, K, w.group, stream())
+    check(code, "gemm_w4" if code == 0 else f"gemm_w4 ({M}x{N}x{K})")
     return out
 
 
-def _gemm_through_16_bits(x, w, bias, out, mode, odt):
-    """The product by the weights written out once in the rows' dtype (exactly, with scales of five significant bits)."""
+# Columns that one tensor-core sum runs over where the result is 32-bit: its additions are cut, not rounded, and what is cut adds up
+# (1,999 x 3,584 x 18,944 against 64 bits: one sum 1.1e-5)
+SUM_COLUMNS = 8192
+
+
+def _gemm_through_16_bits(x, w, bias, out, accumulate):
+    """The product by the weights written out in the rows' dtype (exactly, with scales of five significant bits)."""
     from .basic import gemm_plain
     M, K = x.shape
-    full = dequantize_w4(w, x.dtype)
-    if x.dtype == torch.bfloat16:
-        m = tc.RESIDUAL if mode == W4_ADD else tc.F32 if odt == torch.float32 else tc.STORE
-        if tc.supported(M, w.N, K, m) and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0:
-            return tc.gemm_tc(x, full, bias, mode=m, out=out)
-    return gemm_plain(x, full, bias, out=out, out_f32=odt == torch.float32 and x.dtype != torch.float32, accumulate=mode == W4_ADD)
+    m = tc.RESIDUAL if accumulate else tc.F32 if out.dtype == torch.float32 else tc.STORE
+    if x.dtype == torch.bfloat16 and tc.supported(M, w.N, K, m) and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0:
+        pieces = 1 if m == tc.STORE else (K + SUM_COLUMNS - 1) // SUM_COLUMNS
+        step = (K + 64 * pieces - 1) // (64 * pieces) * 64
+        for lo in range(0, K, step):
+            hi = min(K, lo + step)
+            tc.gemm_tc(x[:, lo:hi], dequantize_w4(w, x.dtype, (lo, hi)), bias if lo == 0 else None, mode=m if lo == 0 else tc.RESIDUAL, out=out)
+        return out
+    return gemm_plain(x, dequantize_w4(w, x.dtype), bias, out=out, out_f32=out.dtype == torch.float32 and x.dtype != torch.float32,
+                      accumulate=accumulate)

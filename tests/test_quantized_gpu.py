@@ -177,11 +177,23 @@ def test_products(kind, M, N, K, G):
     h = numbers(M, N, seed=9)
     got = kernels.gemm_w4(x, w, b.to(DEV), out=h.to(DEV), accumulate=True)
     close(got, want + (h.double() + b.double()).to(DEV), size + (h.double().abs() + b.double().abs()).to(DEV), terms + 2, F32)
-    if kind == "q8" or (kind == "bf16" and M <= 128):
-        for splits in (1, 2, 3, 7, 200):                                              # (more than there are columns to share out)
-            parts = kernels.gemm_w4(x, w, splits=splits)
-            assert parts.shape == (splits, M, N) and parts.dtype == F32
-            close(parts.double().sum(0), want, size, terms, F32)
+
+
+@pytest.mark.parametrize("M,eights,ways,clusters", [(5, 1, 1, 2), (8, 1, 2, 1), (16, 1, 2, 3), (3, 1, 16, 1), (8, 1, 8, 20), (15, 2, 4, 2), (16, 2, 1, 1),
+                                                    (64, 4, 8, 5), (70, 4, 2, 1), (1, 4, 1, 1)])
+@pytest.mark.parametrize("kind", ["q8", "bf16"])
+@pytest.mark.parametrize("splits", [1, 2, 3, 8])
+@pytest.mark.parametrize("N,K,G", [(300, 1088, 32), (130, 200, 64), (17, 2176, 128), (450, 77, 128)])
+def test_every_way_to_share_out_a_product(monkeypatch, M, eights, ways, clusters, kind, splits, N, K, G):
+    """Columns over warps and over CTAs of a cluster (some of which get none), tiles over several rounds, tokens over several blocks."""
+    from rocmforge_b200 import kernels
+    from rocmforge_b200.kernels import quantized
+    monkeypatch.setattr(quantized, "w4_launch", lambda *a: (eights, ways, splits, clusters))
+    x, x64, w, full = product_case(kind, M, N, K, G)
+    x64, full = x64.to(DEV), full.to(DEV)
+    h = numbers(M, N, seed=9)
+    got = kernels.gemm_w4(x, w, out=h.to(DEV), accumulate=True)
+    close(got, x64 @ full.T + h.double().to(DEV), x64.abs() @ full.abs().T + h.double().abs().to(DEV), terms_of(kind, K) + 1, F32)
 
 
 @pytest.mark.parametrize("kind", ["q8", "bf16"])
@@ -220,10 +232,8 @@ def test_empty_and_refused():
     for call in (lambda: kernels.gemm_w4(x[:, :64], w), lambda: kernels.gemm_w4(kernels.quantize_q8(x, 32), w), lambda: kernels.gemm_w4(x.half(), w),
                  lambda: kernels.gemm_w4(x.t(), w), lambda: kernels.gemm_w4(x, x), lambda: kernels.gemm_w4(None, w),
                  lambda: kernels.gemm_w4(r, w, accumulate=True), lambda: kernels.gemm_w4(r, w, out=out), lambda: kernels.gemm_w4(r, w, out=out[:2], out_f32=True),
-                 lambda: kernels.gemm_w4(r, w, out=torch.zeros(32, 3, device=DEV).t(), out_f32=True), lambda: kernels.gemm_w4(r, w, splits=2, out=out),
-                 lambda: kernels.gemm_w4(r, w, out[0], splits=2), lambda: kernels.gemm_w4(r, w, torch.zeros(31, device=DEV)),
-                 lambda: kernels.gemm_w4(r, w, torch.zeros(32, device=DEV, dtype=torch.float16)), lambda: kernels.gemm_w4(x.float(), w, splits=2),
-                 lambda: kernels.gemm_w4(x.new_zeros(200, 128), w, splits=1), lambda: kernels.gemm_w4(r, w, torch.zeros(32)),
+                 lambda: kernels.gemm_w4(r, w, out=torch.zeros(32, 3, device=DEV).t(), out_f32=True), lambda: kernels.gemm_w4(r, w, torch.zeros(31, device=DEV)),
+                 lambda: kernels.gemm_w4(r, w, torch.zeros(32, device=DEV, dtype=torch.float16)), lambda: kernels.gemm_w4(r, w, torch.zeros(32)),
                  lambda: kernels.quantize_q8(x.t(), 64), lambda: kernels.quantize_q8(x, 16), lambda: kernels.quantize_q8(x.int(), 64),
                  lambda: kernels.quantize_w4(x.t(), 64), lambda: kernels.quantize_w4(x[:0], 64), lambda: kernels.quantize_w4(x, 256),
                  lambda: kernels.swiglu_q8(x[:, :127], 64), lambda: kernels.swiglu_q8(x, 64, activation="tanh"),
