@@ -10,8 +10,8 @@ has only a GPU path and no chat templates).  Greedy decoding is selected by
 tokens with their probabilities after the prompt (ten) and for the first steps (five each), or the
 count of NaN and Inf logits with minimum, maximum and mean if there are any; the logits are then
 looked at step by step, outside the replayed graphs.
-Added: --prompt-ids, --prompt-len, --top-k, --seed, --dtype, --stop-ids, --no-graph, --stats-json,
---random-config/--random-seed.  Text goes through a byte-level stand-in tokenizer.  The two
+Added: --prompt-ids, --prompt-len, --top-k, --seed, --dtype, --weight-bits/--weight-group/--row-bits, --stop-ids, --no-graph,
+--stats-json, --random-config/--random-seed.  Text goes through a byte-level stand-in tokenizer.  The two
 statistics lines on stderr are the reference's (src/main.rs:729-734, :989-994).
 """
 from __future__ import annotations
@@ -42,6 +42,11 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--stats-json", metavar="FILE", help="write the run's statistics as JSON to FILE ('-' = stdout)")
     ap.add_argument("--gpu", action="store_true", help="accepted; this engine always runs on the GPU")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    ap.add_argument("--weight-bits", type=int, choices=[4, 16], default=16,
+                    help="4: keep attention projections and dense feed-forwards in 4 bits, quantised when the model is loaded [default: 16]")
+    ap.add_argument("--weight-group", type=int, choices=[32, 64, 128], default=128, help="columns that share a 4-bit weight's scale [default: 128]")
+    ap.add_argument("--row-bits", type=int, choices=[8, 16], default=8,
+                    help="what products with 4-bit weights read while decoding: rows in 8 bits, or as they are [default: 8]")
     ap.add_argument("--stop-ids", default=None, help="comma-separated stop token ids (default: eos_token_id)")
     ap.add_argument("--random-config", help="config.json of a model to fill with random weights")
     ap.add_argument("--random-seed", type=int, default=0)
@@ -106,7 +111,7 @@ def main(argv=None) -> int:
         return 1
     try:
         from .engine.context import Options
-        options = Options(decode_graphs=not args.no_graph)
+        options = Options(decode_graphs=not args.no_graph, weight_bits=args.weight_bits, weight_group=args.weight_group, row_bits=args.row_bits)
         if args.model:
             llm = LLM(args.model, dtype=args.dtype, options=options)
         else:

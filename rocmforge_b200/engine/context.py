@@ -14,6 +14,7 @@ from typing import Optional
 import torch
 
 from .. import kernels
+from ..kernels import Q8Rows, W4Weight
 from .stream import ScaledRows
 
 
@@ -32,6 +33,21 @@ class Options:
     # 1.58 against 1.15 ms
     fused_norm: bool = False
     fused_norm_max_tokens: int = 32
+    # 4: the projections of attention mixers and the dense feed-forwards are quantised when the model is made, every group of weight_group
+    # columns (32, 64 or 128) with a scale of its own; everything else (embedding, head, norms, experts, other mixers) stays as it is
+    weight_bits: int = 16
+    weight_group: int = 128
+    # what such a product reads in steps of at most kernels.W4_FEW_TOKENS tokens: 8, rows in 8 bits with the weight's groups, exact sums within
+    # a group; 16, the rows as they are.  Steps of more tokens read them as they are, with either
+    row_bits: int = 8
+
+    def __post_init__(self):
+        if self.weight_bits not in (4, 16):
+            raise ValueError(f"weight_bits {self.weight_bits}: 4 or 16")
+        if self.weight_group not in kernels.W4_GROUPS:
+            raise ValueError(f"weight_group {self.weight_group} (known: {kernels.W4_GROUPS})")
+        if self.row_bits not in (8, 16):
+            raise ValueError(f"row_bits {self.row_bits}: 8 or 16")
 
 
 class StepContext:
@@ -61,13 +77,16 @@ class StepContext:
 
     # ---------------------------------------------------------------- matrix products
     def uses_tensor_cores(self, x, w, mode) -> bool:
-        return (self.compute_dtype == torch.bfloat16 and self.options.tensor_core_gemm
+        """Whether the tcgen05 kernels take the product (4-bit weights have kernels of their own)."""
+        return (not isinstance(w, W4Weight) and self.compute_dtype == torch.bfloat16 and self.options.tensor_core_gemm
                 and kernels.tensor_core.supported(x.shape[0], w.shape[0], w.shape[1], mode)
                 and x.data_ptr() % 16 == 0 and (x.stride(0) * 2) % 16 == 0)
 
     def unpack_rows(self, x, w, mode):
         """(tensor, row_ss) of an activation: the sums of squares go along where the product scales rows itself,
-        else the rows are normalised first."""
+        else the rows are normalised first.  8-bit rows stay what they are for a weight of their groups."""
+        if isinstance(x, Q8Rows):
+            return (x if isinstance(w, W4Weight) and w.group == x.group else x.materialize()), None
         if not isinstance(x, ScaledRows):
             return x, None
         tc = kernels.tensor_core
@@ -86,20 +105,31 @@ class StepContext:
             return tc.gemm_tc(x, w, bias, mode=mode)
         return self.gemm_plain(x, w, bias, out_f32=out_f32)
 
+    def q8_group(self, w) -> Optional[int]:
+        """The groups in which a product with ``w`` wants this step's rows in 8 bits; None: it wants them as they are."""
+        few = self.T <= kernels.W4_FEW_TOKENS
+        return w.group if isinstance(w, W4Weight) and self.options.row_bits == 8 and few else None
+
     def plain_splits(self, x, w) -> int:
         """K splits of a product of few tokens outside the bfloat16 tensor-core path."""
+        if isinstance(w, W4Weight):
+            return 1                                 # (its kernel adds up what its blocks have of a sum itself)
         return kernels.split_k_for_plain(x, w, self.options.tensor_core_gemm)
 
     def gemm_plain(self, x, w, bias=None, **kw):
         """A product outside the bfloat16 tensor-core path."""
+        if isinstance(w, W4Weight):
+            if not isinstance(x, Q8Rows) and self.q8_group(w) and x.shape[0] <= kernels.W4_FEW_TOKENS:
+                x = kernels.quantize_q8(x, w.group)
+            return kernels.gemm_w4(x, w, bias, **kw)
         return kernels.gemm_plain(x, w, bias, tensor_cores=self.options.tensor_core_gemm, **kw)
 
     def matmul_rows_or_parts(self, x, w):
         """x w^T as [M, N] in the compute dtype, or, where few tokens let K be split, as the float32 stack [S, M, N] of partial
         sums (for consumers that add them up themselves)."""
         tc = kernels.tensor_core
-        if isinstance(x, ScaledRows):
-            x = x.materialize()
+        if isinstance(x, (ScaledRows, Q8Rows)):
+            x = x.materialize() if isinstance(x, ScaledRows) else self.unpack_rows(x, w, tc.PARTIAL)[0]
         if x.shape[0] <= tc.SKINNY_MAX_TOKENS:
             if self.uses_tensor_cores(x, w, tc.PARTIAL):
                 splits = tc.split_k_for(w.shape[0], w.shape[1], tokens=x.shape[0])
@@ -164,11 +194,20 @@ class StepContext:
         stream.flush()
         self.gemm_plain(x, w, bias, out=stream.h, accumulate=True)
 
-    def gated_activation(self, y, gate_up, activation: str = "silu", limit: float = 0.0, alpha: float = 0.0):
+    def gated_activation(self, y, gate_up, activation: str = "silu", limit: float = 0.0, alpha: float = 0.0, reader=None):
         """act(gate) * up from the fused, row-interleaved gate/up matrix (act = silu, relu or gelu_tanh), or "clamped_glu":
-        g sigmoid(alpha g) (u + 1) with g = min(gate, limit), u = clamp(up, -limit, limit)."""
+        g sigmoid(alpha g) (u + 1) with g = min(gate, limit), u = clamp(up, -limit, limit).  ``reader``: the weight of the product
+        that reads the result, which comes in 8 bits where that product wants it so."""
         tc = kernels.tensor_core
         w = gate_up.weight
+        if isinstance(w, W4Weight):
+            if y.shape[0] <= kernels.W4_FEW_TOKENS or self.compute_dtype != torch.bfloat16:
+                gu = self.matmul(y, w, gate_up.bias)
+                if activation == "clamped_glu":
+                    return kernels.clamped_glu(gu, limit, alpha)
+                group = self.q8_group(reader)
+                return kernels.swiglu_q8(gu, group, activation) if group else kernels.swiglu(gu, activation=activation)
+            w = kernels.dequantize_w4(w, self.compute_dtype)         # many tokens: the 16-bit product with the unit in its epilogue
         mode = {"silu": tc.SWIGLU, "relu": tc.REGLU, "gelu_tanh": tc.GEGLU, "clamped_glu": tc.CLAMPGLU}[activation]
         glu = dict(limit=limit, alpha=alpha) if mode == tc.CLAMPGLU else {}
         y, row_ss = self.unpack_rows(y, w, mode)

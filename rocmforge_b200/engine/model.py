@@ -124,7 +124,7 @@ class Model:
         if self.device.type != "cuda":
             raise RuntimeError("rocmforge_b200 models run on a CUDA device only (there is no CPU fallback)")
         self.options = options or Options()
-        build.ensure_built(spec.cuda_modules(compute_dtype))
+        build.ensure_built(spec.cuda_modules(compute_dtype) + (["quantized"] if self.options.weight_bits == 4 else []))
         for prefix, part in spec.named_parts().items():
             local = {name[len(prefix):]: t for name, t in params.items()
                      if name.startswith(prefix) and name[len(prefix):] in part.param_specs()}
@@ -137,6 +137,11 @@ class Model:
         self._scratch: Dict[tuple, torch.Tensor] = {}
         self.weight_bytes = sum(t.numel() * t.element_size()
                                 for t in {t.data_ptr(): t for t in params.values()}.values())
+        if self.options.weight_bits == 4:
+            with torch.cuda.device(self.device):
+                for part in spec.named_parts().values():
+                    for linear in part.linears():
+                        self.weight_bytes -= linear.to_4_bits(self.options.weight_group)
 
     # ---------------------------------------------------------------- construction
     @classmethod

@@ -200,6 +200,12 @@ class GQAAttention(Mixer):
         if self.distance_slopes is not None:
             self.slopes_dev = torch.tensor(self.distance_slopes, dtype=torch.float32, device=w.device)
 
+    def linears(self):
+        return [self.qkv, self.o]
+
+    def input_weight(self):
+        return self.qkv.weight
+
     def cuda_modules(self, compute_dtype):
         mods = ["elementwise", "attention_generic"]
         if compute_dtype == torch.bfloat16 and self.v_head_dim == self.head_dim:

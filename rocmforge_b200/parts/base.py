@@ -36,6 +36,15 @@ class Part:
     def cuda_modules(self, compute_dtype: torch.dtype) -> List[str]:
         return []
 
+    def linears(self) -> list:
+        """The part's bound ``Linear`` products that work with their weight in 4 bits as well."""
+        return []
+
+    def input_weight(self):
+        """The weight of the product that alone reads the part's input, if there is one such product (a norm that knows it may hand
+        on what that product wants)."""
+        return None
+
     def step_table_names(self):
         """Names of int32 tables that this part builds on the host for every step (``step_table``).  They travel with
         the step descriptor in its one copy and reach the part as ``ctx.tables[name]``.  A name identifies its

@@ -40,9 +40,15 @@ class PreNormBlock(Block):
     def entry_norm(self):
         return self.norm1 if self.mixer.accepts_scaled_rows else None
 
+    @staticmethod
+    def _normed(ctx, stream, norm, reader):
+        """The norm's result for the part that reads it: in 8 bits where a 4-bit weight alone reads it."""
+        group = ctx.q8_group(reader.input_weight()) if hasattr(norm, "forward_q8") else None
+        return norm.forward_q8(ctx, stream, group) if group else norm.forward(ctx, stream, deferred_ok=reader.accepts_scaled_rows)
+
     def forward(self, ctx, stream, cache_view):
         after = stream.after_block                   # the norm that follows this block (the model knows the order)
-        y = self.norm1.forward(ctx, stream, deferred_ok=self.mixer.accepts_scaled_rows)
+        y = self._normed(ctx, stream, self.norm1, self.mixer)
         if self.ffn is None:
             stream.next_norm = after
             self.mixer.forward(ctx, y, cache_view, stream)
@@ -52,7 +58,7 @@ class PreNormBlock(Block):
         stream.next_norm = (self.norm2 if self.ffn.accepts_scaled_rows or getattr(self.mixer, "prepares_next_norm", False)
                             else None)
         self.mixer.forward(ctx, y, cache_view, stream)
-        y = self.norm2.forward(ctx, stream, deferred_ok=self.ffn.accepts_scaled_rows)
+        y = self._normed(ctx, stream, self.norm2, self.ffn)
         stream.next_norm = after
         self.ffn.forward(ctx, y, stream)
         stream.next_norm = None

@@ -14,13 +14,19 @@ class Linear:
     On the float32 path a product runs on the tensor cores too, every number as three bfloat16 parts (an exact sum), where TMA can
     fetch the rows, and on CUDA cores otherwise; operands and sums are 32-bit either way.
     On the bfloat16 path the tensor-core kernels are used where the shape allows and the
-    CUDA-core kernel otherwise; both accumulate in 32-bit.
+    CUDA-core kernel otherwise; both accumulate in 32-bit.  A weight in 4 bits (``to_4_bits``) is a ``kernels.W4Weight``.
     """
 
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
         self.weight = weight
         self.bias = bias
         self.N, self.K = weight.shape
+
+    def to_4_bits(self, group: int) -> int:
+        """Keep the weight in 4 bits with a scale for every ``group`` columns from here on; the bytes that this saves."""
+        before = self.weight.numel() * self.weight.element_size()
+        self.weight = kernels.quantize_w4(self.weight, group)
+        return before - self.weight.nbytes
 
     def __call__(self, ctx, x: torch.Tensor, *, out_f32: bool = False) -> torch.Tensor:
         """x [M, K] -> [M, N] in the compute dtype (or float32)."""

@@ -52,15 +52,21 @@ class GatedMLP(FeedForward):
         self.gate_up = Linear(gu)
         self.down = Linear(params[self.names["down"]])
 
+    def linears(self):
+        return [self.gate_up, self.down]
+
+    def input_weight(self):
+        return self.gate_up.weight
+
     def cuda_modules(self, compute_dtype):
         return ["elementwise"]
 
     def forward(self, ctx, y, stream):
-        a = ctx.gated_activation(y, self.gate_up, self.activation, **self.unit_constants)          # [T, I]
+        a = ctx.gated_activation(y, self.gate_up, self.activation, reader=self.down.weight, **self.unit_constants)          # [T, I]
         self.down.add_to_stream(ctx, a, stream)
 
     def output(self, ctx, y):
-        return self.down.f32_parts(ctx, ctx.gated_activation(y, self.gate_up, self.activation, **self.unit_constants))
+        return self.down.f32_parts(ctx, ctx.gated_activation(y, self.gate_up, self.activation, reader=self.down.weight, **self.unit_constants))
 
 
 @FEED_FORWARDS.register("relu2_mlp")
@@ -81,6 +87,12 @@ class SquaredReluMLP(FeedForward):
     def bind(self, params, compute_dtype):
         self.up = Linear(params[self.names["up"]])
         self.down = Linear(params[self.names["down"]])
+
+    def linears(self):
+        return [self.up, self.down]
+
+    def input_weight(self):
+        return self.up.weight
 
     def cuda_modules(self, compute_dtype):
         return ["elementwise"]

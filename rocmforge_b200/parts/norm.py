@@ -58,6 +58,15 @@ class RMSNorm(Norm):
             stream.pending = None           # the kernel added it into h
         return y
 
+    def forward_q8(self, ctx, stream, group: int):
+        """The norm of all rows in 8 bits, groups of ``group`` (``kernels.Q8Rows``), unless whoever updated the stream has run it already."""
+        if stream.prepared is not None and stream.prepared[0] is self and stream.pending is None:
+            return self.forward(ctx, stream)
+        stream.prepared = None
+        y = kernels.add_rmsnorm_q8(stream.h, self.weight, self.eps, self.compute_dtype, group, pending=stream.pending)
+        stream.pending = None               # the kernel added it into h
+        return y
+
 
 @NORMS.register("dyt")
 class DynamicTanh(Norm):

@@ -74,3 +74,27 @@ def test_nothing_runs_on_the_cpu():
                  lambda: kernels.gemm_w4(r, w), lambda: kernels.gemm_w4(x, w)):
         with pytest.raises(KernelError, match="CUDA device"):
             call()
+
+
+def test_options():
+    from rocmforge_b200 import Options
+    from rocmforge_b200.cli import build_parser
+    o = Options()
+    assert (o.weight_bits, o.weight_group, o.row_bits) == (16, 128, 8)
+    for bad in (dict(weight_bits=8), dict(weight_bits=4, weight_group=16), dict(row_bits=4)):
+        with pytest.raises(ValueError):
+            Options(**bad)
+    a = build_parser().parse_args(["-m", "x", "-p", "hi"])
+    assert (a.weight_bits, a.weight_group, a.row_bits) == (16, 128, 8)
+
+
+def test_products_of_a_part():
+    """Which products a model's parts offer for 4 bits: the projections of attention and of dense feed-forwards."""
+    from helpers import CONFIGS, config_dict
+    from rocmforge_b200.config import Qwen2Config, architecture_for
+    from rocmforge_b200.parts.attention import GQAAttention
+    from rocmforge_b200.parts.mlp import GatedMLP
+    cfg = Qwen2Config.from_dict(config_dict(CONFIGS["A"]))
+    spec = architecture_for(cfg.architecture).build(cfg)
+    offering = {type(p) for p in spec.named_parts().values() if type(p).linears is not __import__("rocmforge_b200.parts.base", fromlist=["Part"]).Part.linears}
+    assert offering == {GQAAttention, GatedMLP}
