@@ -42,7 +42,8 @@ MODULES: Dict[str, List[str]] = {
     "streams": ["streams.cu", "common.cuh"],
     "latent": ["latent.cu", "common.cuh"],
     "random_fill": ["random_fill.cu", "common.cuh"],
-    "quantized": ["quantized.cu", "common.cuh"],
+    "quantized": ["quantized.cu", "quantized.cuh", "common.cuh"],
+    "quantized_tc": ["quantized_tc.cu", "quantized.cuh", "tcgen05_common.cuh", "common.cuh"],
     "gemm_tcgen05": ["gemm_tcgen05.cu", "tcgen05_common.cuh", "common.cuh"],
     # has one CTA load a tile for its whole cluster (this GPU's memory only): a file of its own, left out of
     # multi-GPU runs; the package works without it

@@ -5,13 +5,8 @@
 // blocks with Q8_0 rows (hip_kernels/quant/, src/gpu/quant_wrapper.rs) use the same pair, blocks of 32 and halves as scales; the layout,
 // the group sizes and the kernels here are this library's own.
 //
-// How weights are stored.  The unit is a tile of 16 rows by 64 columns, 512 bytes in a row, the tiles of 16 rows one after another along
-// K.  The 16 bytes of lane 4 g + t hold rows g and g + 8 of the columns 32 c + 8 t .. + 7, c = 0, 1, as four words (row g: c = 0, 1; row
-// g + 8: c = 0, 1); the low half of byte b of a word is column b of the eight, the high half column 4 + b.  So a lane's one 16-byte load
-// is what it feeds to two mma.m16n8k32 of 8-bit integers (or four m16n8k16 of bfloat16 numbers): halves of bytes become operands with
-// one shift and one mask, in place, and a row's 8 numbers for the same columns are one 8-byte load of the row as it lies.  The scales
-// lie beside them, [tile of rows, group, 16], row g + 8 r at 2 g + r: the two that a lane needs are one word.
-#include "common.cuh"
+// How weights are stored: quantized.cuh.
+#include "quantized.cuh"
 #include <type_traits>
 
 template <typename T> struct Quad;                       // four neighbouring numbers
@@ -321,12 +316,6 @@ __device__ __forceinline__ void quarter(float (&c)[4], uint32_t lo_row, uint32_t
     mma_bf16(c, two_weights(lo_row >> 4), two_weights(hi_row >> 4), two_weights(lo_row >> 12), two_weights(hi_row >> 12),
              __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
 }
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {       // zeros if it is not there
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
-}
 __device__ __forceinline__ unsigned long long two(float a, float b) {
     unsigned long long r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -346,20 +335,6 @@ __device__ __forceinline__ unsigned long long fma_two(unsigned long long a, unsi
     unsigned long long r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
-}
-
-struct W4Out {
-    void* out;               // [M, N] float32 if is_f32, else bfloat16; add: float32, added into
-    const void* bias;        // [N] or null
-    int bias_is_f32, is_f32, add, M, N;
-};
-__device__ __forceinline__ void w4_write(const W4Out& o, int t, int n, float v) {
-    if (n >= o.N) return;
-    if (o.bias != nullptr) v += load_vec(o.bias, o.bias_is_f32, n);
-    const size_t at = (size_t)t * o.N + n;
-    if (o.add) reinterpret_cast<float*>(o.out)[at] += v;
-    else if (o.is_f32) reinterpret_cast<float*>(o.out)[at] = v;
-    else reinterpret_cast<__nv_bfloat16*>(o.out)[at] = __float2bfloat16_rn(v);
 }
 
 // 8 NB tokens (blockIdx.y) by tiles of 16 rows, one block of 16 warps an SM for as long as there are tiles.  The numbers of the block's
@@ -586,10 +561,6 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint
 }
 
 // ---------------------------------------------------------------- launchers
-static bool bad_group(int G) { return G != 32 && G != 64 && G != 128; }
-static int padded(int K, int G) { const int u = G > 64 ? G : 64; return (K + u - 1) / u * u; }
-static bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
-
 // f(G as a constant)
 template <typename F>
 static void with_group(int G, F f) {

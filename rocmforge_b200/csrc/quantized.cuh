@@ -1,0 +1,36 @@
+// What the kernels with 4-bit weights share: the stored form, asynchronous copies, the output.
+//
+// How weights are stored.  The unit is a tile of 16 rows by 64 columns, 512 bytes in a row, the tiles of 16 rows one after another along
+// K.  The 16 bytes of lane 4 g + t hold rows g and g + 8 of the columns 32 c + 8 t .. + 7, c = 0, 1, as four words (row g: c = 0, 1; row
+// g + 8: c = 0, 1); the low half of byte b of a word is column b of the eight, the high half column 4 + b.  So a lane's one 16-byte load
+// is what it feeds to two mma.m16n8k32 of 8-bit integers (or four m16n8k16 of bfloat16 numbers): halves of bytes become operands with
+// one shift and one mask, in place, and a row's 8 numbers for the same columns are one 8-byte load of the row as it lies.  The scales
+// lie beside them, [tile of rows, group, 16], row g + 8 r at 2 g + r: the two that a lane needs are one word.
+#pragma once
+#include "common.cuh"
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {       // zeros if it is not there
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+
+struct W4Out {
+    void* out;               // [M, N] float32 if is_f32, else bfloat16; add: float32, added into
+    const void* bias;        // [N] or null
+    int bias_is_f32, is_f32, add, M, N;
+};
+__device__ __forceinline__ void w4_write(const W4Out& o, int t, int n, float v) {
+    if (n >= o.N) return;
+    if (o.bias != nullptr) v += load_vec(o.bias, o.bias_is_f32, n);
+    const size_t at = (size_t)t * o.N + n;
+    if (o.add) reinterpret_cast<float*>(o.out)[at] += v;
+    else if (o.is_f32) reinterpret_cast<float*>(o.out)[at] = v;
+    else reinterpret_cast<__nv_bfloat16*>(o.out)[at] = __float2bfloat16_rn(v);
+}
+
+
+static bool bad_group(int G) { return G != 32 && G != 64 && G != 128; }
+static int padded(int K, int G) { const int u = G > 64 ? G : 64; return (K + u - 1) / u * u; }
+static bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }

@@ -1,0 +1,411 @@
+// Products with 4-bit weights on the 5th-generation tensor cores, for more tokens than mma.sync serves at the rate of memory.
+//
+// Weights are the accumulator's rows, tokens its columns.  128 rows of weights go through shared memory a stage at a time: eight warps fetch
+// their tile of 16 rows as it is stored (asynchronous copies into a ring of their own, far ahead, and before the wait for the kernel
+// before), widen it and write it where the MMA reads it; the tokens' numbers come by TMA.  A stage is 128 bytes of a row:
+//   16-bit rows: 64 columns; the weights become bfloat16 numbers, scale and all (exactly, with scales of five significant bits; others are
+//     rounded), and the whole product is one accumulator's.
+//   8-bit rows: 128 columns; the weights become 16 q as signed bytes and a group's sum is exact in whole numbers, in an accumulator of its own,
+//     which eight more warps read, scale by both scales and add to their 32-bit sums while the next groups are multiplied.
+// Long rows are shared out to the CTAs of a cluster, which add up their sums through shared memory in the order of their ranks.
+//
+// Every wait on an mbarrier is bounded (2 s): status word 13.
+#include <type_traits>
+#include "quantized.cuh"
+#include "tcgen05_common.cuh"
+
+#define W4T_THREADS (32 * 18)                            // the tokens' producer, the MMA issuer, eight widening warps, eight adding warps
+#define W4T_PITCH (128 + 4)                              // of the sums that a cluster exchanges, [token][row]
+
+template <int BN, bool BYTES, int G>
+struct TcShape {
+    static constexpr int A = 128 * 128, B = BN * 128, STAGE = A + B, STAGES = BN <= 64 ? 4 : 3;
+    static constexpr int BLOCKS = BYTES ? 2 : 1;         // blocks of 64 columns a stage
+    static constexpr int PARTS = BYTES ? 128 / G : 1;    // accumulators a stage
+    static constexpr int BUFS = BYTES ? (BN <= 64 ? 4 : 2) : 1;
+    static constexpr int TMEM = BUFS * BN < 32 ? 32 : BUFS * BN;
+    static constexpr int SCALES = BYTES ? 0 : (G == 32 ? 2 : 1);        // groups whose scales travel with a stage
+    static constexpr int SLOT = BLOCKS * 512 + SCALES * 32, DEPTH = BYTES ? 8 : 14, RING = 8 * DEPTH * SLOT;
+    static constexpr int FIXED = STAGES * STAGE + RING + 1024 + 256;    // (alignment, barriers)
+    static_assert(STAGES * STAGE >= BN * W4T_PITCH * 4, "the stages' place holds the sums");
+};
+
+template <int BN, bool BYTES>
+__device__ __forceinline__ void mma_step(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+    if constexpr (BYTES) {
+        constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | (8u << 24);       // signed bytes, 32-bit whole sums
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    } else {
+        tcgen05_mma_bf16(d, a, b, make_idesc(BN), accumulate);
+    }
+}
+
+// Four halves of bytes of a word as bfloat16 numbers times a scale, pairs in the order of the columns: `w` has its middle bytes swapped.
+__device__ __forceinline__ uint32_t widened(uint32_t w, __nv_bfloat162 s) {
+    uint32_t v = (w & 0x000f000fu) ^ 0x43084308u;        // 128 + (q + 8)
+    const __nv_bfloat162 r = __hmul2(__hadd2(*reinterpret_cast<__nv_bfloat162*>(&v), __float2bfloat162_rn(-136.f)), s);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <int BN, bool BYTES, int G>
+__global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const uint4* __restrict__ w0, const uint32_t* __restrict__ w1,
+                                                               const float* xs, int blocks, int splits, int* status, W4Out o) {
+    using S = TcShape<BN, BYTES, G>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE + S::RING);       // full, empty, sum full, sum empty
+    constexpr int FULL = 0, EMPTY = S::STAGES, SUM_FULL = 2 * S::STAGES, SUM_EMPTY = SUM_FULL + S::BUFS, BARS = SUM_EMPTY + S::BUFS;
+    static_assert(BARS * 8 + 4 <= 256, "room for the barriers");
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
+    float* scales = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE + S::RING + 256);     // 8-bit rows: [group][token]
+    __shared__ int abort_flag;
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % splits, row0 = blockIdx.x / splits * 128, tok0 = blockIdx.y * BN, live = min(BN, o.M - tok0);
+    const int all = (blocks + S::BLOCKS - 1) / S::BLOCKS, from = (int)((long long)all * rank / splits);
+    const int n = (int)((long long)all * (rank + 1) / splits) - from;
+    const int tiles = (o.N + 15) / 16, all_groups = blocks * 64 / G;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < S::STAGES; ++i) {
+            mbar_init(smem_u32(&bars[FULL + i]), 9);     // eight widening warps and the producer
+            mbar_init(smem_u32(&bars[EMPTY + i]), 1);
+        }
+        for (int i = 0; i < S::BUFS; ++i) {
+            mbar_init(smem_u32(&bars[SUM_FULL + i]), 1);
+            mbar_init(smem_u32(&bars[SUM_EMPTY + i]), 8);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+    }
+    if (warp == 1) {
+        tcgen05_alloc(smem_u32(tmem_slot), S::TMEM);
+        tcgen05_relinquish();
+    }
+    // the widening warps' rings, filled before anything is waited for
+    const int wide = warp - 2, tile = row0 / 16 + wide;
+    const bool widens = wide >= 0 && wide < 8, mine = widens && tile < tiles;
+    const uint32_t ring = smem_u32(smem) + S::STAGES * S::STAGE + wide * S::DEPTH * S::SLOT;
+    auto ask = [&](int i) {
+        if (mine && i < n) {
+            const uint32_t to = ring + i % S::DEPTH * S::SLOT;
+            const int block = (from + i) * S::BLOCKS;
+            const uint4* p = w0 + ((size_t)tile * blocks + block) * 32 + lane;
+            copy16(to + 16 * lane, p, true);
+            if (S::BLOCKS == 2) copy16(to + 512 + 16 * lane, block + 1 < blocks ? p + 32 : p, block + 1 < blocks);
+            if (S::SCALES && lane < 2 * S::SCALES)       // the 16 rows' scales of a group are 32 bytes
+                copy16(to + 512 + 16 * lane, reinterpret_cast<const uint4*>(w1) + ((size_t)tile * all_groups + (from + i) * 64 / G) * 2 + lane, true);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (widens)
+        for (int i = 0; i < S::DEPTH; ++i) ask(i);
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const int add = warp - 10, quarter = warp & 3, cols0 = add >= 4 ? BN / 2 : 0;       // adding warps: 32 rows, half the tokens
+    Two acc[BYTES ? BN / 4 : 1] = {};
+    bool ok = true;
+    if (warp == 0) {
+        // ---------------- the tokens' numbers
+        if (lane == 0) {
+            pdl_wait();
+            for (int i = 0; i < n; ++i) {
+                const int s = i % S::STAGES;
+                if (i >= S::STAGES && !mbar_wait(smem_u32(&bars[EMPTY + s]), ((i / S::STAGES) & 1) ^ 1, &abort_flag)) break;
+                mbar_expect_tx(smem_u32(&bars[FULL + s]), S::B);
+                tma_load_2d(smem_u32(smem) + s * S::STAGE + S::A, &map_x, (from + i) * S::BLOCKS * 64, tok0, smem_u32(&bars[FULL + s]));
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- the products
+        if (elect_one()) {
+            int sum = 0;
+            for (int i = 0; i < n && ok; ++i) {
+                const int s = i % S::STAGES;
+                ok = mbar_wait(smem_u32(&bars[FULL + s]), (i / S::STAGES) & 1, &abort_flag);
+                if (!ok) break;
+                tcgen05_fence_after();
+                const uint64_t da = make_smem_desc(smem_u32(smem) + s * S::STAGE), db = make_smem_desc(smem_u32(smem) + s * S::STAGE + S::A);
+                if constexpr (BYTES) {
+#pragma unroll
+                    for (int p = 0; p < S::PARTS && ok; ++p, ++sum) {
+                        const int buf = sum % S::BUFS;
+                        if (sum >= S::BUFS) {
+                            ok = mbar_wait(smem_u32(&bars[SUM_EMPTY + buf]), ((sum / S::BUFS) & 1) ^ 1, &abort_flag);
+                            tcgen05_fence_after();
+                        }
+                        if (!ok) break;
+#pragma unroll
+                        for (int k = 0; k < 4 / S::PARTS; ++k) {                        // 32 columns an instruction
+                            const int at = 2 * (p * (4 / S::PARTS) + k);
+                            mma_step<BN, BYTES>(tmem + buf * BN, da + at, db + at, k ? 1u : 0u);
+                        }
+                        tcgen05_commit(smem_u32(&bars[SUM_FULL + buf]));
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_step<BN, BYTES>(tmem, da + 2 * k, db + 2 * k, (i | k) ? 1u : 0u);   // 16 columns
+                }
+                tcgen05_commit(smem_u32(&bars[EMPTY + s]));
+            }
+            if (!BYTES) tcgen05_commit(smem_u32(&bars[SUM_FULL]));
+        }
+    } else if (widens) {
+        // ---------------- the weights
+        const int g = lane >> 2, t = lane & 3;
+        for (int i = 0; i < n; ++i) {
+            const int s = i % S::STAGES;
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::DEPTH - 1) : "memory");
+            __syncwarp();
+            const uint8_t* here = smem + S::STAGES * S::STAGE + (wide * S::DEPTH + i % S::DEPTH) * S::SLOT;
+            uint4 w[S::BLOCKS];
+            uint32_t sc[S::SCALES ? S::SCALES : 1];
+#pragma unroll
+            for (int b = 0; b < S::BLOCKS; ++b) w[b] = *reinterpret_cast<const uint4*>(here + 512 * b + 16 * lane);
+#pragma unroll
+            for (int p = 0; p < S::SCALES; ++p) sc[p] = *reinterpret_cast<const uint32_t*>(here + 512 + 32 * p + 4 * g);
+            __syncwarp();                                // all have read the slot
+            ask(i + S::DEPTH);
+            if (i >= S::STAGES && !mbar_wait(smem_u32(&bars[EMPTY + s]), ((i / S::STAGES) & 1) ^ 1, &abort_flag)) break;
+            if (mine) {
+                uint8_t* to = smem + s * S::STAGE + (16 * wide + g) * 128;              // (rows of 128 bytes, 16-byte pieces swapped by row % 8 = g)
+                if constexpr (BYTES) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {        // by the row's parity another block first: four rows' pieces then meet all banks
+                        const int b = (j >> 1) ^ (g & 1), c = j & 1;
+                        const uint4 v = b ? w[1] : w[0];
+                        const int at = ((4 * b + 2 * c + (t >> 1)) ^ g) * 16 + (t & 1) * 8;
+                        const uint32_t m = 0xf0f0f0f0u, lo = c ? v.y : v.x, hi = c ? v.w : v.z;
+                        *reinterpret_cast<uint2*>(to + at) = make_uint2(lo << 4 & m, lo & m);
+                        *reinterpret_cast<uint2*>(to + 8 * 128 + at) = make_uint2(hi << 4 & m, hi & m);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int c = j ^ (g & 1);       // two rows' pieces then meet all banks
+                        const uint32_t s2 = S::SCALES == 2 && c ? sc[S::SCALES - 1] : sc[0];
+                        const int at = ((4 * c + t) ^ g) * 16;
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const uint32_t word = __byte_perm(r ? (c ? w[0].w : w[0].z) : (c ? w[0].y : w[0].x), 0, 0x3120);
+                            const uint32_t both = __byte_perm(s2, 0, r ? 0x3232 : 0x1010);
+                            const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&both);
+                            *reinterpret_cast<uint4*>(to + r * 8 * 128 + at) =
+                                make_uint4(widened(word, f), widened(word >> 8, f), widened(word >> 4, f), widened(word >> 12, f));
+                        }
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) at_arrive(smem_u32(&bars[FULL + s]));
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else {
+        // ---------------- the sums
+        pdl_wait(xs);
+        const int row = row0 + 32 * quarter + lane;
+        if constexpr (BYTES) {
+            const int first = from * S::PARTS, count = n * S::PARTS;
+            for (int i = threadIdx.x - 320; i < count * live; i += 256) {
+                const int tok = i / count, gr = i - tok * count;
+                scales[gr * BN + tok] = first + gr < all_groups ? xs[(size_t)(tok0 + tok) * all_groups + first + gr] : 0.f;
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const __nv_bfloat16* ws = reinterpret_cast<const __nv_bfloat16*>(w1) + (size_t)(row / 16) * all_groups * 16 + 2 * (row % 8) + row % 16 / 8;
+            auto scale_of = [&](int i) { return row < o.N && first + i < all_groups && i < count ? __bfloat162float(ws[(size_t)(first + i) * 16]) * 0.0625f : 0.f; };
+            float next = scale_of(0);
+            const Two less = two(-12582912.f, -12582912.f);
+            for (int i = 0; i < count && ok; ++i) {
+                const int buf = i % S::BUFS;
+                const float f = next;
+                next = scale_of(i + 1);
+                ok = mbar_wait(smem_u32(&bars[SUM_FULL + buf]), (i / S::BUFS) & 1, &abort_flag);
+                if (!ok) break;
+                tcgen05_fence_after();
+                constexpr int CH = 16;                   // (32 numbers beside the sums would not fit the registers)
+                const Two ff = two(f, f);
+#pragma unroll
+                for (int c = 0; c < BN / 2; c += CH) {
+                    uint32_t r[CH];
+                    const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + cols0 + c;
+                    tcgen05_ld16(at, r);
+                    tcgen05_wait_ld();
+                    if (c + CH == BN / 2) {
+                        tcgen05_fence_before();
+                        __syncwarp();
+                        if (lane == 0) at_arrive(smem_u32(&bars[SUM_EMPTY + buf]));
+                    }
+                    const float* a = scales + i * BN + cols0 + c;
+#pragma unroll
+                    for (int j = 0; j < CH; j += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(a + j);
+                        // a whole number below 2^22 as a float: in the last bits of 1.5 2^23
+                        const Two v0 = add2(two(__uint_as_float(r[j] + 0x4b400000u), __uint_as_float(r[j + 1] + 0x4b400000u)), less);
+                        const Two v1 = add2(two(__uint_as_float(r[j + 2] + 0x4b400000u), __uint_as_float(r[j + 3] + 0x4b400000u)), less);
+                        acc[(c + j) / 2] = fma2(v0, mul2(two(x.x, x.y), ff), acc[(c + j) / 2]);
+                        acc[(c + j) / 2 + 1] = fma2(v1, mul2(two(x.z, x.w), ff), acc[(c + j) / 2 + 1]);
+                    }
+                }
+            }
+        } else if (n > 0) {
+            ok = mbar_wait(smem_u32(&bars[SUM_FULL]), 0, &abort_flag);
+            tcgen05_fence_after();
+        }
+    }
+    pdl_wait();                                          // (who writes below may not have waited yet)
+    __syncwarp();
+    // a cluster's sums go through the stages' place; one CTA's straight out
+    if (splits > 1) __syncthreads();                     // (the last sums were there: every product has read its stages)
+    if (add >= 0 && ok) {
+        float* sums = reinterpret_cast<float*>(smem) + 32 * quarter + lane;
+        const int row = row0 + 32 * quarter + lane;
+        auto give = [&](int tok, float v) {
+            if (splits > 1) sums[tok * W4T_PITCH] = v;
+            else if (tok < live) w4_write(o, tok0 + tok, row, v);
+        };
+        if constexpr (BYTES) {
+#pragma unroll
+            for (int j = 0; j < BN / 4; ++j) {
+                float a, b;
+                one(acc[j], a, b);
+                give(cols0 + 2 * j, a);
+                give(cols0 + 2 * j + 1, b);
+            }
+        } else {
+            constexpr int CH = BN / 2 < 32 ? 16 : 32;
+#pragma unroll 1
+            for (int c = 0; c < BN / 2; c += CH) {
+                uint32_t r[CH];
+                const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + cols0 + c;
+                if (n > 0) {
+                    if constexpr (CH == 32) tcgen05_ld32(at, r); else tcgen05_ld16(at, r);
+                    tcgen05_wait_ld();
+                }
+#pragma unroll
+                for (int j = 0; j < CH; ++j) give(cols0 + c + j, n > 0 ? __uint_as_float(r[j]) : 0.f);
+            }
+        }
+    }
+    if (splits > 1) {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        const float* sums = reinterpret_cast<const float*>(smem);
+        for (int i = rank * W4T_THREADS + threadIdx.x; i < live * 128; i += splits * W4T_THREADS) {
+            const int tok = i / 128, r = i % 128;
+            const uint32_t here = smem_u32(sums + tok * W4T_PITCH + r);
+            float v = 0.f;
+            for (int c = 0; c < splits; ++c) {
+                uint32_t there;
+                float f;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(c));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there) : "memory");
+                v += f;
+            }
+            if (!abort_flag) w4_write(o, tok0 + tok, row0 + r, v);
+        }
+        // a CTA's shared memory stays until its peers have read it
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tcgen05_fence_after();
+        tcgen05_dealloc(tmem, S::TMEM);
+    }
+    if (threadIdx.x == 0 && abort_flag && status) atomicExch(status, 13);
+}
+
+// ---------------------------------------------------------------- host side
+// [rows, cols] of 1- or 2-byte numbers, ld apart; a box is 128 bytes of box_rows rows, pieces of 16 bytes swapped as the MMA wants them.
+static int rows_map(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int bytes, int box_rows) {
+    EncodeTiledFn f = encode_fn();
+    if (!f) return RF_ERR_UNSUPPORTED;
+    if ((reinterpret_cast<uintptr_t>(base) & 15) || (ld * bytes) % 16) return RF_ERR_BAD_ARG;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(ld * bytes)};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / bytes), (cuuint32_t)box_rows}, steps[2] = {1, 1};
+    const CUresult r = f(map, bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, steps,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : RF_ERR_BAD_ARG;
+}
+
+template <int BN, bool BYTES, int G>
+static int tc_shared(int blocks, int splits) {
+    using S = TcShape<BN, BYTES, G>;
+    const int all = (blocks + S::BLOCKS - 1) / S::BLOCKS, most = (all + splits - 1) / splits;
+    return S::FIXED + (BYTES ? most * S::PARTS * BN * 4 : 0);
+}
+// f(tokens of a tile, 8-bit rows, group) as constants; false where there is no such kernel
+template <typename F>
+static bool with_tc(int bn, int x_kind, int G, F f) {
+    auto by_group = [&](auto b, auto bytes) {
+        if (G == 32) f(b, bytes, std::integral_constant<int, 32>());
+        else if (G == 64) f(b, bytes, std::integral_constant<int, 64>());
+        else f(b, bytes, std::integral_constant<int, 128>());
+    };
+    auto by_kind = [&](auto b) {
+        if (x_kind == 0) by_group(b, std::true_type());
+        else by_group(b, std::false_type());
+    };
+    if (bn == 32) by_kind(std::integral_constant<int, 32>());
+    else if (bn == 64) by_kind(std::integral_constant<int, 64>());
+    else if (bn == 128) by_kind(std::integral_constant<int, 128>());
+    else return false;
+    return true;
+}
+#define W4T_MOST_SHARED (226 * 1024)                  // (the abort flag has a place of its own)
+
+extern "C" {
+
+// Bytes of shared memory that a block takes with tiles of bn tokens and a share of the columns in `splits` (0: no such kernel).
+int rf_gemm_w4_tc_shared(int x_kind, int K, int G, int bn, int splits) {
+    if (K <= 0 || bad_group(G) || splits < 1) return 0;
+    int bytes = 0;
+    const int blocks = padded(K, G) / 64;
+    with_tc(bn, x_kind, G, [&](auto b, auto kind, auto g) { bytes = tc_shared<decltype(b)::value, decltype(kind)::value, decltype(g)::value>(blocks, splits); });
+    return bytes;
+}
+
+// As rf_gemm_w4 (quantized.cu), with tiles of bn tokens (32, 64, 128); 16-bit rows must start on 16 bytes and lie whole 16 bytes apart.
+int rf_gemm_w4_tc(int x_kind, const void* x, const void* xs, long long ldx, const void* packed, const void* scales, const void* bias, int bias_is_f32,
+                  void* out, int out_is_f32, int add, int bn, int splits, int M, int N, int K, int G, int* status, cudaStream_t st) {
+    if (M <= 0 || N <= 0 || K <= 0 || bad_group(G) || (add && !out_is_f32) || splits < 1 || splits > 8) return RF_ERR_BAD_ARG;
+    if (!aligned(packed, 16) || !aligned(scales, 16)) return RF_ERR_BAD_ARG;
+    const int Kp = padded(K, G), blocks = Kp / 64;
+    const long long x_blocks = (long long)((N + 127) / 128) * splits, y = (M + (long long)bn - 1) / (bn > 0 ? bn : 1);
+    if (x_blocks > 0x7fffffffll || y > 65535) return RF_ERR_UNSUPPORTED;
+    CUtensorMap map;
+    if (const int e = rows_map(&map, x, M, x_kind == 0 ? Kp : K, ldx, x_kind == 0 ? 1 : 2, bn)) return e;
+    const W4Out o{out, bias, bias_is_f32, out_is_f32, add, M, N};
+    int bad = 0;
+    const bool known = with_tc(bn, x_kind, G, [&](auto b, auto kind, auto g) {
+        constexpr int BN = decltype(b)::value, GC = decltype(g)::value;
+        constexpr bool BYTES = decltype(kind)::value;
+        const int smem = tc_shared<BN, BYTES, GC>(blocks, splits);
+        if (smem > W4T_MOST_SHARED) { bad = RF_ERR_UNSUPPORTED; return; }
+        static PerDevice<bool> set;
+        bool& done = set.here();
+        if (!done) {
+            const cudaError_t e = cudaFuncSetAttribute(w4_tc_kernel<BN, BYTES, GC>, cudaFuncAttributeMaxDynamicSharedMemorySize, W4T_MOST_SHARED);
+            if (e != cudaSuccess) { bad = (int)e; return; }
+            done = true;
+        }
+        const dim3 grid((unsigned)x_blocks, (unsigned)y), block(W4T_THREADS);
+        auto go = [&](auto... args) {
+            if (splits > 1) rf_launch_cluster(w4_tc_kernel<BN, BYTES, GC>, grid, block, smem, st, splits, args...);
+            else rf_launch(w4_tc_kernel<BN, BYTES, GC>, grid, block, smem, st, args...);
+        };
+        go(map, (const uint4*)packed, (const uint32_t*)scales, (const float*)xs, blocks, splits, status, o);
+    });
+    if (!known) return RF_ERR_BAD_ARG;
+    if (bad) return bad;
+    RF_LAUNCH_CHECK();
+    return 0;
+}
+
+}  // extern "C"

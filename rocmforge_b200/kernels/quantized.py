@@ -31,9 +31,15 @@ _LAUNCHERS = {
 }
 
 
+_TC_LAUNCHERS = {
+    "rf_gemm_w4_tc_shared": [_i, _i, _i, _i, _i],
+    "rf_gemm_w4_tc": [_i, _p, _p, _n, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p],
+}
+
+
 @functools.lru_cache(None)
 def _f(name: str):
-    return fn("quantized", name, _LAUNCHERS[name])
+    return fn("quantized", name, _LAUNCHERS[name]) if name in _LAUNCHERS else fn("quantized_tc", name, _TC_LAUNCHERS[name])
 
 
 def padded_columns(K: int, group: int) -> int:
@@ -306,6 +312,23 @@ def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
     return best[1:]
 
 
+@functools.lru_cache(4096)
+def w4_tc_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
+    """(tokens of a tile, splits): how ``rf_gemm_w4_tc`` shares out a product, or None where ``rf_gemm_w4`` takes it."""
+    if M <= 16:
+        return None
+    stages, rows = padded_columns(K, group) // (128 if q8 else 64) + 1, (N + 127) // 128
+    bn = 32 if M <= 32 else 64 if M <= 64 else 128
+    tiles, best = rows * ((M + bn - 1) // bn), None
+    for splits in range(1, 9):
+        if _f("rf_gemm_w4_tc_shared")(0 if q8 else 1, K, group, bn, splits) > W4_MOST_SHARED - 1024:
+            continue
+        cost = (tiles + clusters_of(splits) - 1) // clusters_of(splits) * ((stages + splits - 1) // splits + 6) + 2 * (splits > 1)
+        if best is None or cost < best[0]:
+            best = cost, bn, splits
+    return best and best[1:]
+
+
 @functools.lru_cache(None)
 def _clusters_on(device: int):
     return functools.partial(w4_clusters, device=device)
@@ -346,6 +369,14 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
     if not q8 and (dt == torch.float32 or M > W4_FEW_TOKENS):
         return _gemm_through_16_bits(x, w, bias, out, accumulate)
     at, ld = rows.data_ptr(), rows.stride(0)
+    whole = q8 or (ld % 8 == 0 and at % 16 == 0)
+    tiled = w4_tc_launch(q8, M, N, K, w.group, _clusters_on(rows.get_device())) if whole else None
+    if tiled:
+        code = _f("rf_gemm_w4_tc")(0 if q8 else 1, at, x.scales.data_ptr() if q8 else None, ld, w.packed.data_ptr(), w.scales.data_ptr(), ptr(bias),
+                                   bias is not None and bias.dtype == torch.float32, out.data_ptr(), odt == torch.float32, accumulate, *tiled,
+                                   M, N, K, w.group, tc.status_word(rows.device).data_ptr(), stream())
+        check(code, "gemm_w4" if code == 0 else f"gemm_w4 ({M}x{N}x{K}, tiles of {tiled[0]} tokens)")
+        return out
     eights, ways, splits, clusters = w4_launch(q8, M, N, K, w.group, _clusters_on(rows.get_device()))
     code = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales.data_ptr() if q8 else None, ld, w.packed.data_ptr(), w.scales.data_ptr(), ptr(bias),
                             bias is not None and bias.dtype == torch.float32, out.data_ptr(), odt == torch.float32, accumulate, eights, ways, splits,
