@@ -4,7 +4,7 @@
 // their tile of 16 rows as it is stored (asynchronous copies into a ring of their own, far ahead, and before the wait for the kernel
 // before), widen it and write it where the MMA reads it; the tokens' numbers come by TMA.  A stage is 128 bytes of a row:
 //   16-bit rows: 64 columns; the weights become bfloat16 numbers, scale and all (exactly, with scales of five significant bits; others are
-//     rounded), and the whole product is one accumulator's.
+//     rounded), and the whole product is one accumulator's.  Two groups of eight warps widen every second stage each.
 //   8-bit rows: 128 columns; the weights become 16 q as signed bytes and a group's sum is exact in whole numbers, in an accumulator of its own,
 //     which eight more warps read, scale by both scales and add to their 32-bit sums while the next groups are multiplied.
 // Long rows are shared out to the CTAs of a cluster, which add up their sums through shared memory in the order of their ranks.
@@ -19,16 +19,36 @@
 
 template <int BN, bool BYTES, int G>
 struct TcShape {
-    static constexpr int A = 128 * 128, B = BN * 128, STAGE = A + B, STAGES = BN <= 64 ? 4 : 3;
+    static constexpr int A = 128 * 128, B = BN * 128, STAGE = A + B;
+    static constexpr int WIDENS = BYTES ? 1 : 2;         // groups of widening warps: a group must see every second phase of a stage's barriers, or all
+    static constexpr int STAGES = BYTES && BN == 128 ? 3 : 4;
     static constexpr int BLOCKS = BYTES ? 2 : 1;         // blocks of 64 columns a stage
     static constexpr int PARTS = BYTES ? 128 / G : 1;    // accumulators a stage
     static constexpr int BUFS = BYTES ? (BN <= 64 ? 4 : 2) : 1;
     static constexpr int TMEM = BUFS * BN < 32 ? 32 : BUFS * BN;
     static constexpr int SCALES = BYTES ? 0 : (G == 32 ? 2 : 1);        // groups whose scales travel with a stage
-    static constexpr int SLOT = BLOCKS * 512 + SCALES * 32, DEPTH = BYTES ? 8 : 14, RING = 8 * DEPTH * SLOT;
+    static constexpr int SLOT = BLOCKS * 512 + SCALES * 32, DEPTH = 8, RING = 8 * WIDENS * DEPTH * SLOT;
     static constexpr int FIXED = STAGES * STAGE + RING + 1024 + 256;    // (alignment, barriers)
     static_assert(STAGES * STAGE >= BN * W4T_PITCH * 4, "the stages' place holds the sums");
+    static_assert(STAGES % WIDENS == 0, "one parity bit tells two phases apart, not three");
 };
+
+// Bounded wait as mbar_wait, asleep between looks: what waits here waits long, and the widening warps need the issue slots.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long t0 = global_ns();
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > TC_WAIT_LIMIT_NS) { *abort_flag = 1; return false; }
+    }
+}
 
 template <int BN, bool BYTES>
 __device__ __forceinline__ void mma_step(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
@@ -41,11 +61,31 @@ __device__ __forceinline__ void mma_step(uint32_t d, uint64_t a, uint64_t b, uin
     }
 }
 
-// Four halves of bytes of a word as bfloat16 numbers times a scale, pairs in the order of the columns: `w` has its middle bytes swapped.
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t shared4(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void to_shared8(uint32_t at, uint32_t a, uint32_t b) {
+    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(a), "r"(b) : "memory");
+}
+// Two halves of bytes, 16 bits apart, as bfloat16 numbers times a scale.
 __device__ __forceinline__ uint32_t widened(uint32_t w, __nv_bfloat162 s) {
     uint32_t v = (w & 0x000f000fu) ^ 0x43084308u;        // 128 + (q + 8)
     const __nv_bfloat162 r = __hmul2(__hadd2(*reinterpret_cast<__nv_bfloat162*>(&v), __float2bfloat162_rn(-136.f)), s);
     return *reinterpret_cast<const uint32_t*>(&r);
+}
+// A word's eight columns into 16 bytes of shared memory; with the middle bytes swapped, neighbours are 16 bits apart.
+__device__ __forceinline__ void four_pairs(uint32_t at, uint32_t word, uint32_t scale_twice) {
+    const uint32_t w = __byte_perm(word, 0, 0x3120);
+    const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&scale_twice);
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(at), "r"(widened(w, s)), "r"(widened(w >> 8, s)), "r"(widened(w >> 4, s)), "r"(widened(w >> 12, s)) : "memory");
 }
 
 template <int BN, bool BYTES, int G>
@@ -83,19 +123,25 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
         tcgen05_alloc(smem_u32(tmem_slot), S::TMEM);
         tcgen05_relinquish();
     }
-    // the widening warps' rings, filled before anything is waited for
-    const int wide = warp - 2, tile = row0 / 16 + wide;
-    const bool widens = wide >= 0 && wide < 8, mine = widens && tile < tiles;
-    const uint32_t ring = smem_u32(smem) + S::STAGES * S::STAGE + wide * S::DEPTH * S::SLOT;
-    auto ask = [&](int i) {
-        if (mine && i < n) {
-            const uint32_t to = ring + i % S::DEPTH * S::SLOT;
-            const int block = (from + i) * S::BLOCKS;
-            const uint4* p = w0 + ((size_t)tile * blocks + block) * 32 + lane;
-            copy16(to + 16 * lane, p, true);
-            if (S::BLOCKS == 2) copy16(to + 512 + 16 * lane, block + 1 < blocks ? p + 32 : p, block + 1 < blocks);
-            if (S::SCALES && lane < 2 * S::SCALES)       // the 16 rows' scales of a group are 32 bytes
-                copy16(to + 512 + 16 * lane, reinterpret_cast<const uint4*>(w1) + ((size_t)tile * all_groups + (from + i) * 64 / G) * 2 + lane, true);
+    // the widening warps' rings, filled before anything is waited for: stages phase, phase + WIDENS, ... of a tile of 16 rows
+    const int wide = warp - 2, tile = row0 / 16 + (wide & 7), phase = wide >> 3;
+    const bool widens = wide >= 0 && wide < 8 * S::WIDENS, mine = widens && tile < tiles;
+    const uint32_t ring = smem_u32(smem) + S::STAGES * S::STAGE + (widens ? wide : 0) * S::DEPTH * S::SLOT + 16 * lane;
+    constexpr int STEP = S::WIDENS * S::BLOCKS;          // blocks from one of a warp's stages to its next
+    const int block0 = (from + phase) * S::BLOCKS;
+    const uint4* next_w = w0 + ((size_t)tile * blocks + block0) * 32 + lane;
+    const uint4* next_s = reinterpret_cast<const uint4*>(w1) + ((size_t)tile * all_groups + block0 * 64 / G) * 2 + lane;
+    int left = mine ? (n - phase + S::WIDENS - 1) / S::WIDENS : 0, next_block = block0;
+    auto ask = [&](int slot) {
+        if (left > 0) {
+            const uint32_t to = ring + slot * S::SLOT;
+            copy16(to, next_w, true);
+            if (S::BLOCKS == 2) copy16(to + 512, next_block + 1 < blocks ? next_w + 32 : next_w, next_block + 1 < blocks);
+            if (S::SCALES && lane < 2 * S::SCALES) copy16(to + 512, next_s, true);      // the 16 rows' scales of a group are 32 bytes
+            next_w += 32 * STEP;
+            if constexpr (S::SCALES > 0) next_s += 2 * STEP * 64 / G;                   // (two stages on are whole groups on)
+            next_block += STEP;
+            --left;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -115,7 +161,7 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
             pdl_wait();
             for (int i = 0; i < n; ++i) {
                 const int s = i % S::STAGES;
-                if (i >= S::STAGES && !mbar_wait(smem_u32(&bars[EMPTY + s]), ((i / S::STAGES) & 1) ^ 1, &abort_flag)) break;
+                if (i >= S::STAGES && !wait_for(smem_u32(&bars[EMPTY + s]), ((i / S::STAGES) & 1) ^ 1, &abort_flag)) break;
                 mbar_expect_tx(smem_u32(&bars[FULL + s]), S::B);
                 tma_load_2d(smem_u32(smem) + s * S::STAGE + S::A, &map_x, (from + i) * S::BLOCKS * 64, tok0, smem_u32(&bars[FULL + s]));
             }
@@ -126,7 +172,7 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
             int sum = 0;
             for (int i = 0; i < n && ok; ++i) {
                 const int s = i % S::STAGES;
-                ok = mbar_wait(smem_u32(&bars[FULL + s]), (i / S::STAGES) & 1, &abort_flag);
+                ok = wait_for(smem_u32(&bars[FULL + s]), (i / S::STAGES) & 1, &abort_flag);
                 if (!ok) break;
                 tcgen05_fence_after();
                 const uint64_t da = make_smem_desc(smem_u32(smem) + s * S::STAGE), db = make_smem_desc(smem_u32(smem) + s * S::STAGE + S::A);
@@ -135,7 +181,7 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
                     for (int p = 0; p < S::PARTS && ok; ++p, ++sum) {
                         const int buf = sum % S::BUFS;
                         if (sum >= S::BUFS) {
-                            ok = mbar_wait(smem_u32(&bars[SUM_EMPTY + buf]), ((sum / S::BUFS) & 1) ^ 1, &abort_flag);
+                            ok = wait_for(smem_u32(&bars[SUM_EMPTY + buf]), ((sum / S::BUFS) & 1) ^ 1, &abort_flag);
                             tcgen05_fence_after();
                         }
                         if (!ok) break;
@@ -157,47 +203,46 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
     } else if (widens) {
         // ---------------- the weights
         const int g = lane >> 2, t = lane & 3;
-        for (int i = 0; i < n; ++i) {
+        const bool odd = g & 1;
+        const uint32_t here0 = smem_u32(smem) + S::STAGES * S::STAGE + wide * S::DEPTH * S::SLOT;
+        const uint32_t row = smem_u32(smem) + (16 * (wide & 7) + g) * 128;              // (rows of 128 bytes, 16-byte pieces swapped by row % 8 = g)
+        int slot = 0;
+        for (int i = phase; i < n; i += S::WIDENS) {
             const int s = i % S::STAGES;
             asm volatile("cp.async.wait_group %0;" ::"n"(S::DEPTH - 1) : "memory");
             __syncwarp();
-            const uint8_t* here = smem + S::STAGES * S::STAGE + (wide * S::DEPTH + i % S::DEPTH) * S::SLOT;
+            const uint32_t here = here0 + slot * S::SLOT;
             uint4 w[S::BLOCKS];
             uint32_t sc[S::SCALES ? S::SCALES : 1];
 #pragma unroll
-            for (int b = 0; b < S::BLOCKS; ++b) w[b] = *reinterpret_cast<const uint4*>(here + 512 * b + 16 * lane);
+            for (int b = 0; b < S::BLOCKS; ++b) w[b] = shared16(here + 512 * b + 16 * lane);
 #pragma unroll
-            for (int p = 0; p < S::SCALES; ++p) sc[p] = *reinterpret_cast<const uint32_t*>(here + 512 + 32 * p + 4 * g);
-            __syncwarp();                                // all have read the slot
-            ask(i + S::DEPTH);
-            if (i >= S::STAGES && !mbar_wait(smem_u32(&bars[EMPTY + s]), ((i / S::STAGES) & 1) ^ 1, &abort_flag)) break;
-            if (mine) {
-                uint8_t* to = smem + s * S::STAGE + (16 * wide + g) * 128;              // (rows of 128 bytes, 16-byte pieces swapped by row % 8 = g)
-                if constexpr (BYTES) {
+            for (int p = 0; p < S::SCALES; ++p) sc[p] = shared4(here + 512 + 32 * p + 4 * g);
+            if (S::SCALES) __syncwarp();                 // all have read the slot (without scales a lane reads what it copies itself)
+            ask(slot);
+            slot = (slot + 1) % S::DEPTH;
+            if (i >= S::STAGES && !wait_for(smem_u32(&bars[EMPTY + s]), ((i / S::STAGES) & 1) ^ 1, &abort_flag)) break;
+            const uint32_t to = row + s * S::STAGE;
+            if constexpr (BYTES) {
+                // by the row's parity the other block first: four rows' pieces then meet all banks
+                const uint4 v[2] = {odd ? w[1] : w[0], odd ? w[0] : w[1]};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {        // by the row's parity another block first: four rows' pieces then meet all banks
-                        const int b = (j >> 1) ^ (g & 1), c = j & 1;
-                        const uint4 v = b ? w[1] : w[0];
-                        const int at = ((4 * b + 2 * c + (t >> 1)) ^ g) * 16 + (t & 1) * 8;
-                        const uint32_t m = 0xf0f0f0f0u, lo = c ? v.y : v.x, hi = c ? v.w : v.z;
-                        *reinterpret_cast<uint2*>(to + at) = make_uint2(lo << 4 & m, lo & m);
-                        *reinterpret_cast<uint2*>(to + 8 * 128 + at) = make_uint2(hi << 4 & m, hi & m);
-                    }
-                } else {
+                for (int j = 0; j < 4; ++j) {
+                    const int c = j & 1;
+                    const uint32_t at = (((4 * (odd ^ (j >> 1)) + 2 * c + (t >> 1)) ^ g) * 16) + (t & 1) * 8, m = 0xf0f0f0f0u;
+                    const uint32_t lo = c ? v[j >> 1].y : v[j >> 1].x, hi = c ? v[j >> 1].w : v[j >> 1].z;
+                    to_shared8(to + at, lo << 4 & m, lo & m);
+                    to_shared8(to + 1024 + at, hi << 4 & m, hi & m);
+                }
+            } else {
+                // by the row's parity the other half first: two rows' pieces then meet all banks
+                const uint32_t lo[2] = {odd ? w[0].y : w[0].x, odd ? w[0].x : w[0].y}, hi[2] = {odd ? w[0].w : w[0].z, odd ? w[0].z : w[0].w};
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int c = j ^ (g & 1);       // two rows' pieces then meet all banks
-                        const uint32_t s2 = S::SCALES == 2 && c ? sc[S::SCALES - 1] : sc[0];
-                        const int at = ((4 * c + t) ^ g) * 16;
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const uint32_t word = __byte_perm(r ? (c ? w[0].w : w[0].z) : (c ? w[0].y : w[0].x), 0, 0x3120);
-                            const uint32_t both = __byte_perm(s2, 0, r ? 0x3232 : 0x1010);
-                            const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&both);
-                            *reinterpret_cast<uint4*>(to + r * 8 * 128 + at) =
-                                make_uint4(widened(word, f), widened(word >> 8, f), widened(word >> 4, f), widened(word >> 12, f));
-                        }
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t s2 = S::SCALES == 2 ? (odd ^ j ? sc[S::SCALES - 1] : sc[0]) : sc[0];
+                    const uint32_t at = to + (((4 * (odd ^ j) + t) ^ g) * 16);
+                    four_pairs(at, lo[j], __byte_perm(s2, 0, 0x1010));
+                    four_pairs(at + 1024, hi[j], __byte_perm(s2, 0, 0x3232));
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -205,9 +250,10 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
             if (lane == 0) at_arrive(smem_u32(&bars[FULL + s]));
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-    } else {
+    }
+    pdl_wait(xs);                                        // (whoever writes from here on has waited)
+    if (add >= 0) {
         // ---------------- the sums
-        pdl_wait(xs);
         const int row = row0 + 32 * quarter + lane;
         if constexpr (BYTES) {
             const int first = from * S::PARTS, count = n * S::PARTS;
@@ -219,12 +265,11 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
             const __nv_bfloat16* ws = reinterpret_cast<const __nv_bfloat16*>(w1) + (size_t)(row / 16) * all_groups * 16 + 2 * (row % 8) + row % 16 / 8;
             auto scale_of = [&](int i) { return row < o.N && first + i < all_groups && i < count ? __bfloat162float(ws[(size_t)(first + i) * 16]) * 0.0625f : 0.f; };
             float next = scale_of(0);
-            const Two less = two(-12582912.f, -12582912.f);
             for (int i = 0; i < count && ok; ++i) {
                 const int buf = i % S::BUFS;
                 const float f = next;
                 next = scale_of(i + 1);
-                ok = mbar_wait(smem_u32(&bars[SUM_FULL + buf]), (i / S::BUFS) & 1, &abort_flag);
+                ok = wait_for(smem_u32(&bars[SUM_FULL + buf]), (i / S::BUFS) & 1, &abort_flag);
                 if (!ok) break;
                 tcgen05_fence_after();
                 constexpr int CH = 16;                   // (32 numbers beside the sums would not fit the registers)
@@ -244,20 +289,17 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
 #pragma unroll
                     for (int j = 0; j < CH; j += 4) {
                         const float4 x = *reinterpret_cast<const float4*>(a + j);
-                        // a whole number below 2^22 as a float: in the last bits of 1.5 2^23
-                        const Two v0 = add2(two(__uint_as_float(r[j] + 0x4b400000u), __uint_as_float(r[j + 1] + 0x4b400000u)), less);
-                        const Two v1 = add2(two(__uint_as_float(r[j + 2] + 0x4b400000u), __uint_as_float(r[j + 3] + 0x4b400000u)), less);
+                        const Two v0 = two((float)(int)r[j], (float)(int)r[j + 1]), v1 = two((float)(int)r[j + 2], (float)(int)r[j + 3]);     // (exact)
                         acc[(c + j) / 2] = fma2(v0, mul2(two(x.x, x.y), ff), acc[(c + j) / 2]);
                         acc[(c + j) / 2 + 1] = fma2(v1, mul2(two(x.z, x.w), ff), acc[(c + j) / 2 + 1]);
                     }
                 }
             }
         } else if (n > 0) {
-            ok = mbar_wait(smem_u32(&bars[SUM_FULL]), 0, &abort_flag);
+            ok = wait_for(smem_u32(&bars[SUM_FULL]), 0, &abort_flag);
             tcgen05_fence_after();
         }
     }
-    pdl_wait();                                          // (who writes below may not have waited yet)
     __syncwarp();
     // a cluster's sums go through the stages' place; one CTA's straight out
     if (splits > 1) __syncthreads();                     // (the last sums were there: every product has read its stages)
