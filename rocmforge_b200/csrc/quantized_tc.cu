@@ -26,16 +26,16 @@ struct TcShape {
     static constexpr int PARTS = BYTES ? 128 / G : 1;    // accumulators a stage
     static constexpr int BUFS = BYTES ? (BN <= 64 ? 4 : 2) : 1;
     static constexpr int TMEM = BUFS * BN < 32 ? 32 : BUFS * BN;
-    static constexpr int SCALES = BYTES ? 0 : (G == 32 ? 2 : 1);        // groups whose scales travel with a stage
-    static constexpr int SLOT = BLOCKS * 512 + SCALES * 32, DEPTH = 8, RING = 8 * WIDENS * DEPTH * SLOT;
-    static constexpr int FIXED = STAGES * STAGE + RING + 1024 + 256;    // (alignment, barriers)
+    static constexpr int SCALES = BYTES ? 0 : (G == 32 ? 2 : 1);        // groups of a stage whose scales the weights take
+    static constexpr int TURN = STAGES / WIDENS;         // a warp's stages until it is back at the same place
+    static constexpr int AHEAD = (BYTES ? 2 : 4) / TURN * TURN < TURN ? TURN : (BYTES ? 2 : 4) / TURN * TURN;      // its stages whose weights it has asked for
+    static constexpr int FIXED = STAGES * STAGE + 1024 + 256;           // (alignment, barriers)
     static_assert(STAGES * STAGE >= BN * W4T_PITCH * 4, "the stages' place holds the sums");
     static_assert(STAGES % WIDENS == 0, "one parity bit tells two phases apart, not three");
 };
 
 // Bounded wait as mbar_wait, asleep between looks: what waits here waits long, and the widening warps need the issue slots.
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    if (mbar_try_wait(bar, parity)) return true;
+__device__ __noinline__ bool wait_asleep(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     const unsigned long long t0 = global_ns();
     for (;;) {
         uint32_t ok;
@@ -49,6 +49,9 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile
         if (global_ns() - t0 > TC_WAIT_LIMIT_NS) { *abort_flag = 1; return false; }
     }
 }
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    return mbar_try_wait(bar, parity) || wait_asleep(bar, parity, abort_flag);
+}
 
 template <int BN, bool BYTES>
 __device__ __forceinline__ void mma_step(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
@@ -61,16 +64,6 @@ __device__ __forceinline__ void mma_step(uint32_t d, uint64_t a, uint64_t b, uin
     }
 }
 
-__device__ __forceinline__ uint4 shared16(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint32_t shared4(uint32_t at) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    return v;
-}
 __device__ __forceinline__ void to_shared8(uint32_t at, uint32_t a, uint32_t b) {
     asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(a), "r"(b) : "memory");
 }
@@ -94,11 +87,11 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
     using S = TcShape<BN, BYTES, G>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE + S::RING);       // full, empty, sum full, sum empty
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE);       // full, empty, sum full, sum empty
     constexpr int FULL = 0, EMPTY = S::STAGES, SUM_FULL = 2 * S::STAGES, SUM_EMPTY = SUM_FULL + S::BUFS, BARS = SUM_EMPTY + S::BUFS;
     static_assert(BARS * 8 + 4 <= 256, "room for the barriers");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
-    float* scales = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE + S::RING + 256);     // 8-bit rows: [group][token]
+    float* scales = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE + 256);     // 8-bit rows: [group][token]
     __shared__ int abort_flag;
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -123,30 +116,30 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
         tcgen05_alloc(smem_u32(tmem_slot), S::TMEM);
         tcgen05_relinquish();
     }
-    // the widening warps' rings, filled before anything is waited for: stages phase, phase + WIDENS, ... of a tile of 16 rows
-    const int wide = warp - 2, tile = row0 / 16 + (wide & 7), phase = wide >> 3;
-    const bool widens = wide >= 0 && wide < 8 * S::WIDENS, mine = widens && tile < tiles;
-    const uint32_t ring = smem_u32(smem) + S::STAGES * S::STAGE + (widens ? wide : 0) * S::DEPTH * S::SLOT + 16 * lane;
+    // the widening warps' weights: stages phase, phase + WIDENS, ... of a tile of 16 rows, AHEAD of them in registers before anything is waited for
+    const int wide = warp - 2, tile = min(row0 / 16 + (wide & 7), tiles - 1), phase = wide >> 3;        // (rows that are not there: some others)
+    const bool widens = wide >= 0 && wide < 8 * S::WIDENS;
     constexpr int STEP = S::WIDENS * S::BLOCKS;          // blocks from one of a warp's stages to its next
-    const int block0 = (from + phase) * S::BLOCKS;
+    const int block0 = (from + phase) * S::BLOCKS, stages = widens ? (n - phase + S::WIDENS - 1) / S::WIDENS : 0;
     const uint4* next_w = w0 + ((size_t)tile * blocks + block0) * 32 + lane;
-    const uint4* next_s = reinterpret_cast<const uint4*>(w1) + ((size_t)tile * all_groups + block0 * 64 / G) * 2 + lane;
-    int left = mine ? (n - phase + S::WIDENS - 1) / S::WIDENS : 0, next_block = block0;
-    auto ask = [&](int slot) {
-        if (left > 0) {
-            const uint32_t to = ring + slot * S::SLOT;
-            copy16(to, next_w, true);
-            if (S::BLOCKS == 2) copy16(to + 512, next_block + 1 < blocks ? next_w + 32 : next_w, next_block + 1 < blocks);
-            if (S::SCALES && lane < 2 * S::SCALES) copy16(to + 512, next_s, true);      // the 16 rows' scales of a group are 32 bytes
+    const uint32_t* next_s = w1 + ((size_t)tile * all_groups + block0 * 64 / G) * 8 + (lane >> 2);
+    uint4 w[S::AHEAD][S::BLOCKS];
+    uint32_t sc[S::AHEAD][S::SCALES ? S::SCALES : 1];
+    int asked = 0;
+    auto ask = [&](int into) {
+        if (asked < stages) {
+            w[into][0] = *next_w;
+            if constexpr (S::BLOCKS == 2)                // (the last stage's second block may not be there)
+                w[into][1] = asked + 1 < stages || block0 + S::BLOCKS * stages <= blocks ? next_w[32] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int p = 0; p < S::SCALES; ++p) sc[into][p] = next_s[8 * p];
             next_w += 32 * STEP;
-            if constexpr (S::SCALES > 0) next_s += 2 * STEP * 64 / G;                   // (two stages on are whole groups on)
-            next_block += STEP;
-            --left;
+            if constexpr (S::SCALES > 0) next_s += 8 * STEP * 64 / G;                   // (two stages on are whole groups on)
+            ++asked;
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (widens)
-        for (int i = 0; i < S::DEPTH; ++i) ask(i);
+#pragma unroll
+    for (int i = 0; i < S::AHEAD; ++i) ask(i);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -204,52 +197,52 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
         // ---------------- the weights
         const int g = lane >> 2, t = lane & 3;
         const bool odd = g & 1;
-        const uint32_t here0 = smem_u32(smem) + S::STAGES * S::STAGE + wide * S::DEPTH * S::SLOT;
         const uint32_t row = smem_u32(smem) + (16 * (wide & 7) + g) * 128;              // (rows of 128 bytes, 16-byte pieces swapped by row % 8 = g)
-        int slot = 0;
-        for (int i = phase; i < n; i += S::WIDENS) {
-            const int s = i % S::STAGES;
-            asm volatile("cp.async.wait_group %0;" ::"n"(S::DEPTH - 1) : "memory");
-            __syncwarp();
-            const uint32_t here = here0 + slot * S::SLOT;
-            uint4 w[S::BLOCKS];
-            uint32_t sc[S::SCALES ? S::SCALES : 1];
+        const uint32_t full = smem_u32(&bars[FULL + phase]), empty = smem_u32(&bars[EMPTY + phase]);
+        // where this lane's pieces of a stage go: by the row's parity the other half (8-bit rows: block) first, and rows' pieces meet all banks
+        uint32_t place[BYTES ? 4 : 2];
+        if constexpr (BYTES) {
 #pragma unroll
-            for (int b = 0; b < S::BLOCKS; ++b) w[b] = shared16(here + 512 * b + 16 * lane);
+            for (int j = 0; j < 4; ++j) place[j] = row + (((4 * (odd ^ (j >> 1)) + 2 * (j & 1) + (t >> 1)) ^ g) * 16) + (t & 1) * 8;
+        } else {
 #pragma unroll
-            for (int p = 0; p < S::SCALES; ++p) sc[p] = shared4(here + 512 + 32 * p + 4 * g);
-            if (S::SCALES) __syncwarp();                 // all have read the slot (without scales a lane reads what it copies itself)
-            ask(slot);
-            slot = (slot + 1) % S::DEPTH;
-            if (i >= S::STAGES && !wait_for(smem_u32(&bars[EMPTY + s]), ((i / S::STAGES) & 1) ^ 1, &abort_flag)) break;
-            const uint32_t to = row + s * S::STAGE;
-            if constexpr (BYTES) {
-                // by the row's parity the other block first: four rows' pieces then meet all banks
-                const uint4 v[2] = {odd ? w[1] : w[0], odd ? w[0] : w[1]};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int c = j & 1;
-                    const uint32_t at = (((4 * (odd ^ (j >> 1)) + 2 * c + (t >> 1)) ^ g) * 16) + (t & 1) * 8, m = 0xf0f0f0f0u;
-                    const uint32_t lo = c ? v[j >> 1].y : v[j >> 1].x, hi = c ? v[j >> 1].w : v[j >> 1].z;
-                    to_shared8(to + at, lo << 4 & m, lo & m);
-                    to_shared8(to + 1024 + at, hi << 4 & m, hi & m);
-                }
-            } else {
-                // by the row's parity the other half first: two rows' pieces then meet all banks
-                const uint32_t lo[2] = {odd ? w[0].y : w[0].x, odd ? w[0].x : w[0].y}, hi[2] = {odd ? w[0].w : w[0].z, odd ? w[0].z : w[0].w};
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t s2 = S::SCALES == 2 ? (odd ^ j ? sc[S::SCALES - 1] : sc[0]) : sc[0];
-                    const uint32_t at = to + (((4 * (odd ^ j) + t) ^ g) * 16);
-                    four_pairs(at, lo[j], __byte_perm(s2, 0, 0x1010));
-                    four_pairs(at + 1024, hi[j], __byte_perm(s2, 0, 0x3232));
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) at_arrive(smem_u32(&bars[FULL + s]));
+            for (int j = 0; j < 2; ++j) place[j] = row + (((4 * (odd ^ j) + t) ^ g) * 16);
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        uint32_t parity = 1;
+        for (int done = 0; done < stages && ok;) {
+#pragma unroll
+            for (int u = 0; u < S::AHEAD; ++u, ++done) {
+                if (done >= stages) break;
+                const uint32_t to = phase * S::STAGE + u % S::TURN * S::WIDENS * S::STAGE;
+                if (done >= S::TURN) {
+                    ok = wait_for(empty + u % S::TURN * S::WIDENS * 8, parity, &abort_flag);
+                    if (!ok) break;
+                }
+                if constexpr (BYTES) {
+                    const uint4 v[2] = {odd ? w[u][1] : w[u][0], odd ? w[u][0] : w[u][1]};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t m = 0xf0f0f0f0u, lo = j & 1 ? v[j >> 1].y : v[j >> 1].x, hi = j & 1 ? v[j >> 1].w : v[j >> 1].z;
+                        to_shared8(place[j] + to, lo << 4 & m, lo & m);
+                        to_shared8(place[j] + to + 1024, hi << 4 & m, hi & m);
+                    }
+                } else {
+                    const uint4 v = w[u][0];
+                    const uint32_t lo[2] = {odd ? v.y : v.x, odd ? v.x : v.y}, hi[2] = {odd ? v.w : v.z, odd ? v.z : v.w};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t s2 = S::SCALES == 2 ? (odd ^ j ? sc[u][S::SCALES - 1] : sc[u][0]) : sc[u][0];
+                        four_pairs(place[j] + to, lo[j], __byte_perm(s2, 0, 0x1010));
+                        four_pairs(place[j] + to + 1024, hi[j], __byte_perm(s2, 0, 0x3232));
+                    }
+                }
+                ask(u);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) at_arrive(full + u % S::TURN * S::WIDENS * 8);
+                if (u % S::TURN == S::TURN - 1) parity ^= 1;
+            }
+        }
     }
     pdl_wait(xs);                                        // (whoever writes from here on has waited)
     if (add >= 0) {
@@ -262,33 +255,36 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
                 scales[gr * BN + tok] = first + gr < all_groups ? xs[(size_t)(tok0 + tok) * all_groups + first + gr] : 0.f;
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            const __nv_bfloat16* ws = reinterpret_cast<const __nv_bfloat16*>(w1) + (size_t)(row / 16) * all_groups * 16 + 2 * (row % 8) + row % 16 / 8;
-            auto scale_of = [&](int i) { return row < o.N && first + i < all_groups && i < count ? __bfloat162float(ws[(size_t)(first + i) * 16]) * 0.0625f : 0.f; };
-            float next = scale_of(0);
-            for (int i = 0; i < count && ok; ++i) {
+            // this row's scales; what lies behind the last row or group is read from it and meets tokens' scales of zero, or is not written
+            const int r = min(row, 16 * tiles - 1);
+            const __nv_bfloat16* ws = reinterpret_cast<const __nv_bfloat16*>(w1) + ((size_t)(r / 16) * all_groups + first) * 16 + 2 * (r % 8) + r % 16 / 8;
+            const int last = all_groups - 1 - first;
+            float next = __bfloat162float(ws[0]);
+            const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + cols0;
+            const float* a = scales + cols0;
+            for (int i = 0; i < count && ok; ++i, a += BN) {
                 const int buf = i % S::BUFS;
-                const float f = next;
-                next = scale_of(i + 1);
+                const float f = next * 0.0625f;          // (the products hold 16 q)
+                next = __bfloat162float(ws[(size_t)min(i + 1, last) * 16]);
                 ok = wait_for(smem_u32(&bars[SUM_FULL + buf]), (i / S::BUFS) & 1, &abort_flag);
                 if (!ok) break;
                 tcgen05_fence_after();
-                constexpr int CH = 16;                   // (32 numbers beside the sums would not fit the registers)
+                constexpr int CH = BN == 64 ? 32 : 16;   // (32 numbers beside 64 sums would not fit the registers)
                 const Two ff = two(f, f);
 #pragma unroll
                 for (int c = 0; c < BN / 2; c += CH) {
                     uint32_t r[CH];
-                    const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + cols0 + c;
-                    tcgen05_ld16(at, r);
+                    if constexpr (CH == 32) tcgen05_ld32(lanes + buf * BN + c, r);
+                    else tcgen05_ld16(lanes + buf * BN + c, r);
                     tcgen05_wait_ld();
                     if (c + CH == BN / 2) {
                         tcgen05_fence_before();
                         __syncwarp();
                         if (lane == 0) at_arrive(smem_u32(&bars[SUM_EMPTY + buf]));
                     }
-                    const float* a = scales + i * BN + cols0 + c;
 #pragma unroll
                     for (int j = 0; j < CH; j += 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(a + j);
+                        const float4 x = *reinterpret_cast<const float4*>(a + c + j);
                         const Two v0 = two((float)(int)r[j], (float)(int)r[j + 1]), v1 = two((float)(int)r[j + 2], (float)(int)r[j + 3]);     // (exact)
                         acc[(c + j) / 2] = fma2(v0, mul2(two(x.x, x.y), ff), acc[(c + j) / 2]);
                         acc[(c + j) / 2 + 1] = fma2(v1, mul2(two(x.z, x.w), ff), acc[(c + j) / 2 + 1]);
