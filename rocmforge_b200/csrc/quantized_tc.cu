@@ -19,9 +19,10 @@
 
 template <int BN, bool BYTES, int G>
 struct TcShape {
-    static constexpr int A = 128 * 128, B = BN * 128, STAGE = A + B;
+    static constexpr int A = 128 * 128, B = BN * 128;
     static constexpr int WIDENS = BYTES ? 1 : 2;         // groups of widening warps: a group must see every second phase of a stage's barriers, or all
-    static constexpr int STAGES = BYTES && BN == 128 ? 3 : 4;
+    static constexpr int STAGES = 4, ROWS = BYTES && BN == 128 ? 4 : 8;                // places of weights and, further ahead, of tokens' numbers
+    static constexpr int RINGS = STAGES * A + ROWS * B;
     static constexpr int BLOCKS = BYTES ? 2 : 1;         // blocks of 64 columns a stage
     static constexpr int PARTS = BYTES ? 128 / G : 1;    // accumulators a stage
     static constexpr int BUFS = BYTES ? (BN <= 64 ? 4 : 2) : 1;
@@ -29,9 +30,10 @@ struct TcShape {
     static constexpr int SCALES = BYTES ? 0 : (G == 32 ? 2 : 1);        // groups of a stage whose scales the weights take
     static constexpr int TURN = STAGES / WIDENS;         // a warp's stages until it is back at the same place
     static constexpr int AHEAD = (BYTES ? 2 : 4) / TURN * TURN < TURN ? TURN : (BYTES ? 2 : 4) / TURN * TURN;      // its stages whose weights it has asked for
-    static constexpr int FIXED = STAGES * STAGE + 1024 + 256;           // (alignment, barriers)
-    static_assert(STAGES * STAGE >= BN * W4T_PITCH * 4, "the stages' place holds the sums");
+    static constexpr int FIXED = RINGS + 1024 + 512;           // (alignment, barriers)
+    static_assert(RINGS >= BN * W4T_PITCH * 4, "the stages' place holds the sums");
     static_assert(STAGES % WIDENS == 0, "one parity bit tells two phases apart, not three");
+    static_assert(8 % ROWS == 0 && 8 % STAGES == 0 && 8 * PARTS % (2 * BUFS) == 0, "eight stages on, every ring is back where it was");
 };
 
 // Bounded wait as mbar_wait, asleep between looks: what waits here waits long, and the widening warps need the issue slots.
@@ -87,11 +89,12 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
     using S = TcShape<BN, BYTES, G>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE);       // full, empty, sum full, sum empty
-    constexpr int FULL = 0, EMPTY = S::STAGES, SUM_FULL = 2 * S::STAGES, SUM_EMPTY = SUM_FULL + S::BUFS, BARS = SUM_EMPTY + S::BUFS;
-    static_assert(BARS * 8 + 4 <= 256, "room for the barriers");
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::RINGS);     // weights' places full, empty, tokens' full, empty, sums full, empty
+    constexpr int FULL = 0, EMPTY = S::STAGES, ROWS_FULL = 2 * S::STAGES, ROWS_EMPTY = ROWS_FULL + S::ROWS, SUM_FULL = ROWS_EMPTY + S::ROWS;
+    constexpr int SUM_EMPTY = SUM_FULL + S::BUFS, BARS = SUM_EMPTY + S::BUFS;
+    static_assert(BARS * 8 + 4 <= 512, "room for the barriers");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
-    float* scales = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE + 256);     // 8-bit rows: [group][token]
+    float* scales = reinterpret_cast<float*>(smem + S::RINGS + 512);     // 8-bit rows: [group][token]
     __shared__ int abort_flag;
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -102,9 +105,10 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int i = 0; i < S::STAGES; ++i) {
-            mbar_init(smem_u32(&bars[FULL + i]), 9);     // eight widening warps and the producer
+            mbar_init(smem_u32(&bars[FULL + i]), 8);     // eight widening warps
             mbar_init(smem_u32(&bars[EMPTY + i]), 1);
         }
+        for (int i = 0; i < 2 * S::ROWS; ++i) mbar_init(smem_u32(&bars[ROWS_FULL + i]), 1);
         for (int i = 0; i < S::BUFS; ++i) {
             mbar_init(smem_u32(&bars[SUM_FULL + i]), 1);
             mbar_init(smem_u32(&bars[SUM_EMPTY + i]), 8);
@@ -152,46 +156,63 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
         // ---------------- the tokens' numbers
         if (lane == 0) {
             pdl_wait();
-            for (int i = 0; i < n; ++i) {
-                const int s = i % S::STAGES;
-                if (i >= S::STAGES && !wait_for(smem_u32(&bars[EMPTY + s]), ((i / S::STAGES) & 1) ^ 1, &abort_flag)) break;
-                mbar_expect_tx(smem_u32(&bars[FULL + s]), S::B);
-                tma_load_2d(smem_u32(smem) + s * S::STAGE + S::A, &map_x, (from + i) * S::BLOCKS * 64, tok0, smem_u32(&bars[FULL + s]));
+            const uint32_t full = smem_u32(&bars[ROWS_FULL]), empty = smem_u32(&bars[ROWS_EMPTY]), to = smem_u32(smem) + S::STAGES * S::A;
+            for (int i = 0; i < n; i += 8) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    if (i + u >= n || !ok) break;
+                    const int at = u % S::ROWS;
+                    if (i > 0 || u >= S::ROWS) ok = wait_for(empty + 8 * at, (S::ROWS == 8 ? i / 8 & 1 : u / S::ROWS & 1) ^ 1, &abort_flag);
+                    if (!ok) break;
+                    mbar_expect_tx(full + 8 * at, S::B);
+                    tma_load_2d(to + at * S::B, &map_x, (from + i + u) * S::BLOCKS * 64, tok0, full + 8 * at);
+                }
             }
         }
     } else if (warp == 1) {
         // ---------------- the products
+        // Eight stages a turn, after which every ring is back where it was: places, parities and descriptors are constants.  (With remainders and
+        // addresses formed anew this one thread, not the tensor cores, was the limit: 400 cycles a stage, whatever the tile.)
         if (elect_one()) {
-            int sum = 0;
-            for (int i = 0; i < n && ok; ++i) {
-                const int s = i % S::STAGES;
-                ok = wait_for(smem_u32(&bars[FULL + s]), (i / S::STAGES) & 1, &abort_flag);
-                if (!ok) break;
-                tcgen05_fence_after();
-                const uint64_t da = make_smem_desc(smem_u32(smem) + s * S::STAGE), db = make_smem_desc(smem_u32(smem) + s * S::STAGE + S::A);
-                if constexpr (BYTES) {
+            const uint32_t full = smem_u32(&bars[FULL]), empty = smem_u32(&bars[EMPTY]), rows_full = smem_u32(&bars[ROWS_FULL]), rows_empty = smem_u32(&bars[ROWS_EMPTY]);
+            const uint32_t sum_full = smem_u32(&bars[SUM_FULL]), sum_empty = smem_u32(&bars[SUM_EMPTY]);
+            const uint64_t da0 = make_smem_desc(smem_u32(smem)), db0 = make_smem_desc(smem_u32(smem) + S::STAGES * S::A);
+            for (int i = 0; i < n && ok; i += 8) {
+                const uint32_t turn = i / 8 & 1;
 #pragma unroll
-                    for (int p = 0; p < S::PARTS && ok; ++p, ++sum) {
-                        const int buf = sum % S::BUFS;
-                        if (sum >= S::BUFS) {
-                            ok = wait_for(smem_u32(&bars[SUM_EMPTY + buf]), ((sum / S::BUFS) & 1) ^ 1, &abort_flag);
-                            tcgen05_fence_after();
+                for (int u = 0; u < 8; ++u) {
+                    if (i + u >= n) break;
+                    const int a = u % S::STAGES, r = u % S::ROWS;
+                    ok = wait_for(rows_full + 8 * r, S::ROWS == 8 ? turn : u / S::ROWS & 1, &abort_flag) && wait_for(full + 8 * a, u / S::STAGES & 1, &abort_flag);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const uint64_t da = da0 + a * (S::A / 16), db = db0 + r * (S::B / 16);
+                    if constexpr (BYTES) {
+#pragma unroll
+                        for (int p = 0; p < S::PARTS; ++p) {
+                            const int sum = u * S::PARTS + p, buf = sum % S::BUFS;
+                            if (i > 0 || sum >= S::BUFS) {
+                                ok = wait_for(sum_empty + 8 * buf, (sum / S::BUFS & 1) ^ 1, &abort_flag);
+                                if (!ok) break;
+                                tcgen05_fence_after();
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4 / S::PARTS; ++k) {                    // 32 columns an instruction
+                                const int at = 2 * (p * (4 / S::PARTS) + k);
+                                mma_step<BN, BYTES>(tmem + buf * BN, da + at, db + at, k ? 1u : 0u);
+                            }
+                            tcgen05_commit(sum_full + 8 * buf);
                         }
                         if (!ok) break;
+                    } else {
 #pragma unroll
-                        for (int k = 0; k < 4 / S::PARTS; ++k) {                        // 32 columns an instruction
-                            const int at = 2 * (p * (4 / S::PARTS) + k);
-                            mma_step<BN, BYTES>(tmem + buf * BN, da + at, db + at, k ? 1u : 0u);
-                        }
-                        tcgen05_commit(smem_u32(&bars[SUM_FULL + buf]));
+                        for (int k = 0; k < 4; ++k) mma_step<BN, BYTES>(tmem, da + 2 * k, db + 2 * k, (i | u | k) ? 1u : 0u);        // 16 columns
                     }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_step<BN, BYTES>(tmem, da + 2 * k, db + 2 * k, (i | k) ? 1u : 0u);   // 16 columns
+                    tcgen05_commit(empty + 8 * a);
+                    tcgen05_commit(rows_empty + 8 * r);
                 }
-                tcgen05_commit(smem_u32(&bars[EMPTY + s]));
             }
-            if (!BYTES) tcgen05_commit(smem_u32(&bars[SUM_FULL]));
+            if (!BYTES) tcgen05_commit(sum_full);
         }
     } else if (widens) {
         // ---------------- the weights
@@ -213,7 +234,7 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
 #pragma unroll
             for (int u = 0; u < S::AHEAD; ++u, ++done) {
                 if (done >= stages) break;
-                const uint32_t to = phase * S::STAGE + u % S::TURN * S::WIDENS * S::STAGE;
+                const uint32_t to = phase * S::A + u % S::TURN * S::WIDENS * S::A;
                 if (done >= S::TURN) {
                     ok = wait_for(empty + u % S::TURN * S::WIDENS * 8, parity, &abort_flag);
                     if (!ok) break;
@@ -259,35 +280,41 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
             const int r = min(row, 16 * tiles - 1);
             const __nv_bfloat16* ws = reinterpret_cast<const __nv_bfloat16*>(w1) + ((size_t)(r / 16) * all_groups + first) * 16 + 2 * (r % 8) + r % 16 / 8;
             const int last = all_groups - 1 - first;
-            float next = __bfloat162float(ws[0]);
-            const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + cols0;
+            float next[S::BUFS];
+#pragma unroll
+            for (int u = 0; u < S::BUFS; ++u) next[u] = __bfloat162float(ws[(size_t)min(u, last) * 16]);
+            const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + cols0, sum_full = smem_u32(&bars[SUM_FULL]), sum_empty = smem_u32(&bars[SUM_EMPTY]);
             const float* a = scales + cols0;
-            for (int i = 0; i < count && ok; ++i, a += BN) {
-                const int buf = i % S::BUFS;
-                const float f = next * 0.0625f;          // (the products hold 16 q)
-                next = __bfloat162float(ws[(size_t)min(i + 1, last) * 16]);
-                ok = wait_for(smem_u32(&bars[SUM_FULL + buf]), (i / S::BUFS) & 1, &abort_flag);
-                if (!ok) break;
-                tcgen05_fence_after();
-                constexpr int CH = BN == 64 ? 32 : 16;   // (32 numbers beside 64 sums would not fit the registers)
-                const Two ff = two(f, f);
+            uint32_t parity = 0;
+            for (int i = 0; i < count && ok; i += S::BUFS, parity ^= 1) {
 #pragma unroll
-                for (int c = 0; c < BN / 2; c += CH) {
-                    uint32_t r[CH];
-                    if constexpr (CH == 32) tcgen05_ld32(lanes + buf * BN + c, r);
-                    else tcgen05_ld16(lanes + buf * BN + c, r);
-                    tcgen05_wait_ld();
-                    if (c + CH == BN / 2) {
-                        tcgen05_fence_before();
-                        __syncwarp();
-                        if (lane == 0) at_arrive(smem_u32(&bars[SUM_EMPTY + buf]));
-                    }
+                for (int u = 0; u < S::BUFS; ++u, a += BN) {
+                    if (i + u >= count) break;
+                    const float f = next[u] * 0.0625f;   // (the products hold 16 q)
+                    const Two ff = two(f, f);
+                    next[u] = __bfloat162float(ws[(size_t)min(i + u + S::BUFS, last) * 16]);
+                    ok = wait_for(sum_full + 8 * u, parity, &abort_flag);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    constexpr int CH = BN == 64 ? 32 : 16;              // (32 numbers beside 64 sums would not fit the registers)
 #pragma unroll
-                    for (int j = 0; j < CH; j += 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(a + c + j);
-                        const Two v0 = two((float)(int)r[j], (float)(int)r[j + 1]), v1 = two((float)(int)r[j + 2], (float)(int)r[j + 3]);     // (exact)
-                        acc[(c + j) / 2] = fma2(v0, mul2(two(x.x, x.y), ff), acc[(c + j) / 2]);
-                        acc[(c + j) / 2 + 1] = fma2(v1, mul2(two(x.z, x.w), ff), acc[(c + j) / 2 + 1]);
+                    for (int c = 0; c < BN / 2; c += CH) {
+                        uint32_t r[CH];
+                        if constexpr (CH == 32) tcgen05_ld32(lanes + u * BN + c, r);
+                        else tcgen05_ld16(lanes + u * BN + c, r);
+                        tcgen05_wait_ld();
+                        if (c + CH == BN / 2) {
+                            tcgen05_fence_before();
+                            __syncwarp();
+                            if (lane == 0) at_arrive(sum_empty + 8 * u);
+                        }
+#pragma unroll
+                        for (int j = 0; j < CH; j += 4) {
+                            const float4 x = *reinterpret_cast<const float4*>(a + c + j);
+                            const Two v0 = two((float)(int)r[j], (float)(int)r[j + 1]), v1 = two((float)(int)r[j + 2], (float)(int)r[j + 3]);        // (exact)
+                            acc[(c + j) / 2] = fma2(v0, mul2(two(x.x, x.y), ff), acc[(c + j) / 2]);
+                            acc[(c + j) / 2 + 1] = fma2(v1, mul2(two(x.z, x.w), ff), acc[(c + j) / 2 + 1]);
+                        }
                     }
                 }
             }
