@@ -288,19 +288,21 @@ __global__ void __launch_bounds__(256) dequantize_w4_kernel(const uint4* packed,
 __global__ void weights_made_kernel() {}
 
 // ---------------------------------------------------------------- products of few tokens
-// c += A B, A 16 rows by 32 (16) columns of weights, B as many columns by eight tokens.
-__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// d = A B + c, A 16 rows by 32 (16) columns of weights, B as many columns by eight tokens.
+__device__ __forceinline__ void mma_s8(int (&d)[4], const int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-// c += (rows g, g + 8; 32 columns) times the token's numbers: a word of four bytes a row, eight numbers.
-__device__ __forceinline__ void quarter(int (&c)[4], uint32_t lo_row, uint32_t hi_row, const uint2& x) {
+// d = (rows g, g + 8; 32 columns) times the token's numbers + c: a word of four bytes a row, eight numbers.
+__device__ __forceinline__ void quarter(int (&d)[4], const int* c, uint32_t lo_row, uint32_t hi_row, const uint2& x) {
     const uint32_t m = 0xf0f0f0f0u;                      // a half of a byte at its upper end is 16 q as a signed byte
-    mma_s8(c, lo_row << 4 & m, hi_row << 4 & m, lo_row & m, hi_row & m, x.x, x.y);
+    mma_s8(d, c, lo_row << 4 & m, hi_row << 4 & m, lo_row & m, hi_row & m, x.x, x.y);
 }
 // Two halves of bytes, 16 bits apart, as bfloat16 numbers: 128 + (q + 8) in the bits of 128, less 136; both steps are exact.
 __device__ __forceinline__ uint32_t two_weights(uint32_t w) {
@@ -309,12 +311,10 @@ __device__ __forceinline__ uint32_t two_weights(uint32_t w) {
     __nv_bfloat162 r = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&v), less);
     return *reinterpret_cast<uint32_t*>(&r);
 }
-__device__ __forceinline__ void quarter(float (&c)[4], uint32_t lo_row, uint32_t hi_row, const uint4& x) {
-    // columns (0, 2), (1, 3) and (4, 6), (5, 7) of the eight are 16 bits apart in the word; the row's pairs are put together alike
-    mma_bf16(c, two_weights(lo_row), two_weights(hi_row), two_weights(lo_row >> 8), two_weights(hi_row >> 8),
-             __byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));
-    mma_bf16(c, two_weights(lo_row >> 4), two_weights(hi_row >> 4), two_weights(lo_row >> 12), two_weights(hi_row >> 12),
-             __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
+__device__ __forceinline__ void quarter(float (&d)[4], const float* c, uint32_t lo_row, uint32_t hi_row, const uint4& x) {
+    const uint32_t lo = __byte_perm(lo_row, 0, 0x3120), hi = __byte_perm(hi_row, 0, 0x3120);       // neighbouring columns 16 bits apart
+    mma_bf16(d, c, two_weights(lo), two_weights(hi), two_weights(lo >> 8), two_weights(hi >> 8), x.x, x.y);
+    mma_bf16(d, d, two_weights(lo >> 4), two_weights(hi >> 4), two_weights(lo >> 12), two_weights(hi >> 12), x.z, x.w);
 }
 __device__ __forceinline__ unsigned long long two(float a, float b) {
     unsigned long long r;
@@ -337,10 +337,11 @@ __device__ __forceinline__ unsigned long long fma_two(unsigned long long a, unsi
     return r;
 }
 
-// 8 NB tokens (blockIdx.y) by tiles of 16 rows, one block of 16 warps an SM for as long as there are tiles.  The numbers of the block's
+// 8 NB tokens (blockIdx.y) by tiles of 16 RT rows, one block of 16 warps an SM for as long as there are tiles.  With RT = 2 a token's numbers,
+// once in registers, meet 32 rows: from two eights of tokens on the reads of shared memory would otherwise take longer than the products.  The numbers of the block's
 // tokens lie in shared memory from the start (a cluster's CTAs have a share of the columns each, so that they fit), and their scales.  A
 // warp goes through its tiles in units of 128 columns (1 KB of weights), which asynchronous copies bring into a ring of its own, DEPTH
-// units ahead and without regard to where a row of tiles ends; a lane reads back what it has copied itself (but for the scales).  No
+// units ahead and without regard to where a tile ends; a lane reads back what it has copied itself (but for the scales).  No
 // warp waits for another but once a round, when `ways` warps (and the cluster's CTAs) add up what they have of a tile, and not even then
 // where a tile is one warp's.
 // A group's (at most 128 columns') exact sum is formed by the tensor cores in whole numbers and added up in 32 bits; the whole number starts
@@ -348,66 +349,82 @@ __device__ __forceinline__ unsigned long long fma_two(unsigned long long a, unsi
 // needed.
 #define W4_WARPS 16
 #define W4_SLOT (1024 + 128)                             // a unit's weights, and its scales [group][16 rows]
-#define W4_SUMS (16 * W4_WARPS + 4)                      // pitch of the warps' sums [token][16 rows a warp]
+#define W4_SUMS(rt) (16 * (rt) * W4_WARPS + 4)           // pitch of the warps' sums [token][16 rt rows a warp]
 // Shared memory of a block: tokens' numbers (rows a pitch apart by which eight tokens' reads meet every bank once), their scales
-// [group][token], the warps' sums (two sets for a cluster), the rings.
+// [group][token], the warps' sums (two sets for a cluster, none where a tile is one warp's), the rings.
 struct W4Shared {
     int columns, pitch, scales, sums, ring, bytes;
 };
-__host__ __device__ constexpr int w4_depth(int nb) { return nb == 1 ? 6 : nb == 2 ? 4 : 3; }
-__host__ __device__ inline W4Shared w4_shared(int units, int splits, int G, int size, int M, int nb) {
+__host__ __device__ constexpr int w4_depth(int nb, int rt) { return nb == 1 ? 6 : nb == 2 ? 4 / rt + (rt - 1) : 3 - (rt - 1); }
+__host__ __device__ inline W4Shared w4_shared(int units, int ways, int splits, int G, int size, int M, int nb, int rt) {
     W4Shared s;
     s.columns = (units + splits - 1) / splits * 128;
     s.pitch = s.columns * size + (size == 1 ? 32 : 64);
     s.scales = (M < 8 * nb ? M : 8 * nb) * s.pitch;
     s.sums = s.scales + (size == 1 ? s.columns / G * 8 * nb * 4 : 0);
-    s.ring = s.sums + (splits > 1 ? 2 : 1) * 8 * nb * W4_SUMS * 4;
-    s.bytes = s.ring + W4_WARPS * w4_depth(nb) * W4_SLOT;
+    s.ring = s.sums + (splits > 1 ? 2 : ways > 1 ? 1 : 0) * 8 * nb * W4_SUMS(rt) * 4;
+    s.bytes = s.ring + W4_WARPS * w4_depth(nb, rt) * rt * W4_SLOT;
     return s;
 }
 
-template <int G, typename X, int NB>
+template <int G, typename X, int NB, int RT>
 __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint4* __restrict__ w0, const uint32_t* __restrict__ w1, const X* x,
                                                                       const float* xs, long long ldx, int whole, int K, int blocks, int ways, int splits, W4Out o) {
     constexpr bool BYTES = std::is_same<X, int8_t>::value;
-    constexpr int DEPTH = w4_depth(NB), GROUPS = 128 / G, QUARTERS = G / 32, THREADS = 32 * W4_WARPS;
+    constexpr int DEPTH = w4_depth(NB, RT), GROUPS = 128 / G, QUARTERS = G / 32, THREADS = 32 * W4_WARPS, SLOT = RT * W4_SLOT, SUMS = W4_SUMS(RT);
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_trigger();
     const int units = (blocks + 1) / 2, all_groups = blocks * 64 / G;
-    const W4Shared sh = w4_shared(units, splits, G, (int)sizeof(X), o.M, NB);
+    const W4Shared sh = w4_shared(units, ways, splits, G, (int)sizeof(X), o.M, NB, RT);
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % splits, cluster = blockIdx.x / splits, clusters = gridDim.x / splits;
-    const int tiles = (o.N + 15) / 16, at_once = W4_WARPS / ways, rounds = (tiles + clusters * at_once - 1) / (clusters * at_once);
+    const int tiles16 = (o.N + 15) / 16, tiles = (tiles16 + RT - 1) / RT, at_once = W4_WARPS / ways, rounds = (tiles + clusters * at_once - 1) / (clusters * at_once);
     const int tok0 = blockIdx.y * 8 * NB, live = min(8 * NB, o.M - tok0);
     const int first = (int)((long long)units * rank / splits), count = (int)((long long)units * (rank + 1) / splits) - first;
     const int from = first + count * (warp % ways) / ways, to = first + count * (warp % ways + 1) / ways;
     auto tile_of = [&](int round) { return (round * clusters + cluster) * at_once + warp / ways; };
     // the unit that is asked for next, and the ring
-    int ask_round = from < to && tile_of(0) < tiles ? 0 : rounds, ask_unit = from;
-    const uint32_t ring = base + sh.ring + warp * DEPTH * W4_SLOT;
-    int slot = 0;
-    auto ask = [&](int into) {
+    int ask_round = from < to && tile_of(0) < tiles ? 0 : rounds, ask_left = to - from;
+    const uint32_t ring = base + sh.ring + warp * DEPTH * SLOT;
+    uint32_t ask_to = ring + 16 * lane;
+    const uint4* pw[RT];
+    const uint32_t* ps[RT];
+    auto start_tile = [&]() {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int tile = min(RT * tile_of(ask_round) + r, tiles16 - 1);             // (rows that are not there: some others)
+            pw[r] = w0 + ((size_t)tile * blocks + 2 * from) * 32 + lane;
+            ps[r] = w1 + ((size_t)tile * all_groups + from * GROUPS + t) * 8 + g;
+        }
+    };
+    start_tile();
+    const bool half_last = (blocks & 1) && to == units;  // a row's last unit is its first half only: zeros, scales too, for the other
+    const uint32_t scale_at = 1024 + 4 * (8 * t + g) - 16 * lane;
+    auto ask = [&]() {
         if (ask_round < rounds) {
-            const int tile = tile_of(ask_round);
-            const uint32_t to_here = ring + into * W4_SLOT;
-            const uint4* p = w0 + ((size_t)tile * blocks + 2 * ask_unit) * 32 + lane;
-            copy16(to_here + 16 * lane, p, true);
-            const bool second = 2 * ask_unit + 1 < blocks;
-            copy16(to_here + 512 + 16 * lane, second ? p + 32 : p, second);
-            if (t < GROUPS) {
-                const int group = ask_unit * GROUPS + t;
-                const uint32_t* s = w1 + (size_t)tile * all_groups * 8 + g;
-                copy4(to_here + 1024 + (8 * t + g) * 4, group < all_groups ? s + (size_t)group * 8 : s, group < all_groups);
+            const bool second = !(half_last && ask_left == 1);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                copy16(ask_to + r * W4_SLOT, pw[r], true);
+                copy16(ask_to + r * W4_SLOT + 512, second ? pw[r] + 32 : pw[r], second);
+                if (t < GROUPS) {
+                    const bool there = second || 2 * t < GROUPS;
+                    copy4(ask_to + r * W4_SLOT + scale_at, there ? ps[r] : w1, there);
+                }
+                pw[r] += 64;
+                ps[r] += 8 * GROUPS;
             }
-            if (++ask_unit == to) {
-                ask_unit = from;
+            if (--ask_left == 0) {
+                ask_left = to - from;
                 if (tile_of(++ask_round) >= tiles) ask_round = rounds;
+                else start_tile();
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
+        ask_to = ask_to == ring + 16 * lane + (DEPTH - 1) * SLOT ? ring + 16 * lane : ask_to + SLOT;
     };
-    for (int i = 0; i < DEPTH; ++i) ask(i);
+    for (int i = 0; i < DEPTH; ++i) ask();
     pdl_wait(x, xs);
     if (whole) {
         constexpr int EACH = 16 / (int)sizeof(X);
@@ -437,22 +454,23 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint
     asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     float* sums = reinterpret_cast<float*>(smem + sh.sums);
-    const uint8_t* rows[NB];                             // (a token that is not there reads another's numbers: its sums are not written)
+    int rows[NB];                                        // (a token that is not there reads another's numbers: its sums are not written)
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) rows[nb] = smem + min(8 * nb + g, live - 1) * sh.pitch + 8 * t * (int)sizeof(X);
-    const float* scales = reinterpret_cast<const float*>(smem + sh.scales) + 2 * t;
-    unsigned long long acc[NB][2] = {};                  // [eight tokens][row g, g + 8] of two tokens
+    for (int nb = 0; nb < NB; ++nb) rows[nb] = min(8 * nb + g, live - 1) * sh.pitch + (128 * (from - first) + 8 * t) * (int)sizeof(X);
+    const int scales0 = sh.scales + ((from - first) * GROUPS * 8 * NB + 2 * t) * 4, slots0 = sh.ring + warp * DEPTH * SLOT;
+    int slot = slots0;
+    unsigned long long acc[RT][NB][2] = {};              // [tile][eight tokens][row g, g + 8] of two tokens
 
     // a round's sums, over the warps of a tile and the CTAs of the cluster in order; every CTA writes a share
     auto write_round = [&](int round) {
-        const float* at = sums + (splits > 1 ? round & 1 : 0) * 8 * NB * W4_SUMS;
-        const int rows_here = 16 * at_once, n0 = (round * clusters + cluster) * rows_here;
+        const float* at = sums + (splits > 1 ? round & 1 : 0) * 8 * NB * SUMS;
+        const int rows_here = 16 * RT * at_once, n0 = (round * clusters + cluster) * rows_here;
         for (int i = rank * THREADS + threadIdx.x; i < live * rows_here; i += splits * THREADS) {
             const int tok = i / rows_here, r = i - tok * rows_here;
-            const float* p = at + tok * W4_SUMS + r / 16 * ways * 16 + r % 16;
+            const float* p = at + tok * SUMS + r / (16 * RT) * ways * 16 * RT + r % (16 * RT);
             float v = 0.f;
             if (splits == 1) {
-                for (int k = 0; k < ways; ++k) v += p[16 * k];
+                for (int k = 0; k < ways; ++k) v += p[16 * RT * k];
             } else {
                 const uint32_t here = (uint32_t)__cvta_generic_to_shared(p);
                 for (int c = 0; c < splits; ++c) {
@@ -460,7 +478,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(c));
                     for (int k = 0; k < ways; ++k) {
                         float f;
-                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there + 64 * k) : "memory");
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there + 64 * RT * k) : "memory");
                         v += f;
                     }
                 }
@@ -471,85 +489,116 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint
 
     for (int round = 0; round < rounds; ++round) {
         if (tile_of(round) < tiles)
-            for (int u = from; u < to; ++u) {
+            for (int u = 0; u < to - from; ++u) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
                 __syncwarp();
-                const uint8_t* here = smem + sh.ring + (warp * DEPTH + slot) * W4_SLOT;
-                const uint4 wa = *reinterpret_cast<const uint4*>(here + 16 * lane), wb = *reinterpret_cast<const uint4*>(here + 512 + 16 * lane);
-                float sw[GROUPS][2];
+                const uint8_t* here = smem + slot;
+                uint32_t lo[RT][4], hi[RT][4];
+                float sw[RT][GROUPS][2];
 #pragma unroll
-                for (int p = 0; p < GROUPS; ++p) {
-                    const uint32_t s2 = *reinterpret_cast<const uint32_t*>(here + 1024 + (8 * p + g) * 4);
-                    sw[p][0] = __uint_as_float(s2 << 16); sw[p][1] = __uint_as_float(s2 & 0xffff0000u);
-                    if (BYTES) { sw[p][0] *= 0.0625f; sw[p][1] *= 0.0625f; }              // the products hold 16 q
+                for (int r = 0; r < RT; ++r) {
+                    const uint4 wa = *reinterpret_cast<const uint4*>(here + r * W4_SLOT + 16 * lane), wb = *reinterpret_cast<const uint4*>(here + r * W4_SLOT + 512 + 16 * lane);
+                    lo[r][0] = wa.x; lo[r][1] = wa.y; lo[r][2] = wb.x; lo[r][3] = wb.y;
+                    hi[r][0] = wa.z; hi[r][1] = wa.w; hi[r][2] = wb.z; hi[r][3] = wb.w;
+#pragma unroll
+                    for (int p = 0; p < GROUPS; ++p) {
+                        const uint32_t s2 = *reinterpret_cast<const uint32_t*>(here + r * W4_SLOT + 1024 + (8 * p + g) * 4);
+                        sw[r][p][0] = __uint_as_float(s2 << 16); sw[r][p][1] = __uint_as_float(s2 & 0xffff0000u);
+                        if (BYTES) { sw[r][p][0] *= 0.0625f; sw[r][p][1] *= 0.0625f; }    // the products hold 16 q
+                    }
                 }
                 __syncwarp();                            // all have read the slot
-                ask(slot);
-                slot = slot + 1 == DEPTH ? 0 : slot + 1;
-                const uint32_t lo[4] = {wa.x, wa.y, wb.x, wb.y}, hi[4] = {wa.z, wa.w, wb.z, wb.w};
+                ask();
+                slot = slot == slots0 + (DEPTH - 1) * SLOT ? slots0 : slot + SLOT;
+                const uint8_t* numbers = smem + 128 * (int)sizeof(X) * u;
+                const uint8_t* scales = smem + scales0 + GROUPS * 8 * NB * 4 * u;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    const uint8_t* row = rows[nb] + 128 * (u - first) * (int)sizeof(X);
+                    const uint8_t* row = numbers + rows[nb];
                     if constexpr (BYTES) {
-                        int c[GROUPS][4];
+                        const int start[4] = {0x4b400000, 0x4b400000, 0x4b400000, 0x4b400000};
+                        int c[RT][GROUPS][4];
 #pragma unroll
                         for (int h = 0; h < 4; ++h) {
-                            int (&part)[4] = c[h / QUARTERS];
-                            if (h % QUARTERS == 0) part[0] = part[1] = part[2] = part[3] = 0x4b400000;
-                            quarter(part, lo[h], hi[h], *reinterpret_cast<const uint2*>(row + 32 * h));
+                            const uint2 x8 = *reinterpret_cast<const uint2*>(row + 32 * h);
+#pragma unroll
+                            for (int r = 0; r < RT; ++r) {
+                                int (&part)[4] = c[r][h / QUARTERS];
+                                quarter(part, h % QUARTERS ? part : start, lo[r][h], hi[r][h], x8);
+                            }
                         }
 #pragma unroll
                         for (int p = 0; p < GROUPS; ++p) {
-                            const float2 a = *reinterpret_cast<const float2*>(scales + ((u - first) * GROUPS + p) * 8 * NB + 8 * nb);
-                            const unsigned long long xa = two(a.x, a.y), less = two(-12582912.f, -12582912.f);
+                            const unsigned long long xa = *reinterpret_cast<const unsigned long long*>(scales + (p * 8 * NB + 8 * nb) * 4), less = two(-12582912.f, -12582912.f);
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                acc[nb][e] = fma_two(add_two(two(__int_as_float(c[p][2 * e]), __int_as_float(c[p][2 * e + 1])), less),
-                                                     mul_two(xa, two(sw[p][e], sw[p][e])), acc[nb][e]);
+                            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                    acc[r][nb][e] = fma_two(add_two(two(__int_as_float(c[r][p][2 * e]), __int_as_float(c[r][p][2 * e + 1])), less),
+                                                            mul_two(xa, two(sw[r][p][e], sw[r][p][e])), acc[r][nb][e]);
                         }
                     } else {
-                        float c[GROUPS][4];
+                        const float start[4] = {};
+                        float c[RT][GROUPS][4];
 #pragma unroll
                         for (int h = 0; h < 4; ++h) {
-                            float (&part)[4] = c[h / QUARTERS];
-                            if (h % QUARTERS == 0) part[0] = part[1] = part[2] = part[3] = 0.f;
-                            quarter(part, lo[h], hi[h], *reinterpret_cast<const uint4*>(row + 64 * h));
+                            const uint4 x8 = *reinterpret_cast<const uint4*>(row + 64 * h);
+#pragma unroll
+                            for (int r = 0; r < RT; ++r) {
+                                float (&part)[4] = c[r][h / QUARTERS];
+                                quarter(part, h % QUARTERS ? part : start, lo[r][h], hi[r][h], x8);
+                            }
                         }
 #pragma unroll
-                        for (int p = 0; p < GROUPS; ++p)
+                        for (int r = 0; r < RT; ++r)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                acc[nb][e] = fma_two(two(c[p][2 * e], c[p][2 * e + 1]), two(sw[p][e], sw[p][e]), acc[nb][e]);
+                            for (int p = 0; p < GROUPS; ++p)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                    acc[r][nb][e] = fma_two(two(c[r][p][2 * e], c[r][p][2 * e + 1]), two(sw[r][p][e], sw[r][p][e]), acc[r][nb][e]);
                     }
                 }
             }
+        if (splits == 1 && ways == 1) {                  // the warp's own tile: straight out, eight rows of a token at a time
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float a, c;
+                        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(c) : "l"(acc[r][nb][e]));
+                        const int n = (tile_of(round) * RT + r) * 16 + g + 8 * e, tok = 8 * nb + 2 * t;
+                        if (tok < live) w4_write(o, tok0 + tok, n, a);
+                        if (tok + 1 < live) w4_write(o, tok0 + tok + 1, n, c);
+                        acc[r][nb][e] = 0ull;
+                    }
+            continue;
+        }
         if (splits > 1 && round > 0) {
             asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
             write_round(round - 1);
         }
         if (splits == 1 && ways > 1 && round > 0) __syncthreads();              // the sums of the round before are read
-        float* to_a = sums + ((splits > 1 ? round & 1 : 0) * 8 * NB + 2 * t) * W4_SUMS + 16 * warp + g;
+        float* to_a = sums + ((splits > 1 ? round & 1 : 0) * 8 * NB + 2 * t) * SUMS + 16 * RT * warp + g;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float a, c;
-                asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(c) : "l"(acc[nb][e]));
-                to_a[8 * nb * W4_SUMS + 8 * e] = a;
-                to_a[(8 * nb + 1) * W4_SUMS + 8 * e] = c;
-                acc[nb][e] = 0ull;
-            }
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float a, c;
+                    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(c) : "l"(acc[r][nb][e]));
+                    to_a[8 * nb * SUMS + 16 * r + 8 * e] = a;
+                    to_a[(8 * nb + 1) * SUMS + 16 * r + 8 * e] = c;
+                    acc[r][nb][e] = 0ull;
+                }
         if (splits > 1) {
             // two sets of sums in turn: who writes a set for the second time knows, by the barrier between, that all have read the first
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        } else if (ways > 1) {
+        } else {
             __syncthreads();
             write_round(round);
-        } else {                                         // the warp's own tile: half the warp has a token's 16 rows
-            __syncwarp();
-            const int n = tile_of(round) * 16 + lane % 16;
-            for (int tok = lane / 16; tok < live; tok += 2) w4_write(o, tok0 + tok, n, sums[tok * W4_SUMS + 16 * warp + lane % 16]);
-            __syncwarp();
         }
     }
     if (splits > 1) {
@@ -622,25 +671,32 @@ static int launch_add_rmsnorm_q8(float* h, const void* pending, int kind, int n_
     return 0;
 }
 
-// f(group, rows, eights) with the constants and types of a product's kernel
+// f(group, rows, eights, tiles a warp) with the constants and types of a product's kernel; false: there is none
 template <typename F>
-static void with_product(int x_kind, int G, int eights, F f) {
+static bool with_product(int x_kind, int G, int eights, int pair, F f) {
+    if (!(eights == 1 && pair == 1) && !((eights == 2 || eights == 4) && (pair == 1 || pair == 2))) return false;
     with_group(G, [&](auto gc) {
+        using One = std::integral_constant<int, 1>;
+        using Two = std::integral_constant<int, 2>;
+        using Four = std::integral_constant<int, 4>;
         auto with_rows = [&](auto rows) {
-            if (eights == 1) f(gc, rows, std::integral_constant<int, 1>());
-            else if (eights == 2) f(gc, rows, std::integral_constant<int, 2>());
-            else f(gc, rows, std::integral_constant<int, 4>());
+            if (eights == 1) f(gc, rows, One(), One());
+            else if (eights == 2 && pair == 1) f(gc, rows, Two(), One());
+            else if (eights == 2) f(gc, rows, Two(), Two());
+            else if (pair == 1) f(gc, rows, Four(), One());
+            else f(gc, rows, Four(), Two());
         };
         if (x_kind == 0) with_rows(static_cast<const int8_t*>(nullptr));
         else with_rows(static_cast<const __nv_bfloat16*>(nullptr));
     });
+    return true;
 }
-template <int G, typename X, int NB>
+template <int G, typename X, int NB, int RT>
 static int set_shared() {                                // the kernel's limit of shared memory, once a device
     static PerDevice<bool> set;
     bool& done = set.here();
     if (done) return 0;
-    const cudaError_t e = cudaFuncSetAttribute(w4_product_kernel<G, X, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    const cudaError_t e = cudaFuncSetAttribute(w4_product_kernel<G, X, NB, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     done = e == cudaSuccess;
     return (int)e;
 }
@@ -729,15 +785,16 @@ int rf_weights_made(cudaStream_t st) {
     return 0;
 }
 
-// Bytes of shared memory that a product's block takes with `eights` eights of tokens and a share of the columns in `splits`.
-int rf_gemm_w4_shared(int x_kind, int M, int K, int G, int eights, int splits) {
-    return w4_shared((padded(K, G) / 64 + 1) / 2, splits, G, x_kind == 0 ? 1 : 2, M, eights).bytes;
+// Bytes of shared memory that a product's block takes with `eights` eights of tokens, `pair` tiles of 16 rows a warp, `ways` warps a tile and a
+// share of the columns in `splits`.
+int rf_gemm_w4_shared(int x_kind, int M, int K, int G, int eights, int pair, int ways, int splits) {
+    return w4_shared((padded(K, G) / 64 + 1) / 2, ways, splits, G, x_kind == 0 ? 1 : 2, M, eights, pair).bytes;
 }
 
 // Clusters of `splits` blocks, each with an SM of its own, that run at once on the current device (< 0: an error).
 int rf_gemm_w4_clusters(int splits) {
     if (splits < 1 || splits > 8) return RF_ERR_BAD_ARG;
-    if (const int e = set_shared<128, int8_t, 1>()) return -e;
+    if (const int e = set_shared<128, int8_t, 1, 1>()) return -e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits);
     cfg.blockDim = dim3(32 * W4_WARPS);
@@ -748,36 +805,37 @@ int rf_gemm_w4_clusters(int splits) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, w4_product_kernel<128, int8_t, 1>, &cfg);
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, w4_product_kernel<128, int8_t, 1, 1>, &cfg);
     return e == cudaSuccess ? n : -(int)e;
 }
 
 // out = x w^T (+ bias): x_kind 0: 8-bit rows (x int8 [M, Kp], xs float32 [M, Kp / G]), 1: bfloat16 rows [M, K], ldx apart; out as W4Out
-// has it.  eights: eights of tokens a block (1, 2, 4); ways: warps a tile (a power of two up to 16); splits: CTAs of a cluster that share
+// has it.  eights: eights of tokens a block (1, 2, 4); pair: tiles of 16 rows a warp (1; 2 from two eights on); ways: warps a tile (a power of two up to 16); splits: CTAs of a cluster that share
 // out the columns (1 .. 8); clusters: of each share of tokens.
 int rf_gemm_w4(int x_kind, const void* x, const void* xs, long long ldx, const void* packed, const void* scales, const void* bias, int bias_is_f32,
-               void* out, int out_is_f32, int add, int eights, int ways, int splits, int clusters, int M, int N, int K, int G, cudaStream_t st) {
+               void* out, int out_is_f32, int add, int eights, int pair, int ways, int splits, int clusters, int M, int N, int K, int G, cudaStream_t st) {
     if (M <= 0 || N <= 0 || K <= 0 || bad_group(G) || (add && !out_is_f32)) return RF_ERR_BAD_ARG;
     if ((x_kind == 0 && (!aligned(x, 16) || ldx % 16)) || !aligned(packed, 16) || !aligned(scales, 16)) return RF_ERR_BAD_ARG;
-    if (splits < 1 || splits > 8 || clusters < 1 || ways < 1 || ways > W4_WARPS || (ways & (ways - 1)) || (eights != 1 && eights != 2 && eights != 4)) return RF_ERR_BAD_ARG;
+    if (splits < 1 || splits > 8 || clusters < 1 || ways < 1 || ways > W4_WARPS || (ways & (ways - 1)) || eights < 1) return RF_ERR_BAD_ARG;
     const int whole = x_kind == 0 || (K % 8 == 0 && ldx % 8 == 0 && aligned(x, 16));
-    const int blocks = padded(K, G) / 64, smem = rf_gemm_w4_shared(x_kind, M, K, G, eights, splits);
+    const int blocks = padded(K, G) / 64, smem = rf_gemm_w4_shared(x_kind, M, K, G, eights, pair, ways, splits);
     const long long y = (M + 8ll * eights - 1) / (8 * eights);
     if (smem > W4_MOST_SHARED || y > 65535 || (long long)clusters * splits > 0x7fffffffll) return RF_ERR_UNSUPPORTED;
     const W4Out o{out, bias, bias_is_f32, out_is_f32, add, M, N};
     int bad = 0;
-    with_product(x_kind, G, eights, [&](auto gc, auto rows, auto nb) {
+    const bool known = with_product(x_kind, G, eights, pair, [&](auto gc, auto rows, auto nb, auto rt) {
         using X = std::remove_cv_t<std::remove_pointer_t<decltype(rows)>>;
-        constexpr int GC = decltype(gc)::value, NB = decltype(nb)::value;
-        bad = set_shared<GC, X, NB>();
+        constexpr int GC = decltype(gc)::value, NB = decltype(nb)::value, RT = decltype(rt)::value;
+        bad = set_shared<GC, X, NB, RT>();
         if (bad) return;
         const dim3 grid(clusters * splits, (unsigned)y), block(32 * W4_WARPS);
         auto go = [&](auto... args) {
-            if (splits > 1) rf_launch_cluster(w4_product_kernel<GC, X, NB>, grid, block, smem, st, splits, args...);
-            else rf_launch(w4_product_kernel<GC, X, NB>, grid, block, smem, st, args...);
+            if (splits > 1) rf_launch_cluster(w4_product_kernel<GC, X, NB, RT>, grid, block, smem, st, splits, args...);
+            else rf_launch(w4_product_kernel<GC, X, NB, RT>, grid, block, smem, st, args...);
         };
         go((const uint4*)packed, (const uint32_t*)scales, (const X*)x, (const float*)xs, ldx, whole, K, blocks, ways, splits, o);
     });
+    if (!known) return RF_ERR_BAD_ARG;
     if (bad) return bad;
     RF_LAUNCH_CHECK();
     return 0;

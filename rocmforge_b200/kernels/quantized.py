@@ -25,9 +25,9 @@ _LAUNCHERS = {
     "rf_quantize_w4": [_i, _p, _n, _p, _p, _i, _i, _i, _p],
     "rf_dequantize_w4": [_i, _p, _p, _p, _i, _i, _i, _i, _i, _p],
     "rf_weights_made": [_p],
-    "rf_gemm_w4_shared": [_i, _i, _i, _i, _i, _i],
+    "rf_gemm_w4_shared": [_i, _i, _i, _i, _i, _i, _i, _i],
     "rf_gemm_w4_clusters": [_i],
-    "rf_gemm_w4": [_i, _p, _p, _n, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p],
+    "rf_gemm_w4": [_i, _p, _p, _n, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p],
 }
 
 
@@ -292,20 +292,22 @@ def w4_clusters(splits: int, device: int) -> int:
 
 @functools.lru_cache(4096)
 def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
-    """(eights, ways, splits, clusters): how ``rf_gemm_w4`` shares out a product.  Chosen from sizes alone."""
-    units, tiles = (padded_columns(K, group) // 64 + 1) // 2, (N + 15) // 16
+    """(eights of tokens, tiles a warp, warps a tile, splits, clusters): how ``rf_gemm_w4`` shares out a product.  Chosen from sizes alone."""
+    units, rows16 = (padded_columns(K, group) // 64 + 1) // 2, (N + 15) // 16
     eights, best = 1 if M <= 8 else 2 if M <= 16 else 4, None
     while eights and best is None:                       # fewer tokens at once where longer rows leave no room for more
         shares = (M + 8 * eights - 1) // (8 * eights)
-        for splits in range(1, 9):
-            if _f("rf_gemm_w4_shared")(0 if q8 else 1, M, K, group, eights, splits) > W4_MOST_SHARED:
-                continue
-            clusters = max(1, clusters_of(splits) // shares)
-            for ways in (1, 2, 4, 8, 16):
-                rounds = (tiles + clusters * (16 // ways) - 1) // (clusters * (16 // ways))
-                cost = rounds * ((units + splits * ways - 1) // (splits * ways) + 1) + (splits > 1)
-                if best is None or cost < best[0]:
-                    best = cost, eights, ways, splits, min(clusters, (tiles * ways + 15) // 16)
+        for pair in (1, 2) if eights > 1 else (1,):
+            tiles = (rows16 + pair - 1) // pair
+            for splits in range(1, 9):
+                clusters = max(1, clusters_of(splits) // shares)
+                for ways in (1, 2, 4, 8, 16):
+                    if _f("rf_gemm_w4_shared")(0 if q8 else 1, M, K, group, eights, pair, ways, splits) > W4_MOST_SHARED:
+                        continue
+                    rounds = (tiles + clusters * (16 // ways) - 1) // (clusters * (16 // ways))
+                    cost = rounds * ((units + splits * ways - 1) // (splits * ways) * (1.5 if pair == 2 else 1) + 1) + (splits > 1)
+                    if best is None or cost < best[0]:
+                        best = cost, eights, pair, ways, splits, min(clusters, (tiles * ways + 15) // 16)
         eights //= 2
     if best is None:
         raise KernelError(f"gemm_w4: rows of {K} columns are too long")
@@ -377,10 +379,9 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
                                    M, N, K, w.group, tc.status_word(rows.device).data_ptr(), stream())
         check(code, "gemm_w4" if code == 0 else f"gemm_w4 ({M}x{N}x{K}, tiles of {tiled[0]} tokens)")
         return out
-    eights, ways, splits, clusters = w4_launch(q8, M, N, K, w.group, _clusters_on(rows.get_device()))
+    plan = w4_launch(q8, M, N, K, w.group, _clusters_on(rows.get_device()))
     code = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales.data_ptr() if q8 else None, ld, w.packed.data_ptr(), w.scales.data_ptr(), ptr(bias),
-                            bias is not None and bias.dtype == torch.float32, out.data_ptr(), odt == torch.float32, accumulate, eights, ways, splits,
-                            clusters, M, N, K, w.group, stream())
+                            bias is not None and bias.dtype == torch.float32, out.data_ptr(), odt == torch.float32, accumulate, *plan, M, N, K, w.group, stream())
     check(code, "gemm_w4" if code == 0 else f"gemm_w4 ({M}x{N}x{K})")
     return out
 

@@ -179,20 +179,24 @@ def test_products(kind, M, N, K, G):
     close(got, want + (h.double() + b.double()).to(DEV), size + (h.double().abs() + b.double().abs()).to(DEV), terms + 2, F32)
 
 
-@pytest.mark.parametrize("M,eights,ways,clusters", [(5, 1, 1, 2), (8, 1, 2, 1), (16, 1, 2, 3), (3, 1, 16, 1), (8, 1, 8, 20), (15, 2, 4, 2), (16, 2, 1, 1),
-                                                    (64, 4, 8, 5), (70, 4, 2, 1), (1, 4, 1, 1)])
+@pytest.mark.parametrize("M,eights,pair,ways,clusters", [(5, 1, 1, 1, 2), (8, 1, 1, 2, 1), (16, 1, 1, 2, 3), (3, 1, 1, 16, 1), (8, 1, 1, 8, 20), (15, 2, 1, 4, 2),
+                                                         (16, 2, 2, 1, 1), (9, 2, 2, 4, 2), (64, 4, 1, 8, 5), (70, 4, 2, 2, 1), (1, 4, 1, 1, 1), (33, 4, 2, 1, 3), (32, 4, 2, 16, 2)])
 @pytest.mark.parametrize("kind", ["q8", "bf16"])
 @pytest.mark.parametrize("splits", [1, 2, 3, 8])
 @pytest.mark.parametrize("N,K,G", [(300, 1088, 32), (130, 200, 64), (17, 2176, 128), (450, 77, 128)])
-def test_every_way_to_share_out_a_product(monkeypatch, M, eights, ways, clusters, kind, splits, N, K, G):
+def test_every_way_to_share_out_a_product(monkeypatch, M, eights, pair, ways, clusters, kind, splits, N, K, G):
     """Columns over warps and over CTAs of a cluster (some of which get none), tiles over several rounds, tokens over several blocks."""
     from rocmforge_b200 import kernels
     from rocmforge_b200.kernels import quantized
-    monkeypatch.setattr(quantized, "w4_launch", lambda *a: (eights, ways, splits, clusters))
+    monkeypatch.setattr(quantized, "w4_launch", lambda *a: (eights, pair, ways, splits, clusters))
     monkeypatch.setattr(quantized, "w4_tc_launch", lambda *a: None)
     x, x64, w, full = product_case(kind, M, N, K, G)
     x64, full = x64.to(DEV), full.to(DEV)
     h = numbers(M, N, seed=9)
+    if quantized._f("rf_gemm_w4_shared")(0 if kind == "q8" else 1, M, K, G, eights, pair, ways, splits) > quantized.W4_MOST_SHARED:
+        with pytest.raises(kernels.KernelError, match="not supported"):
+            kernels.gemm_w4(x, w, out=h.to(DEV), accumulate=True)
+        return
     got = kernels.gemm_w4(x, w, out=h.to(DEV), accumulate=True)
     close(got, x64 @ full.T + h.double().to(DEV), x64.abs() @ full.abs().T + h.double().abs().to(DEV), terms_of(kind, K) + 1, F32)
 
