@@ -12,7 +12,7 @@ import functools
 import torch
 
 from . import tensor_core as tc
-from ._ffi import KernelError, c_float, c_int, c_ll, c_void_p, check, dtype_code, fn, need, need_cuda, ptr, sm_count, stream
+from ._ffi import KernelError, c_float, c_int, c_ll, c_void_p, check, dtype_code, fn, need, ptr, sm_count, stream
 
 W4_GROUPS = (32, 64, 128)
 W4_MOST_SHARED = 227 * 1024
@@ -56,19 +56,27 @@ def _need_group(group, what: str) -> None:
 _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+def _device_for(index: int) -> int:
+    """The current device (not asked where a tensor lies on the CPU)."""
+    return _device() if index >= 0 else -2
+
+
+def _elsewhere(what: str, index: int) -> None:
+    if index < 0:
+        raise KernelError(f"{what}: rocmforge_b200 kernels run on a CUDA device only; got a tensor on cpu (there is no CPU fallback)")
+    raise KernelError(f"{what}: a tensor on cuda:{index}, the current device is cuda:{_device()}")
+
+
 def _need_here(what: str, *tensors) -> None:
     """Every tensor on the current device, whose stream the launch goes to."""
-    here = -2
+    here = None
     for t in tensors:
-        if t is None:
-            continue
-        at = t.get_device()
-        if at < 0:
-            need_cuda(t)
-        if here == -2:
-            here = _device()
-        if at != here:
-            raise KernelError(f"{what}: a tensor on cuda:{at}, the current device is cuda:{here}")
+        if t is not None:
+            at = t.get_device()
+            if here is None:
+                here = _device_for(at)
+            if at != here:
+                _elsewhere(what, at)
 
 
 class Q8Rows:
@@ -77,45 +85,68 @@ class Q8Rows:
     ``q`` int8 [T, padded_columns(K, group)] with zeros from column K on, ``scales`` float32 [T, padded columns / group]; ``dtype`` is that
     of the rows they stand for, in which ``materialize`` gives them back and a product's result comes."""
 
-    __slots__ = ("q", "scales", "K", "group", "dtype")
+    __slots__ = ("T", "K", "group", "dtype", "index", "at", "scales_at", "_q", "_scales", "_memory")
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, K: int, group: int, dtype: torch.dtype):
         _need_group(group, "Q8Rows")
         Kp = padded_columns(K, group)
-        if not (K > 0 and q.dtype == torch.int8 and q.dim() == 2 and q.shape[1] == Kp and q.is_contiguous() and q.data_ptr() % 16 == 0):
+        at, index = q.data_ptr(), q.get_device()
+        if not (K > 0 and q.dtype == torch.int8 and q.dim() == 2 and q.shape[1] == Kp and q.is_contiguous() and at % 16 == 0):
             raise KernelError(f"Q8Rows: q must be int8 [T, {Kp}], aligned to 16 bytes")
-        if not (scales.dtype == torch.float32 and scales.shape == (q.shape[0], Kp // group) and scales.is_contiguous()):
+        T = q.shape[0]
+        if not (scales.dtype == torch.float32 and scales.shape == (T, Kp // group) and scales.is_contiguous()):
             raise KernelError(f"Q8Rows: scales must be float32 [T, {Kp // group}]")
-        need(q.get_device() == scales.get_device(), "Q8Rows: q and scales must be on one device")
+        if index != scales.get_device():
+            raise KernelError("Q8Rows: q and scales must be on one device")
         dtype_code(dtype)
-        self.q, self.scales, self.K, self.group, self.dtype = q, scales, K, group, dtype
+        self.T, self.K, self.group, self.dtype, self.index = T, K, group, dtype, index
+        self._q, self._scales, self.at, self.scales_at, self._memory = q, scales, at, scales.data_ptr(), None
 
     @classmethod
     def empty(cls, T: int, K: int, group: int, dtype: torch.dtype, device) -> "Q8Rows":
-        """Rows that a kernel is about to fill."""
-        Kp = padded_columns(K, group)
+        """Rows that a kernel is about to fill: numbers and scales in one piece of memory (an allocation is a third of a call's host time)."""
         r = cls.__new__(cls)
-        r.q = torch.empty((T, Kp), dtype=torch.int8, device=device)
-        r.scales = torch.empty((T, Kp // group), dtype=torch.float32, device=device)
-        r.K, r.group, r.dtype = K, group, dtype
+        Kp = padded_columns(K, group)
+        r._memory = memory = torch.empty(T * Kp + 4 * T * (Kp // group), dtype=torch.int8, device=device)
+        r.T, r.K, r.group, r.dtype, r.index = T, K, group, dtype, memory.get_device()
+        r.at = memory.data_ptr()
+        r.scales_at = r.at + T * Kp
+        r._q = r._scales = None
         return r
+
+    def _split(self) -> None:
+        Kp, T = padded_columns(self.K, self.group), self.T
+        self._q = self._memory[:T * Kp].view(T, Kp)
+        self._scales = self._memory[T * Kp:].view(torch.float32).view(T, Kp // self.group)
+
+    @property
+    def q(self) -> torch.Tensor:
+        if self._q is None:
+            self._split()
+        return self._q
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._split()
+        return self._scales
 
     @property
     def shape(self):
-        return torch.Size((self.q.shape[0], self.K))
+        return torch.Size((self.T, self.K))
 
     @property
     def device(self):
-        return self.q.device
+        return (self._memory if self._q is None else self._q).device
 
     def materialize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The rows as an ordinary tensor [T, K]."""
-        q, dtype = self.q, dtype or self.dtype
-        _need_here("Q8Rows.materialize", q)
-        T, K = q.shape[0], self.K
-        out = torch.empty((T, K), dtype=dtype, device=q.device)
-        check(_f("rf_dequantize_q8")(dtype_code(dtype), q.data_ptr(), self.scales.data_ptr(), out.data_ptr(), T, K, self.group, stream()),
-              "Q8Rows.materialize")
+        dtype = dtype or self.dtype
+        code = dtype_code(dtype)
+        if self.index != _device_for(self.index):
+            _elsewhere("Q8Rows.materialize", self.index)
+        out = torch.empty(self.T, self.K, dtype=dtype, device=self.device)
+        check(_f("rf_dequantize_q8")(code, self.at, self.scales_at, out.data_ptr(), self.T, self.K, self.group, stream()), "Q8Rows.materialize")
         return out
 
 
@@ -127,7 +158,7 @@ class W4Weight:
     groups, 16]: entry [2 g + r] is row g + 8 r.  Rows and columns are padded with zeros.  Products read both before they wait for the
     kernel launched before them: whoever writes them with kernels of its own calls ``weights_made`` afterwards."""
 
-    __slots__ = ("packed", "scales", "N", "K", "group")
+    __slots__ = ("packed", "scales", "N", "K", "group", "index", "at", "scales_at")
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, N: int, K: int, group: int):
         _need_group(group, "W4Weight")
@@ -137,9 +168,10 @@ class W4Weight:
             raise KernelError(f"W4Weight: packed must be uint8 [{tiles}, {Kp // 64}, 32, 16]")
         if not (scales.dtype == torch.bfloat16 and scales.shape == (tiles, Kp // group, 16) and scales.is_contiguous()):
             raise KernelError(f"W4Weight: scales must be bfloat16 [{tiles}, {Kp // group}, 16]")
-        need(packed.get_device() == scales.get_device(), "W4Weight: packed and scales must be on one device")
-        need(packed.data_ptr() % 16 == 0 and scales.data_ptr() % 16 == 0, "W4Weight: packed and scales must be aligned to 16 bytes")
-        self.packed, self.scales, self.N, self.K, self.group = packed, scales, N, K, group
+        index, at, scales_at = packed.get_device(), packed.data_ptr(), scales.data_ptr()
+        if index != scales.get_device() or at % 16 or scales_at % 16:
+            raise KernelError("W4Weight: packed and scales must be on one device and aligned to 16 bytes")
+        self.packed, self.scales, self.N, self.K, self.group, self.index, self.at, self.scales_at = packed, scales, N, K, group, index, at, scales_at
 
     @property
     def shape(self):
@@ -219,7 +251,7 @@ def quantize_q8(x: torch.Tensor, group: int = 128) -> Q8Rows:
     T, K = x.shape
     code = dtype_code(x.dtype)
     y = Q8Rows.empty(T, K, group, x.dtype, x.device)
-    check(_f("rf_quantize_q8")(code, x.data_ptr(), x.stride(0), y.q.data_ptr(), y.scales.data_ptr(), T, K, group, stream()), "quantize_q8")
+    check(_f("rf_quantize_q8")(code, x.data_ptr(), x.stride(0), y.at, y.scales_at, T, K, group, stream()), "quantize_q8")
     return y
 
 
@@ -254,8 +286,8 @@ def add_rmsnorm_q8(h: torch.Tensor, weight: torch.Tensor, eps: float, compute_dt
         n_rows = rows.shape[0]
     code = dtype_code(compute_dtype)
     y = Q8Rows.empty(n_rows, H, group, compute_dtype, h.device)
-    check(_f("rf_add_rmsnorm_q8")(code, h.data_ptr(), ptr(pending), kind, n_pending, pstride, weight.data_ptr(), w_is_f32, eps, y.q.data_ptr(),
-                                  y.scales.data_ptr(), ptr(rows), n_rows, T, H, group, stream()), "add_rmsnorm_q8")
+    check(_f("rf_add_rmsnorm_q8")(code, h.data_ptr(), ptr(pending), kind, n_pending, pstride, weight.data_ptr(), w_is_f32, eps, y.at,
+                                  y.scales_at, ptr(rows), n_rows, T, H, group, stream()), "add_rmsnorm_q8")
     return y
 
 
@@ -273,7 +305,7 @@ def swiglu_q8(gu: torch.Tensor, group: int = 128, activation: str = "silu") -> Q
     T, I = gu.shape[0], gu.shape[1] // 2
     code = dtype_code(gu.dtype)
     y = Q8Rows.empty(T, I, group, gu.dtype, gu.device)
-    check(_f("rf_swiglu_q8")(code, gu.data_ptr(), act, y.q.data_ptr(), y.scales.data_ptr(), T, I, group, stream()), "swiglu_q8")
+    check(_f("rf_swiglu_q8")(code, gu.data_ptr(), act, y.at, y.scales_at, T, I, group, stream()), "swiglu_q8")
     return y
 
 
@@ -343,46 +375,51 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
     ``x``: ``Q8Rows`` of the weight's K and group (products inside a group are exact, in whole numbers), or a tensor [M, K] in bfloat16
     or float32.  out_f32: the result is float32 whatever the rows; accumulate: added into ``out`` (float32)."""
     q8 = type(x) is Q8Rows
-    need(q8 or isinstance(x, torch.Tensor), "gemm_w4: x must be Q8Rows or a tensor")
-    need(type(w) is W4Weight, "gemm_w4: w must be a W4Weight")
-    rows = x.q if q8 else x
-    _need_here("gemm_w4", rows, w.packed, bias, out)
+    if not (q8 or isinstance(x, torch.Tensor)) or type(w) is not W4Weight:
+        raise KernelError("gemm_w4: x must be Q8Rows or a tensor, w a W4Weight")
+    dt = x.dtype
+    code = dtype_code(dt)
     if q8:
+        M, K, at, index, ld = x.T, x.K, x.at, x.index, padded_columns(x.K, x.group)
         if x.group != w.group:
             raise KernelError(f"gemm_w4: rows in groups of {x.group}, the weight in groups of {w.group}")
-        K = x.K
     else:
         need(x.dim() == 2 and x.stride(1) == 1, "gemm_w4: x must be [M, K] with unit inner stride")
-        K = x.shape[1]
+        M, K = x.shape
+        at, index, ld = x.data_ptr(), x.get_device(), x.stride(0)
+    here, N = _device_for(index), w.N
+    if index != here or w.index != here:
+        _elsewhere("gemm_w4", w.index if index == here else index)
     if K != w.K:
         raise KernelError(f"gemm_w4: inner sizes differ ({K} vs {w.K})")
-    M, N, dt = rows.shape[0], w.N, x.dtype
-    dtype_code(dt)
+    bias_at, bias_f32 = None, False
     if bias is not None:
-        need(bias.shape == (N,) and bias.dtype in (torch.float32, torch.bfloat16) and bias.is_contiguous(), "gemm_w4: bias must be [N]")
-    odt = torch.float32 if out_f32 or accumulate else dt
+        bias_at, bias_f32 = bias.data_ptr(), bias.dtype == torch.float32
+        need(bias.shape == (N,) and (bias_f32 or bias.dtype == torch.bfloat16) and bias.is_contiguous(), "gemm_w4: bias must be [N]")
+        if bias.get_device() != here:
+            _elsewhere("gemm_w4", bias.get_device())
+    f32 = out_f32 or accumulate or code == 0
     if out is None:
         need(not accumulate, "gemm_w4: accumulate needs an output tensor")
-        out = torch.empty((M, N), dtype=odt, device=rows.device)
+        out = torch.empty(M, N, dtype=torch.float32 if f32 else dt, device=w.packed.device)
     else:
-        need(out.shape == (M, N) and out.dtype == odt and out.is_contiguous(), "gemm_w4: output must be [M, N], contiguous, of the result's dtype")
+        need(out.shape == (M, N) and out.dtype == (torch.float32 if f32 else dt) and out.is_contiguous(),
+             "gemm_w4: output must be [M, N], contiguous, of the result's dtype")
+        if out.get_device() != here:
+            _elsewhere("gemm_w4", out.get_device())
     if M == 0:
         return out
-    if not q8 and (dt == torch.float32 or M > W4_FEW_TOKENS):
+    if not q8 and (code == 0 or M > W4_FEW_TOKENS):
         return _gemm_through_16_bits(x, w, bias, out, accumulate)
-    at, ld = rows.data_ptr(), rows.stride(0)
-    whole = q8 or (ld % 8 == 0 and at % 16 == 0)
-    tiled = w4_tc_launch(q8, M, N, K, w.group, _clusters_on(rows.get_device())) if whole else None
+    on = _clusters_on(here)
+    tiled = w4_tc_launch(q8, M, N, K, w.group, on) if q8 or (ld % 8 == 0 and at % 16 == 0) else None
     if tiled:
-        code = _f("rf_gemm_w4_tc")(0 if q8 else 1, at, x.scales.data_ptr() if q8 else None, ld, w.packed.data_ptr(), w.scales.data_ptr(), ptr(bias),
-                                   bias is not None and bias.dtype == torch.float32, out.data_ptr(), odt == torch.float32, accumulate, *tiled,
-                                   M, N, K, w.group, tc.status_word(rows.device).data_ptr(), stream())
-        check(code, "gemm_w4" if code == 0 else f"gemm_w4 ({M}x{N}x{K}, tiles of {tiled[0]} tokens)")
-        return out
-    plan = w4_launch(q8, M, N, K, w.group, _clusters_on(rows.get_device()))
-    code = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales.data_ptr() if q8 else None, ld, w.packed.data_ptr(), w.scales.data_ptr(), ptr(bias),
-                            bias is not None and bias.dtype == torch.float32, out.data_ptr(), odt == torch.float32, accumulate, *plan, M, N, K, w.group, stream())
-    check(code, "gemm_w4" if code == 0 else f"gemm_w4 ({M}x{N}x{K})")
+        done = _f("rf_gemm_w4_tc")(0 if q8 else 1, at, x.scales_at if q8 else None, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
+                                   *tiled, M, N, K, w.group, tc.status_word(w.packed.device).data_ptr(), stream())
+    else:
+        done = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales_at if q8 else None, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
+                                *w4_launch(q8, M, N, K, w.group, on), M, N, K, w.group, stream())
+    check(done, "gemm_w4" if done == 0 else f"gemm_w4 ({M}x{N}x{K}, groups of {w.group})")
     return out
 
 
