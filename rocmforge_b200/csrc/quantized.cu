@@ -351,18 +351,22 @@ __device__ __forceinline__ unsigned long long fma_two(unsigned long long a, unsi
 #define W4_SLOT (1024 + 128)                             // a unit's weights, and its scales [group][16 rows]
 #define W4_SUMS(rt) (16 * (rt) * W4_WARPS + 4)           // pitch of the warps' sums [token][16 rt rows a warp]
 // Shared memory of a block: tokens' numbers (rows a pitch apart by which eight tokens' reads meet every bank once), their scales
-// [group][token], the warps' sums (two sets for a cluster, none where a tile is one warp's), the rings.
+// [group][token], the warps' sums (two sets for a cluster that has several rounds, none where a tile is one warp's), the rings.
 struct W4Shared {
     int columns, pitch, scales, sums, ring, bytes;
 };
 __host__ __device__ constexpr int w4_depth(int nb, int rt) { return nb == 1 ? 6 : nb == 2 ? 4 / rt + (rt - 1) : 3 - (rt - 1); }
-__host__ __device__ inline W4Shared w4_shared(int units, int ways, int splits, int G, int size, int M, int nb, int rt) {
+__host__ __device__ inline int w4_rounds(int N, int rt, int ways, int clusters) {
+    const int tiles = ((N + 15) / 16 + rt - 1) / rt, at_once = W4_WARPS / ways * clusters;
+    return (tiles + at_once - 1) / at_once;
+}
+__host__ __device__ inline W4Shared w4_shared(int units, int rounds, int ways, int splits, int G, int size, int M, int nb, int rt) {
     W4Shared s;
     s.columns = (units + splits - 1) / splits * 128;
     s.pitch = s.columns * size + (size == 1 ? 32 : 64);
     s.scales = (M < 8 * nb ? M : 8 * nb) * s.pitch;
     s.sums = s.scales + (size == 1 ? s.columns / G * 8 * nb * 4 : 0);
-    s.ring = s.sums + (splits > 1 ? 2 : ways > 1 ? 1 : 0) * 8 * nb * W4_SUMS(rt) * 4;
+    s.ring = s.sums + (splits > 1 && rounds > 1 ? 2 : splits > 1 || ways > 1 ? 1 : 0) * 8 * nb * W4_SUMS(rt) * 4;
     s.bytes = s.ring + W4_WARPS * w4_depth(nb, rt) * rt * W4_SLOT;
     return s;
 }
@@ -375,11 +379,11 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_trigger();
     const int units = (blocks + 1) / 2, all_groups = blocks * 64 / G;
-    const W4Shared sh = w4_shared(units, ways, splits, G, (int)sizeof(X), o.M, NB, RT);
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rank = blockIdx.x % splits, cluster = blockIdx.x / splits, clusters = gridDim.x / splits;
-    const int tiles16 = (o.N + 15) / 16, tiles = (tiles16 + RT - 1) / RT, at_once = W4_WARPS / ways, rounds = (tiles + clusters * at_once - 1) / (clusters * at_once);
+    const int tiles16 = (o.N + 15) / 16, tiles = (tiles16 + RT - 1) / RT, at_once = W4_WARPS / ways, rounds = w4_rounds(o.N, RT, ways, clusters);
+    const W4Shared sh = w4_shared(units, rounds, ways, splits, G, (int)sizeof(X), o.M, NB, RT);
     const int tok0 = blockIdx.y * 8 * NB, live = min(8 * NB, o.M - tok0);
     const int first = (int)((long long)units * rank / splits), count = (int)((long long)units * (rank + 1) / splits) - first;
     const int from = first + count * (warp % ways) / ways, to = first + count * (warp % ways + 1) / ways;
@@ -785,10 +789,10 @@ int rf_weights_made(cudaStream_t st) {
     return 0;
 }
 
-// Bytes of shared memory that a product's block takes with `eights` eights of tokens, `pair` tiles of 16 rows a warp, `ways` warps a tile and a
-// share of the columns in `splits`.
-int rf_gemm_w4_shared(int x_kind, int M, int K, int G, int eights, int pair, int ways, int splits) {
-    return w4_shared((padded(K, G) / 64 + 1) / 2, ways, splits, G, x_kind == 0 ? 1 : 2, M, eights, pair).bytes;
+// Bytes of shared memory that a product's block takes with `eights` eights of tokens, `pair` tiles of 16 rows a warp, `ways` warps a tile, a
+// share of the columns in `splits` and `clusters` clusters.
+int rf_gemm_w4_shared(int x_kind, int M, int N, int K, int G, int eights, int pair, int ways, int splits, int clusters) {
+    return w4_shared((padded(K, G) / 64 + 1) / 2, w4_rounds(N, pair, ways, clusters), ways, splits, G, x_kind == 0 ? 1 : 2, M, eights, pair).bytes;
 }
 
 // Clusters of `splits` blocks, each with an SM of its own, that run at once on the current device (< 0: an error).
@@ -818,7 +822,7 @@ int rf_gemm_w4(int x_kind, const void* x, const void* xs, long long ldx, const v
     if ((x_kind == 0 && (!aligned(x, 16) || ldx % 16)) || !aligned(packed, 16) || !aligned(scales, 16)) return RF_ERR_BAD_ARG;
     if (splits < 1 || splits > 8 || clusters < 1 || ways < 1 || ways > W4_WARPS || (ways & (ways - 1)) || eights < 1) return RF_ERR_BAD_ARG;
     const int whole = x_kind == 0 || (K % 8 == 0 && ldx % 8 == 0 && aligned(x, 16));
-    const int blocks = padded(K, G) / 64, smem = rf_gemm_w4_shared(x_kind, M, K, G, eights, pair, ways, splits);
+    const int blocks = padded(K, G) / 64, smem = rf_gemm_w4_shared(x_kind, M, N, K, G, eights, pair < 1 ? 1 : pair, ways, splits, clusters);
     const long long y = (M + 8ll * eights - 1) / (8 * eights);
     if (smem > W4_MOST_SHARED || y > 65535 || (long long)clusters * splits > 0x7fffffffll) return RF_ERR_UNSUPPORTED;
     const W4Out o{out, bias, bias_is_f32, out_is_f32, add, M, N};

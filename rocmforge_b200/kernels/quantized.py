@@ -25,7 +25,7 @@ _LAUNCHERS = {
     "rf_quantize_w4": [_i, _p, _n, _p, _p, _i, _i, _i, _p],
     "rf_dequantize_w4": [_i, _p, _p, _p, _i, _i, _i, _i, _i, _p],
     "rf_weights_made": [_p],
-    "rf_gemm_w4_shared": [_i, _i, _i, _i, _i, _i, _i, _i],
+    "rf_gemm_w4_shared": [_i, _i, _i, _i, _i, _i, _i, _i, _i, _i],
     "rf_gemm_w4_clusters": [_i],
     "rf_gemm_w4": [_i, _p, _p, _n, _p, _p, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p],
 }
@@ -324,7 +324,9 @@ def w4_clusters(splits: int, device: int) -> int:
 
 @functools.lru_cache(4096)
 def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
-    """(eights of tokens, tiles a warp, warps a tile, splits, clusters): how ``rf_gemm_w4`` shares out a product.  Chosen from sizes alone."""
+    """(eights of tokens, tiles a warp, warps a tile, splits, clusters): how ``rf_gemm_w4`` shares out a product.  Chosen from sizes alone: the
+    units of 128 columns that the busiest warp goes through, 1.9 for a unit of two tiles, one more a round in which warps wait for one
+    another, three more where clusters exchange their sums."""
     units, rows16 = (padded_columns(K, group) // 64 + 1) // 2, (N + 15) // 16
     eights, best = 1 if M <= 8 else 2 if M <= 16 else 4, None
     while eights and best is None:                       # fewer tokens at once where longer rows leave no room for more
@@ -334,12 +336,14 @@ def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
             for splits in range(1, 9):
                 clusters = max(1, clusters_of(splits) // shares)
                 for ways in (1, 2, 4, 8, 16):
-                    if _f("rf_gemm_w4_shared")(0 if q8 else 1, M, K, group, eights, pair, ways, splits) > W4_MOST_SHARED:
+                    used = min(clusters, (tiles * ways + 15) // 16)
+                    if _f("rf_gemm_w4_shared")(0 if q8 else 1, M, N, K, group, eights, pair, ways, splits, used) > W4_MOST_SHARED:
                         continue
-                    rounds = (tiles + clusters * (16 // ways) - 1) // (clusters * (16 // ways))
-                    cost = rounds * ((units + splits * ways - 1) // (splits * ways) * (1.5 if pair == 2 else 1) + 1) + (splits > 1)
+                    rounds = (tiles + used * (16 // ways) - 1) // (used * (16 // ways))
+                    each = (units + splits * ways - 1) // (splits * ways) * (1.9 if pair == 2 else 1)
+                    cost = rounds * (each + (ways > 1 or splits > 1)) + 3 * (splits > 1)
                     if best is None or cost < best[0]:
-                        best = cost, eights, pair, ways, splits, min(clusters, (tiles * ways + 15) // 16)
+                        best = cost, eights, pair, ways, splits, used
         eights //= 2
     if best is None:
         raise KernelError(f"gemm_w4: rows of {K} columns are too long")

@@ -193,7 +193,7 @@ def test_every_way_to_share_out_a_product(monkeypatch, M, eights, pair, ways, cl
     x, x64, w, full = product_case(kind, M, N, K, G)
     x64, full = x64.to(DEV), full.to(DEV)
     h = numbers(M, N, seed=9)
-    if quantized._f("rf_gemm_w4_shared")(0 if kind == "q8" else 1, M, K, G, eights, pair, ways, splits) > quantized.W4_MOST_SHARED:
+    if quantized._f("rf_gemm_w4_shared")(0 if kind == "q8" else 1, M, N, K, G, eights, pair, ways, splits, clusters) > quantized.W4_MOST_SHARED:
         with pytest.raises(kernels.KernelError, match="not supported"):
             kernels.gemm_w4(x, w, out=h.to(DEV), accumulate=True)
         return
