@@ -201,7 +201,7 @@ class StepContext:
         tc = kernels.tensor_core
         w = gate_up.weight
         if isinstance(w, W4Weight):
-            if y.shape[0] <= kernels.W4_FEW_TOKENS or self.compute_dtype != torch.bfloat16:
+            if y.shape[0] <= kernels.W4_TC_MOST or self.compute_dtype != torch.bfloat16:
                 gu = self.matmul(y, w, gate_up.bias)
                 if activation == "clamped_glu":
                     return kernels.clamped_glu(gu, limit, alpha)

@@ -124,7 +124,7 @@ class Model:
         if self.device.type != "cuda":
             raise RuntimeError("rocmforge_b200 models run on a CUDA device only (there is no CPU fallback)")
         self.options = options or Options()
-        build.ensure_built(spec.cuda_modules(compute_dtype) + (["quantized"] if self.options.weight_bits == 4 else []))
+        build.ensure_built(spec.cuda_modules(compute_dtype) + (["quantized", "quantized_tc"] if self.options.weight_bits == 4 else []))
         for prefix, part in spec.named_parts().items():
             local = {name[len(prefix):]: t for name, t in params.items()
                      if name.startswith(prefix) and name[len(prefix):] in part.param_specs()}

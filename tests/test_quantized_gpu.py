@@ -189,7 +189,8 @@ def test_every_way_to_share_out_a_product(monkeypatch, M, eights, pair, ways, cl
     from rocmforge_b200 import kernels
     from rocmforge_b200.kernels import quantized
     monkeypatch.setattr(quantized, "w4_launch", lambda *a: (eights, pair, ways, splits, clusters))
-    monkeypatch.setattr(quantized, "w4_tc_launch", lambda *a: None)
+    monkeypatch.setattr(quantized, "W4_TC_TOKENS", 1000)
+    monkeypatch.setattr(quantized, "W4_FEW_TOKENS", 1000)
     x, x64, w, full = product_case(kind, M, N, K, G)
     x64, full = x64.to(DEV), full.to(DEV)
     h = numbers(M, N, seed=9)
@@ -201,22 +202,21 @@ def test_every_way_to_share_out_a_product(monkeypatch, M, eights, pair, ways, cl
     close(got, x64 @ full.T + h.double().to(DEV), x64.abs() @ full.abs().T + h.double().abs().to(DEV), terms_of(kind, K) + 1, F32)
 
 
-@pytest.mark.parametrize("M,bn", [(1, 32), (32, 32), (40, 32), (64, 64), (33, 64), (129, 64), (128, 128), (100, 128), (300, 128)])
-@pytest.mark.parametrize("kind", ["q8", "bf16"])
+@pytest.mark.parametrize("M,bn", [(1, 32), (32, 32), (40, 32), (64, 64), (33, 64), (129, 64), (128, 128), (100, 128), (300, 128), (256, 256), (129, 256), (300, 256)])
 @pytest.mark.parametrize("splits", [1, 2, 3, 8])
 @pytest.mark.parametrize("N,K,G", [(300, 1088, 32), (130, 200, 64), (17, 2176, 128), (450, 72, 128), (128, 3328, 32)])
-def test_every_tile_on_the_tensor_cores(monkeypatch, M, bn, kind, splits, N, K, G):
+def test_every_tile_on_the_tensor_cores(monkeypatch, M, bn, splits, N, K, G):
     """Tiles of tokens that are not full, rows of weights that end inside a tile, shares of the columns that are empty."""
     from rocmforge_b200 import kernels
     from rocmforge_b200.kernels import quantized
     monkeypatch.setattr(quantized, "w4_tc_launch", lambda *a: (bn, splits))
-    monkeypatch.setattr(quantized, "W4_FEW_TOKENS", 1000)
-    x, x64, w, full = product_case(kind, M, N, K, G)
+    monkeypatch.setattr(quantized, "W4_TC_TOKENS", 1)
+    x, x64, w, full = product_case("bf16", M, N, K, G)
     x64, full = x64.to(DEV), full.to(DEV)
     b, h = numbers(N, seed=2), numbers(M, N, seed=9)
     got = kernels.gemm_w4(x, w, b.to(DEV), out=h.to(DEV), accumulate=True)
-    close(got, x64 @ full.T + (h.double() + b.double()).to(DEV), x64.abs() @ full.abs().T + (h.double().abs() + b.double().abs()).to(DEV), terms_of(kind, K) + 2, F32)
-    close(kernels.gemm_w4(x, w), x64 @ full.T, x64.abs() @ full.abs().T, terms_of(kind, K), BF)
+    close(got, x64 @ full.T + (h.double() + b.double()).to(DEV), x64.abs() @ full.abs().T + (h.double().abs() + b.double().abs()).to(DEV), terms_of("bf16", K) + 2, F32)
+    close(kernels.gemm_w4(x, w), x64 @ full.T, x64.abs() @ full.abs().T, terms_of("bf16", K), BF)
     kernels.tensor_core.check_status(torch.device(DEV))
 
 
