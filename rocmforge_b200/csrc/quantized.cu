@@ -825,7 +825,7 @@ int rf_gemm_w4(int x_kind, const void* x, const void* xs, long long ldx, const v
     const int blocks = padded(K, G) / 64, smem = rf_gemm_w4_shared(x_kind, M, N, K, G, eights, pair < 1 ? 1 : pair, ways, splits, clusters);
     const long long y = (M + 8ll * eights - 1) / (8 * eights);
     if (smem > W4_MOST_SHARED || y > 65535 || (long long)clusters * splits > 0x7fffffffll) return RF_ERR_UNSUPPORTED;
-    const W4Out o{out, bias, bias_is_f32, out_is_f32, add, M, N};
+    const W4Out o = w4_out(out, bias, bias_is_f32, out_is_f32, add, M, N);
     int bad = 0;
     const bool known = with_product(x_kind, G, eights, pair, [&](auto gc, auto rows, auto nb, auto rt) {
         using X = std::remove_cv_t<std::remove_pointer_t<decltype(rows)>>;

@@ -20,6 +20,7 @@ struct W4Out {
     void* out;               // [M, N] float32 if is_f32, else bfloat16; add: float32, added into
     const void* bias;        // [N] or null
     int bias_is_f32, is_f32, add, M, N;
+    int fours;               // four neighbours of a row lie together on a boundary of their size
 };
 __device__ __forceinline__ void w4_write(const W4Out& o, int t, int n, float v) {
     if (n >= o.N) return;
@@ -29,8 +30,34 @@ __device__ __forceinline__ void w4_write(const W4Out& o, int t, int n, float v) 
     else if (o.is_f32) reinterpret_cast<float*>(o.out)[at] = v;
     else reinterpret_cast<__nv_bfloat16*>(o.out)[at] = __float2bfloat16_rn(v);
 }
-
+// Columns n .. n + 3, n a multiple of 4.
+__device__ __forceinline__ void w4_write4(const W4Out& o, int t, int n, float4 v) {
+    if (n >= o.N) return;
+    if (!o.fours) {
+        w4_write(o, t, n, v.x), w4_write(o, t, n + 1, v.y), w4_write(o, t, n + 2, v.z), w4_write(o, t, n + 3, v.w);
+        return;
+    }
+    if (o.bias != nullptr) {
+        v.x += load_vec(o.bias, o.bias_is_f32, n), v.y += load_vec(o.bias, o.bias_is_f32, n + 1);
+        v.z += load_vec(o.bias, o.bias_is_f32, n + 2), v.w += load_vec(o.bias, o.bias_is_f32, n + 3);
+    }
+    const size_t at = (size_t)t * o.N + n;
+    if (o.is_f32) {
+        float4* to = reinterpret_cast<float4*>(reinterpret_cast<float*>(o.out) + at);
+        if (o.add) {
+            const float4 old = *to;
+            v.x += old.x, v.y += old.y, v.z += old.z, v.w += old.w;
+        }
+        *to = v;
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+        *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(o.out) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+}
 
 static bool bad_group(int G) { return G != 32 && G != 64 && G != 128; }
 static int padded(int K, int G) { const int u = G > 64 ? G : 64; return (K + u - 1) / u * u; }
 static bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+static W4Out w4_out(void* out, const void* bias, int bias_is_f32, int is_f32, int add, int M, int N) {
+    return {out, bias, bias_is_f32, is_f32, add, M, N, N % 4 == 0 && aligned(out, is_f32 ? 16 : 8)};
+}

@@ -6,25 +6,34 @@
 // reads it.  Two groups of eight warps do every second stage each.  The tokens' numbers come by TMA into a ring of their own.  Long rows are
 // shared out to the CTAs of a cluster, which add up their sums through shared memory in the order of their ranks.
 //
+// The tensor cores cut what an addition loses instead of rounding it, and what is cut adds up (1,999 x 3,584 x 18,944 against 64 bits: one sum
+// 1.1e-5 off, pieces of 6,315 columns 2.6e-6).  For 32-bit results a sum runs over W4T_PIECE columns at most: the widening warps add it to a
+// second one beside it, rounded, while the next piece goes into another accumulator (tiles of 256 tokens: into the same one, after a wait).
+//
 // Every wait on an mbarrier is bounded (2 s): status word 13.
 #include <type_traits>
 #include "quantized.cuh"
 #include "tcgen05_common.cuh"
 
-#define W4T_THREADS (32 * 18)                            // the tokens' producer, the MMA issuer, sixteen widening warps (eight write the result)
+#define W4T_THREADS (32 * 18)                            // the tokens' producer, the MMA issuer, sixteen widening warps (which write the result)
+#define W4T_PIECE 2048                                   // columns of one sum where the result is 32-bit
 #define W4T_PITCH (128 + 4)                              // of the sums that a cluster exchanges, [token][row]
 #define W4T_MOST_SHARED (226 * 1024)                     // (the abort flag has a place of its own)
 
-template <int BN>
+template <int BN, int G>
 struct TcShape {
-    static constexpr int BLOCKS = BN <= 128 ? 2 : 1;     // blocks of 64 columns a stage: what a stage costs beside its work, twice as rarely
+    static constexpr int BLOCKS = BN <= 64 ? 2 : 1;      // blocks of 64 columns a stage: what a stage costs beside its work, twice as rarely
     static constexpr int A = BLOCKS * 128 * 128, B = BLOCKS * BN * 128;
-    static constexpr int STAGES = 4, ROWS = BN == 128 ? 2 : 4;          // places of weights, of tokens' numbers
+    static constexpr int STAGES = 4, ROWS = BN == 128 ? 8 : 4;          // places of weights, of tokens' numbers
     static constexpr int TURN = STAGES / 2;              // a warp's stages until it is back at the same place (a group sees all phases of it)
-    static constexpr int AHEAD = 8 / BLOCKS;             // stages of its own that a warp has asked for
+    static constexpr int AHEAD = BLOCKS == 2 && G == 32 ? 2 : 4;        // stages of its own that a warp has asked for (more scales leave room for fewer)
+    static constexpr int PIECE = W4T_PIECE / 64 / BLOCKS;                               // stages of a piece
+    static constexpr int BUFS = BN <= 128 ? 2 : 1, TMEM = BN == 256 ? 512 : 4 * BN;     // accumulators; with them, behind, the pieces' sum
+    static constexpr int SHARE = BN / 4 < 16 ? 16 : BN / 4;             // a widening warp's part of the sums: 32 rows, so many tokens
+    static_assert(PIECE % 8 == 0 && PIECE / 2 % AHEAD == 0 && AHEAD % TURN == 0, "pieces end between turns");
     static constexpr int RINGS = STAGES * A + ROWS * B, BYTES = RINGS + 1024 + 256;     // (alignment, barriers)
     static_assert(RINGS >= BN * W4T_PITCH * 4, "the rings' place holds the sums");
-    static_assert(BYTES <= W4T_MOST_SHARED && 8 % ROWS == 0 && 8 % STAGES == 0, "eight stages on, every ring is back where it was");
+    static_assert(BYTES <= W4T_MOST_SHARED && 8 % ROWS == 0 && 8 % STAGES == 0, "eight stages on, every ring is back where it was (one of eight with the parity turned)");
 };
 
 // Bounded wait as mbar_wait, asleep between looks: what waits here waits long, and the widening warps need the issue slots.
@@ -60,16 +69,74 @@ __device__ __forceinline__ void four_pairs(uint32_t at, uint32_t word, uint32_t 
                  ::"r"(at), "r"(widened(w, s)), "r"(widened(w >> 8, s)), "r"(widened(w >> 4, s)), "r"(widened(w >> 12, s)) : "memory");
 }
 
+// A widening warp's share of a piece's sum added to the sum of those before.
+template <int BN, int G>
+__device__ __noinline__ bool add_piece(uint32_t tmem, uint32_t sum_full, int piece, volatile int* abort_flag) {
+    using S = TcShape<BN, G>;
+    const int buf = piece % S::BUFS, warp = threadIdx.x >> 5, share = (warp - 2) / 4 * S::SHARE;
+    if (!__all_sync(0xffffffffu, wait_for(sum_full + 8 * buf, piece / S::BUFS & 1, abort_flag))) return false;
+    tcgen05_fence_after();
+    if (share < BN) {
+        const uint32_t rows = tmem + ((uint32_t)((warp & 3) * 32) << 16) + share;
+#pragma unroll 1
+        for (int c = 0; c < S::SHARE; c += 16) {
+            uint32_t a[16], b[16];
+            tcgen05_ld16(rows + buf * BN + c, a);
+            if (piece > 0) tcgen05_ld16(rows + S::BUFS * BN + c, b);
+            tcgen05_wait_ld();
+            if (piece > 0) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) + __uint_as_float(b[j]));
+            }
+            tcgen05_st16(rows + S::BUFS * BN + c, a);
+        }
+        tcgen05_wait_st();
+    }
+    tcgen05_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) at_arrive(sum_full + 8 * (S::BUFS + buf));
+    return true;
+}
+
+// 32 rows of sixteen tokens (from c on) of the result: the last piece's sum and that of those before, into `sums` ([token][row]) or, without,
+// straight out.  (Functions of their own keep these parts' registers out of the loop over the weights: written there, 64 x 37,888 x 3,584 took
+// 51 us, not 36.)
+__device__ __noinline__ void write_16(uint32_t last_sum, uint32_t sum_before, bool any, bool more, float* sums, int row0, int c, int tok0, int live, W4Out o) {
+    uint32_t r[16], before[16];
+    float old[16];
+    if (any) tcgen05_ld16(last_sum + c, r);
+    if (more) tcgen05_ld16(sum_before + c, before);
+    const int at_row = 32 * (threadIdx.x >> 5 & 3) + (threadIdx.x & 31), row = row0 + at_row;
+    const bool there = row < o.N;
+    const size_t to = (size_t)(tok0 + c) * o.N + row;
+    const float bias = there && o.bias != nullptr ? load_vec(o.bias, o.bias_is_f32, row) : 0.f;
+    if (sums == nullptr && o.add) {                      // (all at once: a load after every store would wait for it)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) old[j] = there && c + j < live ? reinterpret_cast<const float*>(o.out)[to + (size_t)j * o.N] : 0.f;
+    }
+    tcgen05_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const float v = any ? __uint_as_float(r[j]) + (more ? __uint_as_float(before[j]) : 0.f) : 0.f;
+        if (sums != nullptr) sums[(c + j) * W4T_PITCH + at_row] = v;
+        else if (there && c + j < live) {
+            if (o.add) reinterpret_cast<float*>(o.out)[to + (size_t)j * o.N] = v + bias + old[j];
+            else if (o.is_f32) reinterpret_cast<float*>(o.out)[to + (size_t)j * o.N] = v + bias;
+            else reinterpret_cast<__nv_bfloat16*>(o.out)[to + (size_t)j * o.N] = __float2bfloat16_rn(v + bias);
+        }
+    }
+}
+
 template <int BN, int G>
 __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const uint4* __restrict__ w0, const uint32_t* __restrict__ w1,
-                                                               int blocks, int splits, int* status, W4Out o) {
-    using S = TcShape<BN>;
+                                                               int blocks, int splits, bool pieces, int* status, W4Out o) {
+    using S = TcShape<BN, G>;
     constexpr int SCALES = S::BLOCKS * 64 > G ? S::BLOCKS * 64 / G : 1;                 // groups that a stage touches
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::RINGS);                      // weights' places full, empty, tokens' full, empty, the sums
-    constexpr int FULL = 0, EMPTY = S::STAGES, ROWS_FULL = 2 * S::STAGES, ROWS_EMPTY = ROWS_FULL + S::ROWS, SUMS = ROWS_EMPTY + S::ROWS;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + SUMS + 1);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::RINGS);                      // weights' places full, empty, tokens' full, empty, sums full, added
+    constexpr int FULL = 0, EMPTY = S::STAGES, ROWS_FULL = 2 * S::STAGES, ROWS_EMPTY = ROWS_FULL + S::ROWS, SUMS = ROWS_EMPTY + S::ROWS, ADDED = SUMS + S::BUFS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + ADDED + S::BUFS);
     __shared__ int abort_flag;
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -83,12 +150,13 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
             mbar_init(smem_u32(&bars[FULL + i]), 8);     // eight widening warps
             mbar_init(smem_u32(&bars[EMPTY + i]), 1);
         }
-        for (int i = 0; i < 2 * S::ROWS + 1; ++i) mbar_init(smem_u32(&bars[ROWS_FULL + i]), 1);
+        for (int i = 0; i < 2 * S::ROWS + S::BUFS; ++i) mbar_init(smem_u32(&bars[ROWS_FULL + i]), 1);
+        for (int i = 0; i < S::BUFS; ++i) mbar_init(smem_u32(&bars[ADDED + i]), 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
     }
     if (warp == 1) {
-        tcgen05_alloc(smem_u32(tmem_slot), BN);
+        tcgen05_alloc(smem_u32(tmem_slot), S::TMEM);
         tcgen05_relinquish();
     }
     // the widening warps' weights: stages phase, phase + 2, ... of a tile of 16 rows, AHEAD of them in registers before anything is waited for
@@ -119,6 +187,8 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
     tcgen05_fence_after();
     const uint32_t tmem = *tmem_slot;
 
+    const int last = pieces && n > 0 ? (n - 1) / S::PIECE : 0;           // the piece that the result is read from, together with the sum of those before
+    const uint32_t sum_full = smem_u32(&bars[SUMS]), added = smem_u32(&bars[ADDED]);
     bool ok = true;
     if (warp == 0) {
         // ---------------- the tokens' numbers
@@ -130,7 +200,7 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
                 for (int u = 0; u < 8; ++u) {
                     if (i + u >= n) break;
                     const int at = u % S::ROWS;
-                    if (i > 0 || u >= S::ROWS) ok = wait_for(empty + 8 * at, (u / S::ROWS & 1) ^ 1, &abort_flag);
+                    if (i > 0 || u >= S::ROWS) ok = wait_for(empty + 8 * at, ((S::ROWS == 8 ? i / 8 : u / S::ROWS) & 1) ^ 1, &abort_flag);
                     if (!ok) break;
                     mbar_expect_tx(full + 8 * at, S::B);
 #pragma unroll
@@ -146,24 +216,35 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
         if (elect_one()) {
             const uint32_t full = smem_u32(&bars[FULL]), empty = smem_u32(&bars[EMPTY]), rows_full = smem_u32(&bars[ROWS_FULL]), rows_empty = smem_u32(&bars[ROWS_EMPTY]);
             const uint64_t da0 = make_smem_desc(smem_u32(smem)), db0 = make_smem_desc(smem_u32(smem) + S::STAGES * S::A);
-            for (int i = 0; i < n && ok; i += 8) {
+            uint32_t sum = tmem;
+            bool starts = true;
+            for (int i = 0; i < n && ok; i += 8, starts = false) {
+                if (pieces && i > 0 && i % S::PIECE == 0) {
+                    const int piece = i / S::PIECE, buf = piece % S::BUFS;
+                    tcgen05_commit(sum_full + 8 * ((piece - 1) % S::BUFS));
+                    if (piece >= S::BUFS) ok = wait_for(added + 8 * buf, piece / S::BUFS - 1 & 1, &abort_flag);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    sum = tmem + buf * BN;
+                    starts = true;
+                }
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
                     if (i + u >= n) break;
                     const int a = u % S::STAGES, r = u % S::ROWS;
-                    ok = wait_for(rows_full + 8 * r, u / S::ROWS & 1, &abort_flag) && wait_for(full + 8 * a, u / S::STAGES & 1, &abort_flag);
+                    ok = wait_for(rows_full + 8 * r, (S::ROWS == 8 ? i / 8 : u / S::ROWS) & 1, &abort_flag) && wait_for(full + 8 * a, u / S::STAGES & 1, &abort_flag);
                     if (!ok) break;
                     tcgen05_fence_after();
 #pragma unroll
                     for (int k = 0; k < 4 * S::BLOCKS; ++k) {           // 16 columns
                         const uint64_t da = da0 + (a * S::A + k / 4 * 128 * 128) / 16 + 2 * (k % 4), db = db0 + (r * S::B + k / 4 * BN * 128) / 16 + 2 * (k % 4);
-                        tcgen05_mma_bf16(tmem, da, db, make_idesc(BN), (i | u | k) ? 1u : 0u);
+                        tcgen05_mma_bf16(sum, da, db, make_idesc(BN), u || k || !starts ? 1u : 0u);
                     }
                     tcgen05_commit(empty + 8 * a);
                     tcgen05_commit(rows_empty + 8 * r);
                 }
             }
-            tcgen05_commit(smem_u32(&bars[SUMS]));
+            tcgen05_commit(sum_full + 8 * (last % S::BUFS));
         }
     } else {
         // ---------------- the weights
@@ -175,12 +256,19 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
 #pragma unroll
         for (int j = 0; j < 2; ++j) place[j] = smem_u32(smem) + phase * S::A + (16 * (wide & 7) + g) * 128 + (((4 * (odd ^ j) + t) ^ g) * 16);
         const uint32_t full = smem_u32(&bars[FULL + phase]), empty = smem_u32(&bars[EMPTY + phase]);
+        int summed = 0;
         uint32_t parity = 1;
         for (int done = 0; done < stages && ok;) {
 #pragma unroll
             for (int u = 0; u < S::AHEAD; ++u, ++done) {
                 if (done >= stages) break;
                 const int at = u % S::TURN * 2;
+                // (a piece is added once the next one's first stages are on their way)
+                if (u == S::TURN % S::AHEAD && (done - S::TURN) / (S::PIECE / 2) > summed && summed < last) {
+                    ok = add_piece<BN, G>(tmem, smem_u32(&bars[SUMS]), summed, &abort_flag);
+                    if (!ok) break;
+                    ++summed;
+                }
                 if (done >= S::TURN) {
                     ok = wait_for(empty + 8 * at, parity, &abort_flag);
                     if (!ok) break;
@@ -204,55 +292,40 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
                 if (u % S::TURN == S::TURN - 1) parity ^= 1;
             }
         }
+        for (; ok && summed < last; ++summed) ok = add_piece<BN, G>(tmem, smem_u32(&bars[SUMS]), summed, &abort_flag);
     }
     pdl_wait();                                          // (whoever writes from here on has waited)
-    // ---------------- the sums: eight warps read 32 rows of half the tokens each; a cluster's go through the rings' place, one CTA's straight out
-    const int quarter = warp & 3, cols0 = warp >= 14 ? BN / 2 : 0;
-    const bool adds = warp >= 10;
-    if (adds && n > 0) {
-        ok = wait_for(smem_u32(&bars[SUMS]), 0, &abort_flag) && ok;
+    // ---------------- the result: a warp has the same share as of the pieces; a cluster's go through the rings' place, one CTA's straight out
+    const int share = (warp - 2) / 4 * S::SHARE;
+    const bool writes = warp >= 2 && share < BN;
+    if (writes && n > 0) {
+        ok = wait_for(sum_full + 8 * (last % S::BUFS), last / S::BUFS & 1, &abort_flag) && ok;
         tcgen05_fence_after();
     }
-    __syncwarp();
+    ok = __all_sync(0xffffffffu, ok);
     if (splits > 1) __syncthreads();                     // (the sums are there: every product has read the rings)
-    if (adds && ok) {
-        float* sums = reinterpret_cast<float*>(smem) + 32 * quarter + lane;
-        const int row = row0 + 32 * quarter + lane;
-        constexpr int CH = BN / 2 < 32 ? 16 : 32;
+    if (writes && ok) {
+        const uint32_t rows = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
 #pragma unroll 1
-        for (int c = 0; c < BN / 2; c += CH) {
-            uint32_t r[CH];
-            const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + cols0 + c;
-            if (n > 0) {
-                if constexpr (CH == 32) tcgen05_ld32(at, r);
-                else tcgen05_ld16(at, r);
-                tcgen05_wait_ld();
-            }
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                const float v = n > 0 ? __uint_as_float(r[j]) : 0.f;
-                const int tok = cols0 + c + j;
-                if (splits > 1) sums[tok * W4T_PITCH] = v;
-                else if (tok < live) w4_write(o, tok0 + tok, row, v);
-            }
-        }
+        for (int c = share; c < share + S::SHARE; c += 16)
+            write_16(rows + last % S::BUFS * BN, rows + S::BUFS * BN, n > 0, last > 0, splits > 1 ? reinterpret_cast<float*>(smem) : nullptr, row0, c, tok0, live, o);
     }
     if (splits > 1) {
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        const float* sums = reinterpret_cast<const float*>(smem);
-        for (int i = rank * W4T_THREADS + threadIdx.x; i < live * 128; i += splits * W4T_THREADS) {
-            const int tok = i / 128, r = i % 128;
-            const uint32_t here = smem_u32(sums + tok * W4T_PITCH + r);
-            float v = 0.f;
+        for (int i = rank * W4T_THREADS + threadIdx.x; i < live * 32; i += splits * W4T_THREADS) {
+            const int tok = i / 32, r = i % 32 * 4;
+            const uint32_t here = smem_u32(smem) + (tok * W4T_PITCH + r) * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
             for (int c = 0; c < splits; ++c) {
                 uint32_t there;
-                float f;
+                float4 f;
                 asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(c));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there) : "memory");
-                v += f;
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(there));
+                v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
             }
-            if (!abort_flag) w4_write(o, tok0 + tok, row0 + r, v);
+            if (!abort_flag) w4_write4(o, tok0 + tok, row0 + r, v);
         }
         // a CTA's shared memory stays until its peers have read it
         __syncwarp();
@@ -262,7 +335,7 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
     __syncthreads();
     if (warp == 1) {
         tcgen05_fence_after();
-        tcgen05_dealloc(tmem, BN);
+        tcgen05_dealloc(tmem, S::TMEM);
     }
     if (threadIdx.x == 0 && abort_flag && status) atomicExch(status, 13);
 }
@@ -296,23 +369,23 @@ int rf_gemm_w4_tc(const void* x, long long ldx, const void* packed, const void* 
     if (x_blocks > 0x7fffffffll || y > 65535) return RF_ERR_UNSUPPORTED;
     CUtensorMap map;
     if (const int e = make_map(&map, x, M, K, ldx, bn)) return e;
-    const W4Out o{out, bias, bias_is_f32, out_is_f32, add, M, N};
+    const W4Out o = w4_out(out, bias, bias_is_f32, out_is_f32, add, M, N);
     int bad = 0;
     const bool known = with_tc(bn, G, [&](auto b, auto g) {
         constexpr int BN = decltype(b)::value, GC = decltype(g)::value;
         static PerDevice<bool> set;
         bool& done = set.here();
         if (!done) {
-            const cudaError_t e = cudaFuncSetAttribute(w4_tc_kernel<BN, GC>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<BN>::BYTES);
+            const cudaError_t e = cudaFuncSetAttribute(w4_tc_kernel<BN, GC>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<BN, GC>::BYTES);
             if (e != cudaSuccess) { bad = (int)e; return; }
             done = true;
         }
         const dim3 grid((unsigned)x_blocks, (unsigned)y), block(W4T_THREADS);
         auto go = [&](auto... args) {
-            if (splits > 1) rf_launch_cluster(w4_tc_kernel<BN, GC>, grid, block, TcShape<BN>::BYTES, st, splits, args...);
-            else rf_launch(w4_tc_kernel<BN, GC>, grid, block, TcShape<BN>::BYTES, st, args...);
+            if (splits > 1) rf_launch_cluster(w4_tc_kernel<BN, GC>, grid, block, TcShape<BN, GC>::BYTES, st, splits, args...);
+            else rf_launch(w4_tc_kernel<BN, GC>, grid, block, TcShape<BN, GC>::BYTES, st, args...);
         };
-        go(map, (const uint4*)packed, (const uint32_t*)scales, blocks, splits, status, o);
+        go(map, (const uint4*)packed, (const uint32_t*)scales, blocks, splits, out_is_f32 != 0, status, o);
     });
     if (!known) return RF_ERR_BAD_ARG;
     if (bad) return bad;

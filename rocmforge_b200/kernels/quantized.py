@@ -310,9 +310,15 @@ def swiglu_q8(gu: torch.Tensor, group: int = 128, activation: str = "silu") -> Q
 # tokens: 67 against 52).
 W4_FEW_TOKENS = 64
 # 16-bit rows: from so many tokens on the tensor cores' kernel (16 x 37,888 x 3,584: rf_gemm_w4 23.8 us, rf_gemm_w4_tc 31.4; 32: 57.4, 31.7), up to
-# so many (512 x 37,888 x 3,584: 146 us, 163 by the weights written out in 16 bits; 512 x 3,584 x 18,944: 70, 130; 1,024: 290, 252 and 125, 155).
+# so many (512 x 37,888 x 3,584: 142 us, 165 by the weights written out in 16 bits; 512 x 3,584 x 18,944: 70, 125; 1,024: 314, 253 and 123, 136).
 W4_TC_TOKENS = 17
 W4_TC_MOST = 512
+# 32-bit results of rows longer than SUM_COLUMNS: up to so many, since that other way takes a pass over the result for every such piece (2,048 x
+# 3,584 x 18,944: 297 us against 332; 4,096: 626, 578)
+W4_TC_MOST_F32 = 2048
+# Columns that one tensor-core sum runs over where the result is 32-bit: its additions are cut, not rounded, and what is cut adds up
+# (1,999 x 3,584 x 18,944 against 64 bits: one sum 1.1e-5, pieces of 6,315 2.6e-6, of 2,048 5e-7)
+SUM_COLUMNS = 2048
 
 
 @functools.lru_cache(None)
@@ -353,22 +359,18 @@ def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
     return best[1:]
 
 
-# Columns that one tensor-core sum runs over where the result is 32-bit: its additions are cut, not rounded, and what is cut adds up
-# (1,999 x 3,584 x 18,944 against 64 bits: one sum 1.1e-5)
-SUM_COLUMNS = 8192
 # What a block of rf_gemm_w4_tc takes, by the tokens of its tile: us for 128 columns, us beside them (within 15 % of what 55 products of 8 to
 # 2,048 tokens measured).
 W4_TC_COST = {32: (0.37, 4.5), 64: (0.42, 6.0), 128: (0.62, 8.0), 256: (0.86, 12.0)}
 
 
 @functools.lru_cache(4096)
-def w4_tc_launch(M: int, N: int, K: int, group: int, f32: bool, clusters_of):
-    """(tokens of a tile, splits): how ``rf_gemm_w4_tc`` shares out a product of 16-bit rows, chosen from sizes alone.  One sum runs over at
-    most SUM_COLUMNS columns where the result is 32-bit, as far as eight splits go."""
+def w4_tc_launch(M: int, N: int, K: int, group: int, clusters_of):
+    """(tokens of a tile, splits): how ``rf_gemm_w4_tc`` shares out a product of 16-bit rows, chosen from sizes alone."""
     units, rows, best = (padded_columns(K, group) + 127) // 128, (N + 127) // 128, None
     for bn, (unit, beside) in W4_TC_COST.items():
         tiles = rows * ((M + bn - 1) // bn)
-        for splits in range(min(8, (K + SUM_COLUMNS - 1) // SUM_COLUMNS) if f32 else 1, 9):
+        for splits in range(1, 9):
             rounds = (tiles + clusters_of(splits) - 1) // clusters_of(splits)
             cost = rounds * ((units + splits - 1) // splits * unit + beside) + 0.5 * (splits > 1)
             if best is None or cost < best[0]:
@@ -424,11 +426,11 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
         return out
     on = _clusters_on(here)
     tiled = not q8 and M >= W4_TC_TOKENS and code != 0 and ld % 8 == 0 and at % 16 == 0
-    if not q8 and (code == 0 or M > (W4_TC_MOST if tiled else W4_FEW_TOKENS)):
+    if not q8 and (code == 0 or M > (W4_FEW_TOKENS if not tiled else W4_TC_MOST_F32 if f32 and K > SUM_COLUMNS else W4_TC_MOST)):
         return _gemm_through_16_bits(x, w, bias, out, accumulate)
     if tiled:
         done = _f("rf_gemm_w4_tc")(at, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
-                                   *w4_tc_launch(M, N, K, w.group, f32, on), M, N, K, w.group, tc.status_word(w.packed.device).data_ptr(), stream())
+                                   *w4_tc_launch(M, N, K, w.group, on), M, N, K, w.group, tc.status_word(w.packed.device).data_ptr(), stream())
     else:
         done = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales_at if q8 else None, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
                                 *w4_launch(q8, M, N, K, w.group, on), M, N, K, w.group, stream())

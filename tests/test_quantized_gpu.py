@@ -204,7 +204,7 @@ def test_every_way_to_share_out_a_product(monkeypatch, M, eights, pair, ways, cl
 
 @pytest.mark.parametrize("M,bn", [(1, 32), (32, 32), (40, 32), (64, 64), (33, 64), (129, 64), (128, 128), (100, 128), (300, 128), (256, 256), (129, 256), (300, 256)])
 @pytest.mark.parametrize("splits", [1, 2, 3, 8])
-@pytest.mark.parametrize("N,K,G", [(300, 1088, 32), (130, 200, 64), (17, 2176, 128), (450, 72, 128), (128, 3328, 32)])
+@pytest.mark.parametrize("N,K,G", [(300, 1088, 32), (130, 200, 64), (17, 2176, 128), (450, 72, 128), (128, 3328, 32), (20, 8200, 128)])
 def test_every_tile_on_the_tensor_cores(monkeypatch, M, bn, splits, N, K, G):
     """Tiles of tokens that are not full, rows of weights that end inside a tile, shares of the columns that are empty."""
     from rocmforge_b200 import kernels
