@@ -304,17 +304,18 @@ __device__ __forceinline__ void quarter(int (&d)[4], const int* c, uint32_t lo_r
     const uint32_t m = 0xf0f0f0f0u;                      // a half of a byte at its upper end is 16 q as a signed byte
     mma_s8(d, c, lo_row << 4 & m, hi_row << 4 & m, lo_row & m, hi_row & m, x.x, x.y);
 }
-// Two halves of bytes, 16 bits apart, as bfloat16 numbers: 128 + (q + 8) in the bits of 128, less 136; both steps are exact.
-__device__ __forceinline__ uint32_t two_weights(uint32_t w) {
-    uint32_t v = (w & 0x000f000fu) ^ 0x43084308u;
+// Two bytes q + 8 below 0x43 each are 128 + q + 8, less 136; exact.
+__device__ __forceinline__ uint32_t two_weights(uint32_t bytes, uint32_t which) {
+    uint32_t v = __byte_perm(bytes, 0x43434343u, which);
     const __nv_bfloat162 less = __float2bfloat162_rn(-136.f);
     __nv_bfloat162 r = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&v), less);
     return *reinterpret_cast<uint32_t*>(&r);
 }
 __device__ __forceinline__ void quarter(float (&d)[4], const float* c, uint32_t lo_row, uint32_t hi_row, const uint4& x) {
-    const uint32_t lo = __byte_perm(lo_row, 0, 0x3120), hi = __byte_perm(hi_row, 0, 0x3120);       // neighbouring columns 16 bits apart
-    mma_bf16(d, c, two_weights(lo), two_weights(hi), two_weights(lo >> 8), two_weights(hi >> 8), x.x, x.y);
-    mma_bf16(d, d, two_weights(lo >> 4), two_weights(hi >> 4), two_weights(lo >> 12), two_weights(hi >> 12), x.z, x.w);
+    const uint32_t m = 0x0f0f0f0fu, eight = 0x08080808u;
+    const uint32_t l0 = (lo_row & m) ^ eight, h0 = (hi_row & m) ^ eight, l1 = (lo_row >> 4 & m) ^ eight, h1 = (hi_row >> 4 & m) ^ eight;
+    mma_bf16(d, c, two_weights(l0, 0x4140), two_weights(h0, 0x4140), two_weights(l0, 0x4342), two_weights(h0, 0x4342), x.x, x.y);
+    mma_bf16(d, d, two_weights(l1, 0x4140), two_weights(h1, 0x4140), two_weights(l1, 0x4342), two_weights(h1, 0x4342), x.z, x.w);
 }
 __device__ __forceinline__ unsigned long long two(float a, float b) {
     unsigned long long r;

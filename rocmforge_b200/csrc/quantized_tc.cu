@@ -1,83 +1,107 @@
 // Products of bfloat16 rows with 4-bit weights on the 5th-generation tensor cores, from 17 tokens on.
 //
-// Weights are the accumulator's rows, tokens its columns.  128 rows of weights go through shared memory a stage at a time: eight warps have a
-// tile of 16 rows each as it is stored, in registers, asked for AHEAD stages before (and before the wait for the kernel before); they widen
-// it to bfloat16 numbers, scale and all (exactly, with scales of five significant bits; others are rounded), and write it where the MMA
-// reads it.  Two groups of eight warps do every second stage each.  The tokens' numbers come by TMA into a ring of their own.  Long rows are
-// shared out to the CTAs of a cluster, which add up their sums through shared memory in the order of their ranks.
+// Weights are the accumulator's rows, tokens its columns.  128 rows' weights come as they are stored, by TMA, four blocks of 128 columns a stage,
+// ahead and before the wait for the kernel before.  Four groups of four warps have every fourth block each: a lane reads a row's (whatever the
+// order in which the result's rows then lie), widens them to bfloat16 numbers, scale and all (exactly, with scales of five significant bits;
+// others are rounded), and writes them into tensor memory, where the MMA takes its first operand from.  (Through shared memory instead,
+// writing them there and the MMA's reading them were the limit: 64 x 37,888 x 3,584 33.7 us.)  The tokens' numbers come by TMA into a ring of
+// their own.  Long rows are shared out to the CTAs of a cluster, which add up their sums through shared memory in the order of their ranks.
 //
 // The tensor cores cut what an addition loses instead of rounding it, and what is cut adds up (1,999 x 3,584 x 18,944 against 64 bits: one sum
 // 1.1e-5 off, pieces of 6,315 columns 2.6e-6).  For 32-bit results a sum runs over W4T_PIECE columns at most: the widening warps add it to a
-// second one beside it, rounded, while the next piece goes into another accumulator (tiles of 256 tokens: into the same one, after a wait).
+// second one beside it, rounded, while the next piece goes into another accumulator (tiles of 128 tokens: into the same one, after a wait).
 //
 // Every wait on an mbarrier is bounded (2 s): status word 13.
 #include <type_traits>
 #include "quantized.cuh"
 #include "tcgen05_common.cuh"
 
-#define W4T_THREADS (32 * 18)                            // the tokens' producer, the MMA issuer, sixteen widening warps (which write the result)
+#define W4T_THREADS (32 * 20)                            // the tokens' producer, the MMA issuer, the weights' producer, one idle, sixteen widening warps
 #define W4T_PIECE 2048                                   // columns of one sum where the result is 32-bit
 #define W4T_PITCH (128 + 4)                              // of the sums that a cluster exchanges, [token][row]
 #define W4T_MOST_SHARED (226 * 1024)                     // (the abort flag has a place of its own)
 
 template <int BN, int G>
 struct TcShape {
-    static constexpr int BLOCKS = BN <= 64 ? 2 : 1;      // blocks of 64 columns a stage: what a stage costs beside its work, twice as rarely
-    static constexpr int A = BLOCKS * 128 * 128, B = BLOCKS * BN * 128;
-    static constexpr int STAGES = 4, ROWS = BN == 128 ? 8 : 4;          // places of weights, of tokens' numbers
-    static constexpr int TURN = STAGES / 2;              // a warp's stages until it is back at the same place (a group sees all phases of it)
-    static constexpr int AHEAD = BLOCKS == 2 && G == 32 ? 2 : 4;        // stages of its own that a warp has asked for (more scales leave room for fewer)
-    static constexpr int PIECE = W4T_PIECE / 64 / BLOCKS;                               // stages of a piece
-    static constexpr int BUFS = BN <= 128 ? 2 : 1, TMEM = BN == 256 ? 512 : 4 * BN;     // accumulators; with them, behind, the pieces' sum
+    static constexpr int GROUPS = 4, STORED = 8;         // of widening warps; a stage's blocks of 64 columns as they are stored
+    static constexpr int WORDS = STORED * 512, SCALES = 512 / G * 32, STAGES = 2;       // bytes of a stage, of a tile of 16 rows
+    static constexpr int PLACES = 4, ROWS = BN == 128 ? 4 : 8;          // blocks of 128 columns in tensor memory; of tokens' numbers
+    static constexpr int B = BN * 256, RINGS = ROWS * B + STAGES * 8 * (WORDS + SCALES), BYTES = 1024 + RINGS + 512;      // (alignment, barriers)
+    static constexpr int BUFS = BN == 128 ? 1 : 2, SUMS = 64 * PLACES;  // accumulators and, behind them, the pieces' sum, behind the weights
     static constexpr int SHARE = BN / 4 < 16 ? 16 : BN / 4;             // a widening warp's part of the sums: 32 rows, so many tokens
-    static_assert(PIECE % 8 == 0 && PIECE / 2 % AHEAD == 0 && AHEAD % TURN == 0, "pieces end between turns");
-    static constexpr int RINGS = STAGES * A + ROWS * B, BYTES = RINGS + 1024 + 256;     // (alignment, barriers)
-    static_assert(RINGS >= BN * W4T_PITCH * 4, "the rings' place holds the sums");
-    static_assert(BYTES <= W4T_MOST_SHARED && 8 % ROWS == 0 && 8 % STAGES == 0, "eight stages on, every ring is back where it was (one of eight with the parity turned)");
+    static constexpr int PIECE = W4T_PIECE / 128, PIECE_STAGES = PIECE / GROUPS;
+    static_assert(BYTES <= W4T_MOST_SHARED && RINGS >= BN * W4T_PITCH * 4, "the rings' place holds the sums");
+    static_assert(SUMS + (BUFS + 1) * BN <= 512 && PIECE % ROWS == 0, "");
+    static_assert(PLACES % GROUPS == 0 && ROWS % GROUPS == 0, "one parity bit tells two phases apart, not three");
 };
 
-// Bounded wait as mbar_wait, asleep between looks: what waits here waits long, and the widening warps need the issue slots.
+// Bounded wait as mbar_wait, asleep between looks: what waits here waits long, and the widening warps need the issue slots.  (The clock is
+// not read before the first sleep has ended without what it was for.)
+__device__ __forceinline__ bool look_asleep(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
+    return ok;
+}
 __device__ __noinline__ bool wait_asleep(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     const unsigned long long t0 = global_ns();
-    for (;;) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
-        if (ok) return true;
+    while (!look_asleep(bar, parity)) {
         if (*abort_flag) return false;
         if (global_ns() - t0 > TC_WAIT_LIMIT_NS) { *abort_flag = 1; return false; }
     }
+    return true;
 }
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    return mbar_try_wait(bar, parity) || wait_asleep(bar, parity, abort_flag);
+    return look_asleep(bar, parity) || wait_asleep(bar, parity, abort_flag);
+}
+// After a wait that gave up: until the last `places` of `asked` copies have landed (a limited wait), so that none comes after the block's end.
+__device__ __noinline__ void let_land(uint32_t full, int places, int asked) {
+    int never = 0;
+    for (int i = asked > places ? asked - places : 0; i < asked; ++i) wait_asleep(full + 8 * (i % places), i / places & 1, &never);
 }
 
-// Two halves of bytes, 16 bits apart, as bfloat16 numbers times a scale.
-__device__ __forceinline__ uint32_t widened(uint32_t w, __nv_bfloat162 s) {
-    uint32_t v = (w & 0x000f000fu) ^ 0x43084308u;        // 128 + (q + 8)
-    const __nv_bfloat162 r = __hmul2(__hadd2(*reinterpret_cast<__nv_bfloat162*>(&v), __float2bfloat162_rn(-136.f)), s);
-    return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
-// A word's eight columns into 16 bytes of shared memory; with the middle bytes swapped, neighbours are 16 bits apart.
-__device__ __forceinline__ void four_pairs(uint32_t at, uint32_t word, uint32_t scale_twice) {
-    const uint32_t w = __byte_perm(word, 0, 0x3120);
-    const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&scale_twice);
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
-                 ::"r"(at), "r"(widened(w, s)), "r"(widened(w >> 8, s)), "r"(widened(w >> 4, s)), "r"(widened(w >> 12, s)) : "memory");
+__device__ __forceinline__ uint2 shared8(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
 }
+__device__ __forceinline__ uint32_t shared2(uint32_t at) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+    return v;
+}
+
+// Eight columns, a word's, as bfloat16 numbers times a scale: bytes q + 8 below 0x43 are 128 + q + 8, less 136.
+__device__ __forceinline__ void widen(uint32_t* out, uint32_t w, __nv_bfloat162 s) {
+    const uint32_t low = (w & 0x0f0f0f0fu) ^ 0x08080808u, high = (w >> 4 & 0x0f0f0f0fu) ^ 0x08080808u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t v = __byte_perm(j & 2 ? high : low, 0x43434343u, j & 1 ? 0x4342 : 0x4140);
+        const __nv_bfloat162 r = __hmul2(__hadd2(*reinterpret_cast<__nv_bfloat162*>(&v), __float2bfloat162_rn(-136.f)), s);
+        out[j] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+}
+
+// The row of the block that a lane of a warp has (accumulators' rows 32 (warp & 3) + lane).
+__device__ __forceinline__ int row_of(int warp, int lane) { return 32 * (warp & 3) + 8 * (lane & 3) + (lane >> 2); }
 
 // A widening warp's share of a piece's sum added to the sum of those before.
 template <int BN, int G>
 __device__ __noinline__ bool add_piece(uint32_t tmem, uint32_t sum_full, int piece, volatile int* abort_flag) {
     using S = TcShape<BN, G>;
-    const int buf = piece % S::BUFS, warp = threadIdx.x >> 5, share = (warp - 2) / 4 * S::SHARE;
+    const int buf = piece % S::BUFS, warp = threadIdx.x >> 5, share = (warp - 4) / 4 * S::SHARE;
     if (!__all_sync(0xffffffffu, wait_for(sum_full + 8 * buf, piece / S::BUFS & 1, abort_flag))) return false;
     tcgen05_fence_after();
     if (share < BN) {
-        const uint32_t rows = tmem + ((uint32_t)((warp & 3) * 32) << 16) + share;
+        const uint32_t rows = tmem + ((uint32_t)((warp & 3) * 32) << 16) + S::SUMS + share;
 #pragma unroll 1
         for (int c = 0; c < S::SHARE; c += 16) {
             uint32_t a[16], b[16];
@@ -98,18 +122,17 @@ __device__ __noinline__ bool add_piece(uint32_t tmem, uint32_t sum_full, int pie
     return true;
 }
 
-// 32 rows of sixteen tokens (from c on) of the result: the last piece's sum and that of those before, into `sums` ([token][row]) or, without,
-// straight out.  (Functions of their own keep these parts' registers out of the loop over the weights: written there, 64 x 37,888 x 3,584 took
-// 51 us, not 36.)
+// A lane's row of sixteen tokens (from c on) of the result: the last piece's sum and that of those before, into `sums` ([token][row]) or, without,
+// straight out.  (Functions of their own keep these parts' registers out of the loop over the weights.)
 __device__ __noinline__ void write_16(uint32_t last_sum, uint32_t sum_before, bool any, bool more, float* sums, int row0, int c, int tok0, int live, W4Out o) {
     uint32_t r[16], before[16];
-    float old[16];
     if (any) tcgen05_ld16(last_sum + c, r);
     if (more) tcgen05_ld16(sum_before + c, before);
-    const int at_row = 32 * (threadIdx.x >> 5 & 3) + (threadIdx.x & 31), row = row0 + at_row;
+    const int at_row = row_of(threadIdx.x >> 5, threadIdx.x & 31), row = row0 + at_row;
     const bool there = row < o.N;
     const size_t to = (size_t)(tok0 + c) * o.N + row;
     const float bias = there && o.bias != nullptr ? load_vec(o.bias, o.bias_is_f32, row) : 0.f;
+    float old[16];
     if (sums == nullptr && o.add) {                      // (all at once: a load after every store would wait for it)
 #pragma unroll
         for (int j = 0; j < 16; ++j) old[j] = there && c + j < live ? reinterpret_cast<const float*>(o.out)[to + (size_t)j * o.N] : 0.f;
@@ -128,194 +151,184 @@ __device__ __noinline__ void write_16(uint32_t last_sum, uint32_t sum_before, bo
 }
 
 template <int BN, int G>
-__global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const uint4* __restrict__ w0, const uint32_t* __restrict__ w1,
-                                                               int blocks, int splits, bool pieces, int* status, W4Out o) {
+__global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                                                               const __grid_constant__ CUtensorMap map_s, int blocks, int splits, bool pieces, int* status, W4Out o) {
     using S = TcShape<BN, G>;
-    constexpr int SCALES = S::BLOCKS * 64 > G ? S::BLOCKS * 64 / G : 1;                 // groups that a stage touches
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::RINGS);                      // weights' places full, empty, tokens' full, empty, sums full, added
-    constexpr int FULL = 0, EMPTY = S::STAGES, ROWS_FULL = 2 * S::STAGES, ROWS_EMPTY = ROWS_FULL + S::ROWS, SUMS = ROWS_EMPTY + S::ROWS, ADDED = SUMS + S::BUFS;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + ADDED + S::BUFS);
+    const uint32_t rows_at = smem_u32(smem), weights_at = rows_at + S::ROWS * S::B, scales_at = weights_at + S::STAGES * 8 * S::WORDS, bars = rows_at + S::RINGS;
+    // stages of weights full, empty; blocks in tensor memory full, tokens' numbers full, a block's products done; sums full, read; every product done
+    constexpr int W_FULL = 0, W_EMPTY = W_FULL + 8 * S::STAGES, A_FULL = W_EMPTY + 8 * S::STAGES, X_FULL = A_FULL + 8 * S::PLACES;
+    constexpr int DONE = X_FULL + 8 * S::ROWS, S_FULL = DONE + 8 * S::ROWS, S_READ = S_FULL + 8 * S::BUFS, END = S_READ + 8 * S::BUFS;
+    static_assert(END + 8 <= 512, "room for the barriers");
+    __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x % splits, row0 = blockIdx.x / splits * 128, tok0 = blockIdx.y * BN, live = min(BN, o.M - tok0);
-    const int all = (blocks + S::BLOCKS - 1) / S::BLOCKS, from = (int)((long long)all * rank / splits);
-    const int n = (int)((long long)all * (rank + 1) / splits) - from;
-    const int tiles = (o.N + 15) / 16, all_groups = blocks * 64 / G;
+    // stages of four blocks, the last one of a row with what is left
+    const int all = (blocks + S::STORED - 1) / S::STORED, from = (int)((long long)all * rank / splits), n = (int)((long long)all * (rank + 1) / splits) - from;
+    const int nb = n > 0 ? (min(S::STORED * n, blocks - S::STORED * from) + 1) / 2 : 0;
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int i = 0; i < S::STAGES; ++i) {
-            mbar_init(smem_u32(&bars[FULL + i]), 8);     // eight widening warps
-            mbar_init(smem_u32(&bars[EMPTY + i]), 1);
-        }
-        for (int i = 0; i < 2 * S::ROWS + S::BUFS; ++i) mbar_init(smem_u32(&bars[ROWS_FULL + i]), 1);
-        for (int i = 0; i < S::BUFS; ++i) mbar_init(smem_u32(&bars[ADDED + i]), 16);
+        for (int i = 0; i < S::PLACES; ++i) mbar_init(bars + A_FULL + 8 * i, 4);
+        for (int i = 0; i < S::ROWS; ++i) mbar_init(bars + X_FULL + 8 * i, 1), mbar_init(bars + DONE + 8 * i, 1);
+        for (int i = 0; i < S::BUFS; ++i) mbar_init(bars + S_FULL + 8 * i, 1), mbar_init(bars + S_READ + 8 * i, 16);
+        mbar_init(bars + END, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
     }
-    if (warp == 1) {
-        tcgen05_alloc(smem_u32(tmem_slot), S::TMEM);
+    auto ask_weights = [&](int i) {
+        const int at = i % S::STAGES;
+        mbar_expect_tx(bars + W_FULL + 8 * at, 8 * (S::WORDS + S::SCALES));
+        tma_load_3d(weights_at + at * 8 * S::WORDS, &map_w, 0, (from + i) * S::STORED * 4, row0 / 16, bars + W_FULL + 8 * at);
+        tma_load_2d(scales_at + at * 8 * S::SCALES, &map_s, (from + i) * (S::SCALES / 2), row0 / 16, bars + W_FULL + 8 * at);
+    };
+    if (warp == 2 && lane == 0) {                        // (the first before anything else)
+        for (int i = 0; i < S::STAGES; ++i) mbar_init(bars + W_FULL + 8 * i, 1), mbar_init(bars + W_EMPTY + 8 * i, 16);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int i = 0; i < min(n, S::STAGES); ++i) ask_weights(i);
+    }
+    if (warp == 3) {
+        tcgen05_alloc(smem_u32(&tmem_slot), 512);
         tcgen05_relinquish();
     }
-    // the widening warps' weights: stages phase, phase + 2, ... of a tile of 16 rows, AHEAD of them in registers before anything is waited for
-    const int wide = warp - 2, tile = min(row0 / 16 + (wide & 7), tiles - 1), phase = wide >> 3;        // (rows that are not there: some others)
-    const int block0 = (from + phase) * S::BLOCKS, stages = wide >= 0 ? (n - phase + 1) / 2 : 0;
-    const uint4* next_w = w0 + ((size_t)tile * blocks + block0) * 32 + lane;
-    const uint32_t* next_s = w1 + ((size_t)tile * all_groups + block0 * 64 / G) * 8 + (lane >> 2);
-    uint4 w[S::AHEAD][S::BLOCKS];
-    uint32_t sc[S::AHEAD][SCALES];
-    int asked = 0;
-    auto ask = [&](int into) {
-        if (asked < stages) {
-            // (the last stage's second block may not be there)
-            const bool second = S::BLOCKS == 2 && (asked + 1 < stages || block0 + 2 * S::BLOCKS * (stages - 1) + 1 < blocks);
-            w[into][0] = next_w[0];
-            if constexpr (S::BLOCKS == 2) w[into][1] = second ? next_w[32] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-            for (int p = 0; p < SCALES; ++p) sc[into][p] = S::BLOCKS == 1 || second || p * G < 64 ? next_s[8 * p] : 0u;
-            next_w += 2 * S::BLOCKS * 32;                // (two stages on are whole groups on)
-            next_s += 2 * S::BLOCKS * 64 / G * 8;
-            ++asked;
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < S::AHEAD; ++i) ask(i);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = *tmem_slot;
-
-    const int last = pieces && n > 0 ? (n - 1) / S::PIECE : 0;           // the piece that the result is read from, together with the sum of those before
-    const uint32_t sum_full = smem_u32(&bars[SUMS]), added = smem_u32(&bars[ADDED]);
+    const uint32_t tmem = tmem_slot;
+    const int last = pieces && nb > 0 ? (nb - 1) / S::PIECE : 0;         // the piece that the result is read from, with the sum of those before
     bool ok = true;
     if (warp == 0) {
         // ---------------- the tokens' numbers
         if (lane == 0) {
             pdl_wait();
-            const uint32_t full = smem_u32(&bars[ROWS_FULL]), empty = smem_u32(&bars[ROWS_EMPTY]), to = smem_u32(smem) + S::STAGES * S::A;
-            for (int i = 0; i < n && ok; i += 8) {
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    if (i + u >= n) break;
-                    const int at = u % S::ROWS;
-                    if (i > 0 || u >= S::ROWS) ok = wait_for(empty + 8 * at, ((S::ROWS == 8 ? i / 8 : u / S::ROWS) & 1) ^ 1, &abort_flag);
-                    if (!ok) break;
-                    mbar_expect_tx(full + 8 * at, S::B);
-#pragma unroll
-                    for (int b = 0; b < S::BLOCKS; ++b)
-                        tma_load_2d(to + at * S::B + b * BN * 128, &map_x, ((from + i + u) * S::BLOCKS + b) * 64, tok0, full + 8 * at);
-                }
+            int i = 0;
+            for (; i < nb; ++i) {
+                const int at = i % S::ROWS, column = (from * S::GROUPS + i) * 128;
+                if (i >= S::ROWS && !wait_for(bars + DONE + 8 * at, (i / S::ROWS & 1) ^ 1, &abort_flag)) break;
+                mbar_expect_tx(bars + X_FULL + 8 * at, S::B);
+                tma_load_2d(rows_at + at * S::B, &map_x, column, tok0, bars + X_FULL + 8 * at);
+                tma_load_2d(rows_at + at * S::B + S::B / 2, &map_x, column + 64, tok0, bars + X_FULL + 8 * at);
             }
+            if (i < nb) let_land(bars + X_FULL, S::ROWS, i);
+        }
+    } else if (warp == 2) {
+        // ---------------- the weights (sixteen bulk copies a stage, a tile's weights and scales each, took 1,800 cycles to issue)
+        if (lane == 0) {
+            int i = min(n, S::STAGES);
+            for (; i < n; ++i) {
+                if (!wait_for(bars + W_EMPTY + 8 * (i % S::STAGES), (i / S::STAGES & 1) ^ 1, &abort_flag)) break;
+                ask_weights(i);
+            }
+            if (i < n) let_land(bars + W_FULL, S::STAGES, i);
         }
     } else if (warp == 1) {
         // ---------------- the products
-        // Eight stages a turn, after which every ring is back where it was: places, parities and descriptors are constants.  (With remainders and
-        // addresses formed anew this one thread, not the tensor cores, was the limit.)
+        // ROWS blocks a turn, after which every ring is back where it was: places and descriptors are constants.
         if (elect_one()) {
-            const uint32_t full = smem_u32(&bars[FULL]), empty = smem_u32(&bars[EMPTY]), rows_full = smem_u32(&bars[ROWS_FULL]), rows_empty = smem_u32(&bars[ROWS_EMPTY]);
-            const uint64_t da0 = make_smem_desc(smem_u32(smem)), db0 = make_smem_desc(smem_u32(smem) + S::STAGES * S::A);
-            uint32_t sum = tmem;
+            const uint64_t db0 = make_smem_desc(rows_at);
+            uint32_t sum = tmem + S::SUMS;
             bool starts = true;
-            for (int i = 0; i < n && ok; i += 8, starts = false) {
+            for (int i = 0; i < nb && ok; i += S::ROWS, starts = false) {
                 if (pieces && i > 0 && i % S::PIECE == 0) {
                     const int piece = i / S::PIECE, buf = piece % S::BUFS;
-                    tcgen05_commit(sum_full + 8 * ((piece - 1) % S::BUFS));
-                    if (piece >= S::BUFS) ok = wait_for(added + 8 * buf, piece / S::BUFS - 1 & 1, &abort_flag);
+                    tcgen05_commit(bars + S_FULL + 8 * ((piece - 1) % S::BUFS));
+                    if (piece >= S::BUFS) ok = wait_for(bars + S_READ + 8 * buf, piece / S::BUFS - 1 & 1, &abort_flag);
                     if (!ok) break;
                     tcgen05_fence_after();
-                    sum = tmem + buf * BN;
+                    sum = tmem + S::SUMS + buf * BN;
                     starts = true;
                 }
+                const uint32_t turn = i / S::ROWS & 1;
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    if (i + u >= n) break;
-                    const int a = u % S::STAGES, r = u % S::ROWS;
-                    ok = wait_for(rows_full + 8 * r, (S::ROWS == 8 ? i / 8 : u / S::ROWS) & 1, &abort_flag) && wait_for(full + 8 * a, u / S::STAGES & 1, &abort_flag);
+                for (int u = 0; u < S::ROWS; ++u) {
+                    if (i + u >= nb) break;
+                    const int a = u % S::PLACES;
+                    ok = wait_for(bars + X_FULL + 8 * u, turn, &abort_flag) && wait_for(bars + A_FULL + 8 * a, S::ROWS == S::PLACES ? turn : u / S::PLACES & 1, &abort_flag);
                     if (!ok) break;
                     tcgen05_fence_after();
 #pragma unroll
-                    for (int k = 0; k < 4 * S::BLOCKS; ++k) {           // 16 columns
-                        const uint64_t da = da0 + (a * S::A + k / 4 * 128 * 128) / 16 + 2 * (k % 4), db = db0 + (r * S::B + k / 4 * BN * 128) / 16 + 2 * (k % 4);
-                        tcgen05_mma_bf16(sum, da, db, make_idesc(BN), u || k || !starts ? 1u : 0u);
-                    }
-                    tcgen05_commit(empty + 8 * a);
-                    tcgen05_commit(rows_empty + 8 * r);
+                    for (int k = 0; k < 8; ++k)          // 16 columns
+                        tcgen05_mma_bf16_ts(sum, tmem + a * 64 + k * 8, db0 + (u * S::B + k / 4 * (S::B / 2)) / 16 + 2 * (k % 4), make_idesc(BN), u || k || !starts ? 1u : 0u);
+                    tcgen05_commit(bars + DONE + 8 * u);
                 }
             }
-            tcgen05_commit(sum_full + 8 * (last % S::BUFS));
+            tcgen05_commit(bars + END);
+            if (!ok) let_land(bars + END, 1, 1);
         }
-    } else {
-        // ---------------- the weights
-        const int g = lane >> 2, t = lane & 3;
-        const bool odd = g & 1;
-        // where this lane's 16 bytes of a row's half go (rows of 128 bytes, pieces swapped by row % 8 = g): by the row's parity the other half
-        // first, so that two rows' pieces meet all banks
-        uint32_t place[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) place[j] = smem_u32(smem) + phase * S::A + (16 * (wide & 7) + g) * 128 + (((4 * (odd ^ j) + t) ^ g) * 16);
-        const uint32_t full = smem_u32(&bars[FULL + phase]), empty = smem_u32(&bars[EMPTY + phase]);
+    } else if (warp >= 4) {
+        // ---------------- the weights into tensor memory: a group of warps has every fourth block, a warp 32 rows, a lane one
+        const int group = (warp - 4) / 4, g = lane >> 2, t = lane & 3, tile = 2 * (warp & 3) + (t >> 1);
+        const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + group * 64;
+        // entry 4 g + p of a stored block: rows of 128 bytes, two g each, their pieces of 16 swapped by row % 8
+        const uint32_t words_at = weights_at + tile * S::WORDS + group * 1024 + g / 2 * 128 + 8 * (t & 1), piece0 = ((g & 1) * 4 ^ g / 2) * 16;
+        const uint32_t scale_at = scales_at + tile * S::SCALES + group * 128 / G * 32 + 4 * g + 2 * (t & 1);
         int summed = 0;
-        uint32_t parity = 1;
-        for (int done = 0; done < stages && ok;) {
-#pragma unroll
-            for (int u = 0; u < S::AHEAD; ++u, ++done) {
-                if (done >= stages) break;
-                const int at = u % S::TURN * 2;
-                // (a piece is added once the next one's first stages are on their way)
-                if (u == S::TURN % S::AHEAD && (done - S::TURN) / (S::PIECE / 2) > summed && summed < last) {
-                    ok = add_piece<BN, G>(tmem, smem_u32(&bars[SUMS]), summed, &abort_flag);
-                    if (!ok) break;
-                    ++summed;
-                }
-                if (done >= S::TURN) {
-                    ok = wait_for(empty + 8 * at, parity, &abort_flag);
-                    if (!ok) break;
-                }
-#pragma unroll
-                for (int b = 0; b < S::BLOCKS; ++b) {
-                    const uint4 v = w[u][b];
-                    const uint32_t lo[2] = {odd ? v.y : v.x, odd ? v.x : v.y}, hi[2] = {odd ? v.w : v.z, odd ? v.z : v.w};
-                    const uint32_t to = at * S::A + b * 128 * 128;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint32_t s2 = G == 32 ? (odd ^ j ? sc[u][2 * b + 1] : sc[u][2 * b]) : sc[u][G == 64 ? b : 0];
-                        four_pairs(place[j] + to, lo[j], __byte_perm(s2, 0, 0x1010));
-                        four_pairs(place[j] + to + 8 * 128, hi[j], __byte_perm(s2, 0, 0x3232));
-                    }
-                }
-                ask(u);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) at_arrive(full + 8 * at);
-                if (u % S::TURN == S::TURN - 1) parity ^= 1;
+        for (int i = 0; i < n && ok; ++i) {
+            if ((i - 1) / S::PIECE_STAGES > summed && summed < last) {  // (a piece is added once the next one's first stage is on its way)
+                ok = add_piece<BN, G>(tmem, bars + S_FULL, summed, &abort_flag);
+                if (!ok) break;
+                ++summed;
             }
+            const int at = i % S::STAGES, number = i * S::GROUPS + group;
+            ok = __all_sync(0xffffffffu, wait_for(bars + W_FULL + 8 * at, i / S::STAGES & 1, &abort_flag));
+            if (!ok || number >= nb) break;
+            const uint32_t here = words_at + at * 8 * S::WORDS;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {                // stored blocks (rows and columns that are not there: zeros)
+                uint32_t out[32];
+                const uint32_t its = scale_at + at * 8 * S::SCALES + 64 * h / G * 32;
+                uint32_t s0 = shared2(its), s1 = G == 32 ? shared2(its + 32) : s0;
+                s0 |= s0 << 16;
+                s1 |= s1 << 16;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const uint2 v = shared8(here + 512 * h + (piece0 ^ 64 * h ^ 16 * p));
+                    widen(out + 4 * p, v.x, *reinterpret_cast<const __nv_bfloat162*>(&s0));
+                    widen(out + 16 + 4 * p, v.y, *reinterpret_cast<const __nv_bfloat162*>(&s1));
+                }
+                if (h == 1) {
+                    __syncwarp();                        // all have read the stage
+                    if (lane == 0) at_arrive(bars + W_EMPTY + 8 * at);
+                } else if (i > 0) {
+                    const int before = number - S::PLACES;
+                    ok = __all_sync(0xffffffffu, wait_for(bars + DONE + before % S::ROWS * 8, before / S::ROWS & 1, &abort_flag));
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                }
+                tcgen05_st32(to + 32 * h, out);
+            }
+            if (!ok) break;
+            tcgen05_wait_st();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) at_arrive(bars + A_FULL + 8 * group);
         }
-        for (; ok && summed < last; ++summed) ok = add_piece<BN, G>(tmem, smem_u32(&bars[SUMS]), summed, &abort_flag);
+        for (; ok && summed < last; ++summed) ok = add_piece<BN, G>(tmem, bars + S_FULL, summed, &abort_flag);
     }
     pdl_wait();                                          // (whoever writes from here on has waited)
-    // ---------------- the result: a warp has the same share as of the pieces; a cluster's go through the rings' place, one CTA's straight out
-    const int share = (warp - 2) / 4 * S::SHARE;
-    const bool writes = warp >= 2 && share < BN;
-    if (writes && n > 0) {
-        ok = wait_for(sum_full + 8 * (last % S::BUFS), last / S::BUFS & 1, &abort_flag) && ok;
+    // ---------------- the result: a cluster's sums go through the rings' place, one CTA's straight out
+    const int share = (warp - 4) / 4 * S::SHARE;
+    const bool writes = warp >= 4 && share < BN;
+    if (writes && nb > 0) {
+        ok = wait_for(bars + END, 0, &abort_flag) && ok;
         tcgen05_fence_after();
     }
     ok = __all_sync(0xffffffffu, ok);
-    if (splits > 1) __syncthreads();                     // (the sums are there: every product has read the rings)
+    if (splits > 1) __syncthreads();                     // (every product is done: the rings have been read)
     if (writes && ok) {
-        const uint32_t rows = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t rows = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + S::SUMS;
 #pragma unroll 1
         for (int c = share; c < share + S::SHARE; c += 16)
-            write_16(rows + last % S::BUFS * BN, rows + S::BUFS * BN, n > 0, last > 0, splits > 1 ? reinterpret_cast<float*>(smem) : nullptr, row0, c, tok0, live, o);
+            write_16(rows + last % S::BUFS * BN, rows + S::BUFS * BN, nb > 0, last > 0, splits > 1 ? reinterpret_cast<float*>(smem) : nullptr, row0, c, tok0, live, o);
     }
     if (splits > 1) {
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         for (int i = rank * W4T_THREADS + threadIdx.x; i < live * 32; i += splits * W4T_THREADS) {
             const int tok = i / 32, r = i % 32 * 4;
-            const uint32_t here = smem_u32(smem) + (tok * W4T_PITCH + r) * 4;
+            const uint32_t here = rows_at + (tok * W4T_PITCH + r) * 4;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
             for (int c = 0; c < splits; ++c) {
@@ -333,11 +346,33 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
     }
     tcgen05_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == 3) {
         tcgen05_fence_after();
-        tcgen05_dealloc(tmem, S::TMEM);
+        tcgen05_dealloc(tmem, 512);
     }
     if (threadIdx.x == 0 && abort_flag && status) atomicExch(status, 13);
+}
+
+// ---------------------------------------------------------------- host side
+// The stored weights as rows of 128 bytes, [tiles of 16 rows][4 a block][128], pieces of 16 bytes swapped by row % 8; a box is a stage of eight
+// tiles.  Their scales as [tiles][groups of 16].
+static int weights_map(CUtensorMap* map, const void* base, long long tiles, long long blocks, int stored) {
+    EncodeTiledFn f = encode_fn();
+    if (!f) return RF_ERR_UNSUPPORTED;
+    cuuint64_t dims[3] = {128, (cuuint64_t)(4 * blocks), (cuuint64_t)tiles}, strides[2] = {128, (cuuint64_t)(512 * blocks)};
+    cuuint32_t box[3] = {128, (cuuint32_t)(4 * stored), 8}, steps[3] = {1, 1, 1};
+    const CUresult r = f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : RF_ERR_BAD_ARG;
+}
+static int scales_map(CUtensorMap* map, const void* base, long long tiles, long long groups, int groups_of_stage) {
+    EncodeTiledFn f = encode_fn();
+    if (!f) return RF_ERR_UNSUPPORTED;
+    cuuint64_t dims[2] = {(cuuint64_t)(16 * groups), (cuuint64_t)tiles}, strides[1] = {(cuuint64_t)(32 * groups)};
+    cuuint32_t box[2] = {(cuuint32_t)(16 * groups_of_stage), 8}, steps[2] = {1, 1};
+    const CUresult r = f(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : RF_ERR_BAD_ARG;
 }
 
 // f(tokens of a tile, group) as constants; false where there is no such kernel
@@ -351,7 +386,6 @@ static bool with_tc(int bn, int G, F f) {
     if (bn == 32) by_group(std::integral_constant<int, 32>());
     else if (bn == 64) by_group(std::integral_constant<int, 64>());
     else if (bn == 128) by_group(std::integral_constant<int, 128>());
-    else if (bn == 256) by_group(std::integral_constant<int, 256>());
     else return false;
     return true;
 }
@@ -359,33 +393,35 @@ static bool with_tc(int bn, int G, F f) {
 extern "C" {
 
 // out = x w^T (+ bias): x bfloat16 [M, K], rows ldx apart, whole 16 bytes on 16-byte boundaries; out as W4Out has it.  bn: tokens of a tile (32, 64,
-// 128, 256); splits: CTAs of a cluster that share out the columns (1 .. 8).
+// 128); splits: CTAs of a cluster that share out the columns (1 .. 8).
 int rf_gemm_w4_tc(const void* x, long long ldx, const void* packed, const void* scales, const void* bias, int bias_is_f32, void* out, int out_is_f32, int add,
                   int bn, int splits, int M, int N, int K, int G, int* status, cudaStream_t st) {
     if (M <= 0 || N <= 0 || K <= 0 || bad_group(G) || (add && !out_is_f32) || splits < 1 || splits > 8 || bn < 1) return RF_ERR_BAD_ARG;
-    if (!aligned(packed, 16) || !aligned(scales, 16) || ldx < K || ldx > 0x7fffffff) return RF_ERR_BAD_ARG;
+    if (!aligned(packed, 16) || !aligned(scales, 16) || ldx < K) return RF_ERR_BAD_ARG;
     const int blocks = padded(K, G) / 64;
-    const long long x_blocks = (long long)((N + 127) / 128) * splits, y = (M + (long long)bn - 1) / bn;
+    const long long tiles = ((long long)N + 15) / 16, x_blocks = (tiles + 7) / 8 * splits, y = (M + (long long)bn - 1) / bn;
     if (x_blocks > 0x7fffffffll || y > 65535) return RF_ERR_UNSUPPORTED;
-    CUtensorMap map;
-    if (const int e = make_map(&map, x, M, K, ldx, bn)) return e;
+    CUtensorMap map_x, map_w, map_s;
+    if (const int e = make_map(&map_x, x, M, K, ldx, bn)) return e;
     const W4Out o = w4_out(out, bias, bias_is_f32, out_is_f32, add, M, N);
     int bad = 0;
     const bool known = with_tc(bn, G, [&](auto b, auto g) {
         constexpr int BN = decltype(b)::value, GC = decltype(g)::value;
+        using S = TcShape<BN, GC>;
+        if ((bad = weights_map(&map_w, packed, tiles, blocks, S::STORED)) || (bad = scales_map(&map_s, scales, tiles, (long long)blocks * 64 / GC, 64 * S::STORED / GC))) return;
         static PerDevice<bool> set;
         bool& done = set.here();
         if (!done) {
-            const cudaError_t e = cudaFuncSetAttribute(w4_tc_kernel<BN, GC>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<BN, GC>::BYTES);
+            const cudaError_t e = cudaFuncSetAttribute(w4_tc_kernel<BN, GC>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
             if (e != cudaSuccess) { bad = (int)e; return; }
             done = true;
         }
         const dim3 grid((unsigned)x_blocks, (unsigned)y), block(W4T_THREADS);
         auto go = [&](auto... args) {
-            if (splits > 1) rf_launch_cluster(w4_tc_kernel<BN, GC>, grid, block, TcShape<BN, GC>::BYTES, st, splits, args...);
-            else rf_launch(w4_tc_kernel<BN, GC>, grid, block, TcShape<BN, GC>::BYTES, st, args...);
+            if (splits > 1) rf_launch_cluster(w4_tc_kernel<BN, GC>, grid, block, S::BYTES, st, splits, args...);
+            else rf_launch(w4_tc_kernel<BN, GC>, grid, block, S::BYTES, st, args...);
         };
-        go(map, (const uint4*)packed, (const uint32_t*)scales, blocks, splits, out_is_f32 != 0, status, o);
+        go(map_x, map_w, map_s, blocks, splits, out_is_f32 != 0, status, o);
     });
     if (!known) return RF_ERR_BAD_ARG;
     if (bad) return bad;

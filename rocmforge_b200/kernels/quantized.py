@@ -306,15 +306,15 @@ def swiglu_q8(gu: torch.Tensor, group: int = 128, activation: str = "silu") -> Q
     return y
 
 
-# Products of up to so many tokens take rows in 8 bits where a step may choose (64 x 37,888 x 3,584: 34.7 us against 35.6 of 16-bit rows, 128
-# tokens: 67 against 52).
-W4_FEW_TOKENS = 64
-# 16-bit rows: from so many tokens on the tensor cores' kernel (16 x 37,888 x 3,584: rf_gemm_w4 23.8 us, rf_gemm_w4_tc 31.4; 32: 57.4, 31.7), up to
-# so many (512 x 37,888 x 3,584: 142 us, 165 by the weights written out in 16 bits; 512 x 3,584 x 18,944: 70, 125; 1,024: 314, 253 and 123, 136).
+# Products of up to so many tokens take rows in 8 bits where a step may choose (32 x 37,888 x 3,584: 22.0 us against 27.8 of 16-bit rows; 64 tokens:
+# 34.7, 29.3; 64 x 3,584 x 18,944: 30.6, 19.7).
+W4_FEW_TOKENS = 32
+# 16-bit rows: from so many tokens on the tensor cores' kernel (16 x 37,888 x 3,584: rf_gemm_w4 21.3 us, rf_gemm_w4_tc 27.6; 24 tokens: 31.4, 27.7), up
+# to so many (512 x 37,888 x 3,584: 148 us, 165 by the weights written out in 16 bits; 512 x 3,584 x 18,944: 63, 124; 1,024: 317, 257 and 128, 137).
 W4_TC_TOKENS = 17
 W4_TC_MOST = 512
 # 32-bit results of rows longer than SUM_COLUMNS: up to so many, since that other way takes a pass over the result for every such piece (2,048 x
-# 3,584 x 18,944: 297 us against 332; 4,096: 626, 578)
+# 3,584 x 18,944: 288 us against 332; 4,096: 626, 578)
 W4_TC_MOST_F32 = 2048
 # Columns that one tensor-core sum runs over where the result is 32-bit: its additions are cut, not rounded, and what is cut adds up
 # (1,999 x 3,584 x 18,944 against 64 bits: one sum 1.1e-5, pieces of 6,315 2.6e-6, of 2,048 5e-7)
@@ -359,20 +359,19 @@ def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
     return best[1:]
 
 
-# What a block of rf_gemm_w4_tc takes, by the tokens of its tile: us for 128 columns, us beside them (within 15 % of what 55 products of 8 to
-# 2,048 tokens measured).
-W4_TC_COST = {32: (0.37, 4.5), 64: (0.42, 6.0), 128: (0.62, 8.0), 256: (0.86, 12.0)}
+# What a block of rf_gemm_w4_tc takes, by the tokens of its tile: us for 512 columns, us beside them.
+W4_TC_COST = {32: (1.48, 3.2), 64: (1.5, 3.8), 128: (1.5, 7.5)}
 
 
 @functools.lru_cache(4096)
 def w4_tc_launch(M: int, N: int, K: int, group: int, clusters_of):
     """(tokens of a tile, splits): how ``rf_gemm_w4_tc`` shares out a product of 16-bit rows, chosen from sizes alone."""
-    units, rows, best = (padded_columns(K, group) + 127) // 128, (N + 127) // 128, None
-    for bn, (unit, beside) in W4_TC_COST.items():
+    stages, rows, best = (padded_columns(K, group) + 511) // 512, (N + 127) // 128, None
+    for bn, (stage, beside) in W4_TC_COST.items():
         tiles = rows * ((M + bn - 1) // bn)
         for splits in range(1, 9):
             rounds = (tiles + clusters_of(splits) - 1) // clusters_of(splits)
-            cost = rounds * ((units + splits - 1) // splits * unit + beside) + 0.5 * (splits > 1)
+            cost = rounds * ((stages + splits - 1) // splits * stage + beside) + 0.5 * (splits > 1)
             if best is None or cost < best[0]:
                 best = cost, bn, splits
     return best[1:]
@@ -424,11 +423,16 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
             _elsewhere("gemm_w4", out.get_device())
     if M == 0:
         return out
+    if code == 0 and not q8:
+        return _gemm_by_16_bits(x, w, bias, out, accumulate)
     on = _clusters_on(here)
-    tiled = not q8 and M >= W4_TC_TOKENS and code != 0 and ld % 8 == 0 and at % 16 == 0
-    if not q8 and (code == 0 or M > (W4_FEW_TOKENS if not tiled else W4_TC_MOST_F32 if f32 and K > SUM_COLUMNS else W4_TC_MOST)):
-        return _gemm_through_16_bits(x, w, bias, out, accumulate)
-    if tiled:
+    if not q8 and M >= W4_TC_TOKENS:
+        if M > (W4_TC_MOST_F32 if f32 and K > SUM_COLUMNS else W4_TC_MOST) and at % 16 == 0 and ld % 8 == 0 and ld >= K and tc.supported(M, N, K, tc.STORE):
+            return _gemm_by_16_bits(x, w, bias, out, accumulate)
+        if at % 16 or ld % 8 or ld < K:                  # the kernel copies whole 16 bytes (64 x 37,888 x 3,583 by rf_gemm_w4: 100 us)
+            x, rows = torch.empty(M, (K + 7) // 8 * 8, dtype=dt, device=x.device), x
+            x[:, :K] = rows
+            at, ld = x.data_ptr(), x.stride(0)
         done = _f("rf_gemm_w4_tc")(at, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
                                    *w4_tc_launch(M, N, K, w.group, on), M, N, K, w.group, tc.status_word(w.packed.device).data_ptr(), stream())
     else:
@@ -438,17 +442,16 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
     return out
 
 
-def _gemm_through_16_bits(x, w, bias, out, accumulate):
+def _gemm_by_16_bits(x, w, bias, out, accumulate):
     """The product by the weights written out in the rows' dtype (exactly, with scales of five significant bits)."""
     from .basic import gemm_plain
-    M, K = x.shape
+    K = x.shape[1]
+    if x.dtype == torch.float32:
+        return gemm_plain(x, dequantize_w4(w, x.dtype), bias, out=out, accumulate=accumulate)
     m = tc.RESIDUAL if accumulate else tc.F32 if out.dtype == torch.float32 else tc.STORE
-    if x.dtype == torch.bfloat16 and tc.supported(M, w.N, K, m) and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0:
-        pieces = 1 if m == tc.STORE else (K + SUM_COLUMNS - 1) // SUM_COLUMNS
-        step = (K + 64 * pieces - 1) // (64 * pieces) * 64
-        for lo in range(0, K, step):
-            hi = min(K, lo + step)
-            tc.gemm_tc(x[:, lo:hi], dequantize_w4(w, x.dtype, (lo, hi)), bias if lo == 0 else None, mode=m if lo == 0 else tc.RESIDUAL, out=out)
-        return out
-    return gemm_plain(x, dequantize_w4(w, x.dtype), bias, out=out, out_f32=out.dtype == torch.float32 and x.dtype != torch.float32,
-                      accumulate=accumulate)
+    pieces = 1 if m == tc.STORE else (K + SUM_COLUMNS - 1) // SUM_COLUMNS
+    step = (K + 64 * pieces - 1) // (64 * pieces) * 64
+    for lo in range(0, K, step):
+        hi = min(K, lo + step)
+        tc.gemm_tc(x[:, lo:hi], dequantize_w4(w, x.dtype, (lo, hi)), bias if lo == 0 else None, mode=m if lo == 0 else tc.RESIDUAL, out=out)
+    return out
