@@ -59,15 +59,28 @@ __device__ __forceinline__ uint32_t to_8_bits(const float* v, float& scale) {
     return out;
 }
 
+// Where a thread of a block of 256 is that has EACH columns at a time: narrow rows share a block (`across` of them), wide ones take several.
+template <int EACH>
+struct Place {
+    int across, sub, c;                                  // (a thread without a row of its own: columns behind the last)
+    __device__ __forceinline__ Place(int Kp) {
+        const int units = Kp / EACH;
+        across = units < 256 ? 256 / units : 1;
+        sub = units < 256 ? threadIdx.x / units : 0;
+        c = units < 256 ? (sub < across ? EACH * (threadIdx.x - sub * units) : Kp) : EACH * (blockIdx.x * 256 + threadIdx.x);
+    }
+};
+
 // ---------------------------------------------------------------- rows to 8 bits
-// A lane has four columns; a block 1,024 columns of a row.
+// A lane has four columns.
 template <typename T, int G, bool VEC>
 __global__ void __launch_bounds__(256) quantize_q8_kernel(const T* x, long long ldx, int8_t* __restrict__ q, float* __restrict__ scales,
                                                           int T_, int K, int Kp) {
     pdl_trigger();
     pdl_wait(x);
-    const int c = 4 * (blockIdx.x * 256 + threadIdx.x);
-    for (int t = blockIdx.y; t < T_; t += gridDim.y) {
+    const Place<4> at(Kp);
+    for (int t0 = blockIdx.y * at.across; t0 < T_; t0 += gridDim.y * at.across) {
+        const int t = t0 + at.sub, c = t < T_ ? at.c : Kp;               // (all lanes of a group do the same)
         float v[4], s;
         load_quad<T, VEC>(x + (size_t)t * ldx, c, K, v);
         const uint32_t p = to_8_bits<G>(v, s);
@@ -78,20 +91,31 @@ __global__ void __launch_bounds__(256) quantize_q8_kernel(const T* x, long long 
     }
 }
 
-// ... and the numbers that 8-bit rows stand for.
-template <typename T>
+// ... and the numbers that 8-bit rows stand for, eight (rows of whole eights, on 16-byte boundaries) or four columns a thread.
+template <typename T, int EACH>
 __global__ void __launch_bounds__(256) dequantize_q8_kernel(const int8_t* q, const float* scales, T* __restrict__ y, int T_, int K, int Kp, int G) {
     pdl_trigger();
     pdl_wait(q, scales);
-    const int c = 4 * (blockIdx.x * 256 + threadIdx.x);
+    const Place<EACH> at(Kp);
+    const int c = at.c;
     if (c >= K) return;
-    for (int t = blockIdx.y; t < T_; t += gridDim.y) {
-        const char4 p = *reinterpret_cast<const char4*>(q + (size_t)t * Kp + c);
+    for (int t = blockIdx.y * at.across + at.sub; t < T_; t += gridDim.y * at.across) {
         const float s = scales[(size_t)t * (Kp / G) + c / G];
-        const float v[4] = {p.x * s, p.y * s, p.z * s, p.w * s};
+        T* to = y + (size_t)t * K + c;
+        if constexpr (EACH == 8) {
+            const uint2 p = *reinterpret_cast<const uint2*>(q + (size_t)t * Kp + c);
+            __align__(16) T v[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c + i < K) y[(size_t)t * K + c + i] = Cvt<T>::from_f32(v[i]);
+            for (int i = 0; i < 8; ++i) v[i] = Cvt<T>::from_f32((float)(int8_t)((i < 4 ? p.x : p.y) >> (8 * (i & 3))) * s);
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(v)[i];
+        } else {
+            const char4 p = *reinterpret_cast<const char4*>(q + (size_t)t * Kp + c);
+            const float v[4] = {p.x * s, p.y * s, p.z * s, p.w * s};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < K) to[i] = Cvt<T>::from_f32(v[i]);
+        }
     }
 }
 
@@ -101,8 +125,9 @@ template <typename T, int ACT, int G, bool VEC>
 __global__ void __launch_bounds__(256) swiglu_q8_kernel(const T* gu, int8_t* __restrict__ q, float* __restrict__ scales, int T_, int I, int Ip) {
     pdl_trigger();
     pdl_wait(gu);
-    const int c = 4 * (blockIdx.x * 256 + threadIdx.x);
-    for (int t = blockIdx.y; t < T_; t += gridDim.y) {
+    const Place<4> at(Ip);
+    for (int t0 = blockIdx.y * at.across; t0 < T_; t0 += gridDim.y * at.across) {
+        const int t = t0 + at.sub, c = t < T_ ? at.c : Ip;
         const T* row = gu + (size_t)t * 2 * I;
         float a[4], b[4], v[4], s;
         load_quad<T, VEC>(row, 2 * c, 2 * I, a);
@@ -144,6 +169,7 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_q8_kernel(float* __restrict_
         const int c = 4 * (threadIdx.x + i * blockDim.x);
         load_quad<float, VEC>(hrow, c, H, v[i]);
         if (kind == 1) {
+#pragma unroll 4                                        // (loads before sums)
             for (int s = 0; s < n_pending; ++s) {
                 float p[4];
                 load_quad<float, VEC>(reinterpret_cast<const float*>(pending) + (size_t)s * pstride + (size_t)t * H, c, H, p);
@@ -622,7 +648,10 @@ static void with_group(int G, F f) {
     else if (G == 64) f(std::integral_constant<int, 64>());
     else f(std::integral_constant<int, 128>());
 }
-static dim3 quad_grid(int T_, int Kp) { return dim3((Kp + 1023) / 1024, T_ < 65535 ? T_ : 65535); }
+static dim3 place_grid(int T_, int Kp, int each) {
+    const int units = Kp / each, across = units < 256 ? 256 / units : 1, rows = (T_ + across - 1) / across;
+    return dim3((units + 255) / 256, rows < 65535 ? rows : 65535);
+}
 
 template <typename T>
 static int launch_quantize_q8(const T* x, long long ldx, int8_t* q, float* s, int T_, int K, int G, cudaStream_t st) {
@@ -630,8 +659,8 @@ static int launch_quantize_q8(const T* x, long long ldx, int8_t* q, float* s, in
     const bool vec = K % 4 == 0 && ldx % 4 == 0 && aligned(x, 4 * sizeof(T));
     with_group(G, [&](auto gc) {
         constexpr int GC = decltype(gc)::value;
-        if (vec) rf_launch(quantize_q8_kernel<T, GC, true>, quad_grid(T_, Kp), dim3(256), 0, st, x, ldx, q, s, T_, K, Kp);
-        else rf_launch(quantize_q8_kernel<T, GC, false>, quad_grid(T_, Kp), dim3(256), 0, st, x, ldx, q, s, T_, K, Kp);
+        if (vec) rf_launch(quantize_q8_kernel<T, GC, true>, place_grid(T_, Kp, 4), dim3(256), 0, st, x, ldx, q, s, T_, K, Kp);
+        else rf_launch(quantize_q8_kernel<T, GC, false>, place_grid(T_, Kp, 4), dim3(256), 0, st, x, ldx, q, s, T_, K, Kp);
     });
     RF_LAUNCH_CHECK();
     return 0;
@@ -643,8 +672,8 @@ static int launch_swiglu_q8(const T* gu, int8_t* q, float* s, int T_, int I, int
     const bool vec = I % 2 == 0 && aligned(gu, 4 * sizeof(T));
     with_group(G, [&](auto gc) {
         constexpr int GC = decltype(gc)::value;
-        if (vec) rf_launch(swiglu_q8_kernel<T, ACT, GC, true>, quad_grid(T_, Ip), dim3(256), 0, st, gu, q, s, T_, I, Ip);
-        else rf_launch(swiglu_q8_kernel<T, ACT, GC, false>, quad_grid(T_, Ip), dim3(256), 0, st, gu, q, s, T_, I, Ip);
+        if (vec) rf_launch(swiglu_q8_kernel<T, ACT, GC, true>, place_grid(T_, Ip, 4), dim3(256), 0, st, gu, q, s, T_, I, Ip);
+        else rf_launch(swiglu_q8_kernel<T, ACT, GC, false>, place_grid(T_, Ip, 4), dim3(256), 0, st, gu, q, s, T_, I, Ip);
     });
     RF_LAUNCH_CHECK();
     return 0;
@@ -656,21 +685,26 @@ static int launch_add_rmsnorm_q8(float* h, const void* pending, int kind, int n_
     const int Hp = padded(H, G), quads = Hp / 4;
     if (quads > 8 * 1024) return RF_ERR_UNSUPPORTED;
     const bool vec = H % 4 == 0 && pstride % 4 == 0 && aligned(h, 16) && (kind == 0 || aligned(pending, kind == 1 ? 16 : 4 * sizeof(T)));
-    int threads = (quads + 31) / 32 * 32;
-    if (threads > 1024) threads = 1024;
-    const int per = (quads + threads - 1) / threads;
+    int per = (quads + 1023) / 1024;
+    per = per <= 1 ? 1 : per <= 2 ? 2 : 8;
+    // Two quads a thread where there are rows for every SM and long ones: more of them at once (2,048 x 3,584 after a 16-bit update 22.3 -> 16.6 us,
+    // four 17.9; 512 x 3,584 after four sums 11.0 -> 10.1).  Few or short rows want all the threads: 1 x 896 2.1 us, with two 3.0; 4,096 x 512
+    // 10.2, 11.1.
+    if (per == 1 && quads >= 384 && n_rows >= 2 * 148) per = 2;
+    const int threads = ((quads + per - 1) / per + 31) / 32 * 32;
     with_group(G, [&](auto gc) {
         constexpr int GC = decltype(gc)::value;
         auto go = [&](auto kernel) {
             rf_launch(kernel, dim3(n_rows), dim3(threads), 0, st, h, pending, kind, n_pending, pstride, w, w_is_f32, eps, q, s, rows, n_h, H, Hp);
         };
-        if (vec) {
-            if (per <= 1) go(add_rmsnorm_q8_kernel<T, GC, 1, true>);
-            else if (per <= 2) go(add_rmsnorm_q8_kernel<T, GC, 2, true>);
-            else go(add_rmsnorm_q8_kernel<T, GC, 8, true>);
-        } else {
-            go(add_rmsnorm_q8_kernel<T, GC, 8, false>);
-        }
+        auto by_form = [&](auto v) {
+            constexpr bool VEC = decltype(v)::value;
+            if (per == 1) go(add_rmsnorm_q8_kernel<T, GC, 1, VEC>);
+            else if (per == 2) go(add_rmsnorm_q8_kernel<T, GC, 2, VEC>);
+            else go(add_rmsnorm_q8_kernel<T, GC, 8, VEC>);
+        };
+        if (vec) by_form(std::true_type());
+        else by_form(std::false_type());
     });
     RF_LAUNCH_CHECK();
     return 0;
@@ -721,8 +755,12 @@ int rf_dequantize_q8(int dtype, const void* q, const void* scales, void* y, int 
     if (T_ < 0 || K <= 0 || bad_group(G)) return RF_ERR_BAD_ARG;
     if (T_ == 0) return 0;
     const int Kp = padded(K, G);
-    if (dtype == 0) rf_launch(dequantize_q8_kernel<float>, quad_grid(T_, Kp), dim3(256), 0, st, (const int8_t*)q, (const float*)scales, (float*)y, T_, K, Kp, G);
-    else rf_launch(dequantize_q8_kernel<__nv_bfloat16>, quad_grid(T_, Kp), dim3(256), 0, st, (const int8_t*)q, (const float*)scales, (__nv_bfloat16*)y, T_, K, Kp, G);
+    auto go = [&](auto kernel, auto* out, int each) { rf_launch(kernel, place_grid(T_, Kp, each), dim3(256), 0, st, (const int8_t*)q, (const float*)scales, out, T_, K, Kp, G); };
+    const bool eights = K % 8 == 0 && aligned(y, 16);
+    if (dtype == 0 && eights) go(dequantize_q8_kernel<float, 8>, (float*)y, 8);
+    else if (dtype == 0) go(dequantize_q8_kernel<float, 4>, (float*)y, 4);
+    else if (eights) go(dequantize_q8_kernel<__nv_bfloat16, 8>, (__nv_bfloat16*)y, 8);
+    else go(dequantize_q8_kernel<__nv_bfloat16, 4>, (__nv_bfloat16*)y, 4);
     RF_LAUNCH_CHECK();
     return 0;
 }
