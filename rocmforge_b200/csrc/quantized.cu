@@ -496,25 +496,29 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint
     auto write_round = [&](int round) {
         const float* at = sums + (splits > 1 ? round & 1 : 0) * 8 * NB * SUMS;
         const int rows_here = 16 * RT * at_once, n0 = (round * clusters + cluster) * rows_here;
-        for (int i = rank * THREADS + threadIdx.x; i < live * rows_here; i += splits * THREADS) {
-            const int tok = i / rows_here, r = i - tok * rows_here;
+        for (int i = rank * THREADS + threadIdx.x; i < live * rows_here / 4; i += splits * THREADS) {
+            const int tok = i / (rows_here / 4), r = (i - tok * (rows_here / 4)) * 4;
             const float* p = at + tok * SUMS + r / (16 * RT) * ways * 16 * RT + r % (16 * RT);
-            float v = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (splits == 1) {
-                for (int k = 0; k < ways; ++k) v += p[16 * RT * k];
+#pragma unroll 4
+                for (int k = 0; k < ways; ++k) {
+                    const float4 f = *reinterpret_cast<const float4*>(p + 16 * RT * k);
+                    v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
+                }
             } else {
                 const uint32_t here = (uint32_t)__cvta_generic_to_shared(p);
-                for (int c = 0; c < splits; ++c) {
+#pragma unroll 4                                        // (loads before sums: a peer's shared memory is far)
+                for (int j = 0, c = 0, k = 0; j < splits * ways; ++j) {
                     uint32_t there;
+                    float4 f;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(c));
-                    for (int k = 0; k < ways; ++k) {
-                        float f;
-                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there + 64 * RT * k) : "memory");
-                        v += f;
-                    }
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(there + 64 * RT * k));
+                    if (++k == ways) k = 0, ++c;
+                    v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
                 }
             }
-            w4_write(o, tok0 + tok, n0 + r, v);
+            w4_write4(o, tok0 + tok, n0 + r, v);
         }
     };
 

@@ -30,28 +30,38 @@ __device__ __forceinline__ void w4_write(const W4Out& o, int t, int n, float v) 
     else if (o.is_f32) reinterpret_cast<float*>(o.out)[at] = v;
     else reinterpret_cast<__nv_bfloat16*>(o.out)[at] = __float2bfloat16_rn(v);
 }
-// Columns n .. n + 3, n a multiple of 4.
-__device__ __forceinline__ void w4_write4(const W4Out& o, int t, int n, float4 v) {
+// Columns n .. n + 3, n a multiple of 4.  (What is read is read before anything is written: a load behind a store would wait for it.)
+__device__ __forceinline__ void w4_write4(const W4Out& o, int t, int n, float4 v4) {
     if (n >= o.N) return;
-    if (!o.fours) {
-        w4_write(o, t, n, v.x), w4_write(o, t, n + 1, v.y), w4_write(o, t, n + 2, v.z), w4_write(o, t, n + 3, v.w);
-        return;
-    }
+    const int live = min(4, o.N - n);
+    float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    float* to = reinterpret_cast<float*>(o.out) + (size_t)t * o.N + n;   // (32-bit results)
     if (o.bias != nullptr) {
-        v.x += load_vec(o.bias, o.bias_is_f32, n), v.y += load_vec(o.bias, o.bias_is_f32, n + 1);
-        v.z += load_vec(o.bias, o.bias_is_f32, n + 2), v.w += load_vec(o.bias, o.bias_is_f32, n + 3);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < live) v[j] += load_vec(o.bias, o.bias_is_f32, n + j);
     }
-    const size_t at = (size_t)t * o.N + n;
-    if (o.is_f32) {
-        float4* to = reinterpret_cast<float4*>(reinterpret_cast<float*>(o.out) + at);
-        if (o.add) {
-            const float4 old = *to;
-            v.x += old.x, v.y += old.y, v.z += old.z, v.w += old.w;
-        }
-        *to = v;
+    if (o.add) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < live) v[j] += to[j];
+    }
+    if (o.fours && o.is_f32) {
+        *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if (o.is_f32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < live) to[j] = v[j];
     } else {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-        *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(o.out) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        __nv_bfloat16* to16 = reinterpret_cast<__nv_bfloat16*>(o.out) + (size_t)t * o.N + n;
+        if (o.fours) {
+            const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+            *reinterpret_cast<uint2*>(to16) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < live) to16[j] = __float2bfloat16_rn(v[j]);
+        }
     }
 }
 
