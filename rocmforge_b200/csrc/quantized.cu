@@ -714,23 +714,26 @@ static int launch_add_rmsnorm_q8(float* h, const void* pending, int kind, int n_
     return 0;
 }
 
-// f(group, rows, eights, tiles a warp) with the constants and types of a product's kernel; false: there is none
+// f(group, rows, eights, tiles a warp) with the constants and types of a product's kernel; false: there is none (more than sixteen 16-bit rows
+// are the tensor cores' kernel's)
 template <typename F>
 static bool with_product(int x_kind, int G, int eights, int pair, F f) {
-    if (!(eights == 1 && pair == 1) && !((eights == 2 || eights == 4) && (pair == 1 || pair == 2))) return false;
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    using Four = std::integral_constant<int, 4>;
+    if (!(eights == 1 && pair == 1) && !(eights == 2 && (pair == 1 || pair == 2)) && !(eights == 4 && (pair == 1 || pair == 2) && x_kind == 0)) return false;
     with_group(G, [&](auto gc) {
-        using One = std::integral_constant<int, 1>;
-        using Two = std::integral_constant<int, 2>;
-        using Four = std::integral_constant<int, 4>;
-        auto with_rows = [&](auto rows) {
+        const int8_t* bytes = nullptr;
+        const __nv_bfloat16* wide = nullptr;
+        auto few = [&](auto rows) {
             if (eights == 1) f(gc, rows, One(), One());
-            else if (eights == 2 && pair == 1) f(gc, rows, Two(), One());
-            else if (eights == 2) f(gc, rows, Two(), Two());
-            else if (pair == 1) f(gc, rows, Four(), One());
-            else f(gc, rows, Four(), Two());
+            else if (pair == 1) f(gc, rows, Two(), One());
+            else f(gc, rows, Two(), Two());
         };
-        if (x_kind == 0) with_rows(static_cast<const int8_t*>(nullptr));
-        else with_rows(static_cast<const __nv_bfloat16*>(nullptr));
+        if (x_kind != 0) few(wide);
+        else if (eights < 4) few(bytes);
+        else if (pair == 1) f(gc, bytes, Four(), One());
+        else f(gc, bytes, Four(), Two());
     });
     return true;
 }

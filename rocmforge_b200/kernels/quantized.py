@@ -331,32 +331,39 @@ def w4_clusters(splits: int, device: int) -> int:
     return n
 
 
+# What a warp of rf_gemm_w4 takes for 128 columns of its tiles, by 8-bit rows, eights of tokens and tiles a warp, as a share of what four eights
+# of 8-bit rows by one tile take; half of one more a round in which warps wait for one another, one where clusters exchange their sums.  (In
+# 165 cases from 1 x 896 x 896 to 128 x 3,584 x 18,944 the plans chosen by it took 1 % more than the best of all, 14 % at most.)
+W4_COST = {(True, 1, 1): 0.3, (True, 2, 1): 0.55, (True, 2, 2): 0.9, (True, 4, 1): 1.0, (True, 4, 2): 1.9,
+           (False, 1, 1): 0.4, (False, 2, 1): 0.5, (False, 2, 2): 1.05}
+
+
 @functools.lru_cache(4096)
 def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
-    """(eights of tokens, tiles a warp, warps a tile, splits, clusters): how ``rf_gemm_w4`` shares out a product.  Chosen from sizes alone: the
-    units of 128 columns that the busiest warp goes through, 1.9 for a unit of two tiles, one more a round in which warps wait for one
-    another, three more where clusters exchange their sums."""
+    """(eights of tokens, tiles a warp, warps a tile, splits, clusters): how ``rf_gemm_w4`` shares out a product, chosen from sizes alone by
+    what the busiest warp takes; None where no way fits into shared memory."""
     units, rows16 = (padded_columns(K, group) // 64 + 1) // 2, (N + 15) // 16
-    eights, best = 1 if M <= 8 else 2 if M <= 16 else 4, None
-    while eights and best is None:                       # fewer tokens at once where longer rows leave no room for more
-        shares = (M + 8 * eights - 1) // (8 * eights)
-        for pair in (1, 2) if eights > 1 else (1,):
-            tiles = (rows16 + pair - 1) // pair
-            for splits in range(1, 9):
-                clusters = max(1, clusters_of(splits) // shares)
-                for ways in (1, 2, 4, 8, 16):
-                    used = min(clusters, (tiles * ways + 15) // 16)
-                    if _f("rf_gemm_w4_shared")(0 if q8 else 1, M, N, K, group, eights, pair, ways, splits, used) > W4_MOST_SHARED:
-                        continue
-                    rounds = (tiles + used * (16 // ways) - 1) // (used * (16 // ways))
-                    each = (units + splits * ways - 1) // (splits * ways) * (1.9 if pair == 2 else 1)
-                    cost = rounds * (each + (ways > 1 or splits > 1)) + 3 * (splits > 1)
-                    if best is None or cost < best[0]:
-                        best = cost, eights, pair, ways, splits, used
-        eights //= 2
-    if best is None:
-        raise KernelError(f"gemm_w4: rows of {K} columns are too long")
-    return best[1:]
+    # tokens at once: fewer than there are only where longer rows leave no room, or (above 16) where that is faster
+    for some in ((1,),) if M <= 8 else ((2,), (1,)) if M <= 16 or not q8 else ((2, 4), (1,)):
+        best = None
+        for eights in some:
+            shares = (M + 8 * eights - 1) // (8 * eights)
+            for pair in (1, 2) if eights > 1 else (1,):
+                tiles = (rows16 + pair - 1) // pair
+                for splits in range(1, 9):
+                    clusters = max(1, clusters_of(splits) // shares)
+                    for ways in (1, 2, 4, 8, 16):
+                        used = min(clusters, (tiles * ways + 15) // 16)
+                        if _f("rf_gemm_w4_shared")(0 if q8 else 1, M, N, K, group, eights, pair, ways, splits, used) > W4_MOST_SHARED:
+                            continue
+                        rounds = (tiles + used * (16 // ways) - 1) // (used * (16 // ways))
+                        each = (units + splits * ways - 1) // (splits * ways) * W4_COST[q8, eights, pair]
+                        cost = rounds * (each + 0.5 * (ways > 1 or splits > 1)) + (splits > 1)
+                        if best is None or cost < best[0]:
+                            best = cost, eights, pair, ways, splits, used
+        if best is not None:
+            return best[1:]
+    return None
 
 
 # What a block of rf_gemm_w4_tc takes, by the tokens of its tile: us for 512 columns, us beside them.
@@ -426,18 +433,22 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
     if code == 0 and not q8:
         return _gemm_by_16_bits(x, w, bias, out, accumulate)
     on = _clusters_on(here)
-    if not q8 and M >= W4_TC_TOKENS:
-        if M > (W4_TC_MOST_F32 if f32 and K > SUM_COLUMNS else W4_TC_MOST) and at % 16 == 0 and ld % 8 == 0 and ld >= K and tc.supported(M, N, K, tc.STORE):
+    plan = w4_launch(q8, M, N, K, w.group, on) if q8 or M < W4_TC_TOKENS else None
+    if plan is not None:
+        done = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales_at if q8 else None, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
+                                *plan, M, N, K, w.group, stream())
+    elif q8:
+        raise KernelError(f"gemm_w4: rows of {K} columns are too long")
+    else:
+        rows_fit = at % 16 == 0 and ld % 8 == 0 and ld >= K             # the kernels copy whole 16 bytes
+        if M > (W4_TC_MOST_F32 if f32 and K > SUM_COLUMNS else W4_TC_MOST) and rows_fit and tc.supported(M, N, K, tc.STORE):
             return _gemm_by_16_bits(x, w, bias, out, accumulate)
-        if at % 16 or ld % 8 or ld < K:                  # the kernel copies whole 16 bytes (64 x 37,888 x 3,583 by rf_gemm_w4: 100 us)
+        if not rows_fit:                                 # (64 x 37,888 x 3,583 by rf_gemm_w4, which would take them: 100 us)
             x, rows = torch.empty(M, (K + 7) // 8 * 8, dtype=dt, device=x.device), x
             x[:, :K] = rows
             at, ld = x.data_ptr(), x.stride(0)
         done = _f("rf_gemm_w4_tc")(at, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
                                    *w4_tc_launch(M, N, K, w.group, on), M, N, K, w.group, tc.status_word(w.packed.device).data_ptr(), stream())
-    else:
-        done = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales_at if q8 else None, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
-                                *w4_launch(q8, M, N, K, w.group, on), M, N, K, w.group, stream())
     check(done, "gemm_w4" if done == 0 else f"gemm_w4 ({M}x{N}x{K}, groups of {w.group})")
     return out
 

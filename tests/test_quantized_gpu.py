@@ -188,6 +188,8 @@ def test_every_way_to_share_out_a_product(monkeypatch, M, eights, pair, ways, cl
     """Columns over warps and over CTAs of a cluster (some of which get none), tiles over several rounds, tokens over several blocks."""
     from rocmforge_b200 import kernels
     from rocmforge_b200.kernels import quantized
+    if kind == "bf16" and eights == 4:
+        pytest.skip("more than sixteen 16-bit rows are the tensor cores' kernel's")
     monkeypatch.setattr(quantized, "w4_launch", lambda *a: (eights, pair, ways, splits, clusters))
     monkeypatch.setattr(quantized, "W4_TC_TOKENS", 1000)
     x, x64, w, full = product_case(kind, M, N, K, G)
