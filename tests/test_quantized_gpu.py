@@ -155,7 +155,7 @@ def terms_of(kind, K):
     return K // 32 + 24 if kind == "q8" else 2 * K + 24
 
 
-SIZES = [(16, 64, 32), (17, 100, 64), (1, 128, 128), (1003, 1100, 32), (100, 896, 128), (200, 2050, 64), (48, 19001, 128)]
+SIZES = [(16, 64, 32), (5, 1, 32), (33, 8, 64), (17, 100, 64), (1, 128, 128), (1003, 1100, 32), (100, 896, 128), (200, 2050, 64), (48, 19001, 128)]
 
 
 @pytest.mark.parametrize("kind", ["q8", "bf16", "f32"])
@@ -221,6 +221,53 @@ def test_every_tile_on_the_tensor_cores(monkeypatch, M, bn, splits, N, K, G):
     kernels.tensor_core.check_status(torch.device(DEV))
 
 
+@pytest.mark.parametrize("M,K", [(513, 256), (600, 2104), (2049, 2104), (2049, 2103), (5000, 72)])
+def test_many_tokens(M, K):
+    """Where the weights are written out in 16 bits for the 16-bit product, in pieces of the columns for 32-bit results, and next to it."""
+    from rocmforge_b200 import kernels
+    x, x64, w, full = product_case("bf16", M, 130, K, 128)
+    x64, full = x64.to(DEV), full.to(DEV)
+    want, size, b, h = x64 @ full.T, x64.abs() @ full.abs().T, numbers(130, seed=2), numbers(M, 130, seed=9)
+    close(kernels.gemm_w4(x, w), want, size, terms_of("bf16", K), BF)
+    close(kernels.gemm_w4(x, w, b.to(DEV), out_f32=True), want + b.double().to(DEV), size + b.double().abs().to(DEV), terms_of("bf16", K) + 1, F32)
+    close(kernels.gemm_w4(x, w, out=h.to(DEV), accumulate=True), want + h.double().to(DEV), size + h.double().abs().to(DEV), terms_of("bf16", K) + 2, F32)
+
+
+@pytest.mark.parametrize("kind", ["q8", "bf16"])
+def test_long_sums_are_rounded_not_cut(kind):
+    """Sums of numbers of one sign, where what the tensor cores cut would add up: 40 tokens, 18,944 columns, against a 32-bit sum's error."""
+    from rocmforge_b200 import kernels
+    w = kernels.quantize_w4(numbers(64, 18944, spread=False).abs().to(DEV), 64)
+    x = numbers(40, 18944, dt=BF, spread=False).abs().to(DEV)
+    r = kernels.quantize_q8(x, 64) if kind == "q8" else x
+    x64 = stands_for(r).to(DEV) if kind == "q8" else x.double()
+    want = x64 @ kernels.dequantize_w4(w, F32).double().T
+    # pieces of 2,048 columns: 128 additions of 16 products, each cut by at most 2^-23 of a sum that grows evenly (half of it on average); ten
+    # roundings between pieces.  8-bit rows: 296 groups' roundings, two a factor
+    bound = (128 / 2 + 10) * 2.0 ** -23 if kind == "bf16" else (296 / 2 + 4) * 2.0 ** -24
+    err = ((kernels.gemm_w4(r, w, out_f32=True).double() - want).abs() / want).max().item()
+    assert err <= bound, (err, bound)
+
+
+def test_products_on_two_streams_at_once():
+    """Products of every kind, clusters among them, on two streams at the same time: what they are alone."""
+    from rocmforge_b200 import kernels
+    w, _ = weight(1000, 8200, 128)
+    xs = [numbers(M, 8200, seed=M, dt=BF).to(DEV) for M in (1, 16, 40, 300)]
+    calls = [lambda x=x: kernels.gemm_w4(x, w, out_f32=True) for x in xs] + [lambda x=x: kernels.gemm_w4(kernels.quantize_q8(x, 128), w, out_f32=True) for x in xs[:3]]
+    alone = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for i in range(len(calls)):
+        for j, side in enumerate(streams):
+            with torch.cuda.stream(side):
+                got[j].append(calls[i if j == 0 else len(calls) - 1 - i]())
+    torch.cuda.synchronize()
+    for i, want in enumerate(alone):
+        assert torch.equal(got[0][i], want) and torch.equal(got[1][len(calls) - 1 - i], want)
+    kernels.tensor_core.check_status(torch.device(DEV))
+
+
 @pytest.mark.parametrize("kind", ["q8", "bf16"])
 def test_a_row_does_not_depend_on_its_neighbours(kind):
     from rocmforge_b200 import kernels
@@ -275,7 +322,7 @@ def test_empty_and_refused():
 
 # ---------------------------------------------------------------- norm and gated unit
 @pytest.mark.parametrize("G", [32, 64, 128])
-@pytest.mark.parametrize("T,H", [(1, 64), (1, 896), (2, 100), (3, 1003), (64, 5120), (5, 8192), (1, 16384), (2, 30000), (300, 256)])
+@pytest.mark.parametrize("T,H", [(1, 64), (1, 896), (2, 100), (3, 1003), (64, 5120), (5, 8192), (1, 16384), (2, 30000), (300, 256), (300, 1600), (297, 1601)])
 @pytest.mark.parametrize("pending", [None, 1, 5, 17, "same", "f32"])
 def test_norm_to_8_bits(G, T, H, pending):
     from rocmforge_b200 import kernels
@@ -377,6 +424,33 @@ def test_a_layers_run_captured_and_replayed_on_another_stream():
             gu = keep["gu"].cpu().double()
             check_rows(keep["a"], gu[:, ::2] * torch.sigmoid(gu[:, ::2]) * gu[:, 1::2], 2.0 ** -20)
             close(h, start.double().to(DEV) + a64 @ f2.T, start.double().abs().to(DEV) + a64.abs() @ f2.abs().T, terms_of("q8", I) + 1, F32)
+    torch.cuda.current_stream().wait_stream(side)
+
+
+def test_a_prompts_products_captured_and_replayed():
+    """16-bit rows on the tensor cores' kernel, aligned and not, and through the weights in 16 bits, in one graph, replayed with other rows."""
+    from rocmforge_b200 import kernels
+    w, full = weight(200, 264, 64)
+    full = full.to(DEV)
+    x = torch.zeros(700, 264, device=DEV, dtype=BF)
+    odd, _ = weight(48, 263, 64)
+    body = lambda: (kernels.gemm_w4(x[:40], w), kernels.gemm_w4(x[:33, :263], odd), kernels.gemm_w4(x, w))  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        body()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = body()
+        for seed in (1, 2):
+            x.copy_(numbers(700, 264, seed=seed, dt=BF))
+            graph.replay()
+            torch.cuda.synchronize()
+            x64 = x.double()
+            close(out[0], x64[:40] @ full.T, x64[:40].abs() @ full.abs().T, terms_of("bf16", 264), BF)
+            close(out[2], x64 @ full.T, x64.abs() @ full.abs().T, terms_of("bf16", 264), BF)
+            for now, then in zip(out, body()):
+                assert torch.equal(now, then)
     torch.cuda.current_stream().wait_stream(side)
 
 
