@@ -72,7 +72,7 @@ struct Place {
 };
 
 // ---------------------------------------------------------------- rows to 8 bits
-// A lane has four columns.
+// A lane has four columns.  (64 x 3,584 1.6 us: a launch; 2,048 x 3,584 9.9, floor 3.4: a group's two divisions and shuffles in every lane.)
 template <typename T, int G, bool VEC>
 __global__ void __launch_bounds__(256) quantize_q8_kernel(const T* x, long long ldx, int8_t* __restrict__ q, float* __restrict__ scales,
                                                           int T_, int K, int Kp) {
@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(256) quantize_q8_kernel(const T* x, long long 
     }
 }
 
-// ... and the numbers that 8-bit rows stand for, eight (rows of whole eights, on 16-byte boundaries) or four columns a thread.
+// ... and the numbers that 8-bit rows stand for, eight (rows of whole eights, on 16-byte boundaries: 2,048 x 3,584 5.5 us, by fours 9.2) or four
+// columns a thread.
 template <typename T, int EACH>
 __global__ void __launch_bounds__(256) dequantize_q8_kernel(const int8_t* q, const float* scales, T* __restrict__ y, int T_, int K, int Kp, int G) {
     pdl_trigger();
@@ -120,7 +121,8 @@ __global__ void __launch_bounds__(256) dequantize_q8_kernel(const int8_t* q, con
 }
 
 // ---------------------------------------------------------------- gated unit to 8 bits
-// y[t, j] = act(gu[t, 2j]) gu[t, 2j + 1] (the fused weight's rows are interleaved), in 32 bits and from there to 8.
+// y[t, j] = act(gu[t, 2j]) gu[t, 2j + 1] (the fused weight's rows are interleaved), in 32 bits and from there to 8.  128 x 18,944 5.9 us (the one with a
+// 16-bit result 8.0, floor 1.9): exponentials and divisions; 1 x 4,864 1.7: a launch.
 template <typename T, int ACT, int G, bool VEC>
 __global__ void __launch_bounds__(256) swiglu_q8_kernel(const T* gu, int8_t* __restrict__ q, float* __restrict__ scales, int T_, int I, int Ip) {
     pdl_trigger();
@@ -151,7 +153,9 @@ __global__ void __launch_bounds__(256) swiglu_q8_kernel(const T* gu, int8_t* __r
 
 // ---------------------------------------------------------------- add + RMSNorm to 8 bits
 // v = h[row] + sum_s pending[s][row];  y = v rsqrt(mean(v^2) + eps) w, to 8 bits from 32.  The kinds of pending and of rows are those
-// of add_rmsnorm (elementwise.cu).  A block has a row, a lane four columns at a time, in registers.
+// of add_rmsnorm (elementwise.cu).  A block has a row, a lane four columns at a time, in registers: one pass over the stream and what is added to
+// it.  2,048 x 3,584 after a 16-bit update 16.6 us, 4.9 TB/s (the norm with a 16-bit result 21.1); 64 x 5,120 after five sums 4.6 and 1 x 896 after
+// four 2.0: a chain of trips to L2 and of the block's sum.
 template <typename T, int G, int NV, bool VEC>
 __global__ void __launch_bounds__(1024) add_rmsnorm_q8_kernel(float* __restrict__ h, const void* pending, int kind, int n_pending,
                                                               size_t pstride, const void* w, int w_is_f32, float eps,
@@ -373,7 +377,12 @@ __device__ __forceinline__ unsigned long long fma_two(unsigned long long a, unsi
 // where a tile is one warp's.
 // A group's (at most 128 columns') exact sum is formed by the tensor cores in whole numbers and added up in 32 bits; the whole number starts
 // at 1.5 2^23 as a float's bits, so that its bits are that float plus the sum (below 2^22: 128 columns of 16 * 8 * 127), and no conversion is
-// needed.
+// needed.  16-bit rows: the halves of bytes become bfloat16 numbers and a group's sum is a float.
+// What bounds it, and what it took (device time in a chain of launches over weights larger than L2): 1 to 8 8-bit rows x 37,888 x 3,584 12.9 to
+// 13.1 us, 5.5 TB/s: the weights' stream; 1 x 4,608 x 3,584 4.4 us, 1 x 896 x 896 2.4: a launch, one trip to memory and the warps' sums.  16 rows
+// 14.4 us, 32 21.4, 64 35.2 (in groups of 32 columns 59), 64 x 3,584 x 18,944 in groups of 64 33.2: instructions; at 64 x 37,888 x 3,584 the
+// schedulers issue in 60 % of cycles and the tensor cores are busy in 38 %.  16-bit rows: 1 x 37,888 x
+// 3,584 19 us, 16 x 27,648 x 5,120 26.7: widening the weights, whatever the tokens.
 #define W4_WARPS 16
 #define W4_SLOT (1024 + 128)                             // a unit's weights, and its scales [group][16 rows]
 #define W4_SUMS(rt) (16 * (rt) * W4_WARPS + 4)           // pitch of the warps' sums [token][16 rt rows a warp]
