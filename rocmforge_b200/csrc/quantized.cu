@@ -869,8 +869,8 @@ int rf_gemm_w4_clusters(int splits) {
 }
 
 // out = x w^T (+ bias): x_kind 0: 8-bit rows (x int8 [M, Kp], xs float32 [M, Kp / G]), 1: bfloat16 rows [M, K], ldx apart; out as W4Out
-// has it.  eights: eights of tokens a block (1, 2, 4); pair: tiles of 16 rows a warp (1; 2 from two eights on); ways: warps a tile (a power of two up to 16); splits: CTAs of a cluster that share
-// out the columns (1 .. 8); clusters: of each share of tokens.
+// has it.  eights: eights of tokens a block (1, 2; 8-bit rows 4 too); pair: tiles of 16 rows a warp (1; 2 from two eights on); ways: warps a tile
+// (a power of two up to 16); splits: CTAs of a cluster that share out the columns (1 .. 8); clusters: of each share of tokens.
 int rf_gemm_w4(int x_kind, const void* x, const void* xs, long long ldx, const void* packed, const void* scales, const void* bias, int bias_is_f32,
                void* out, int out_is_f32, int add, int eights, int pair, int ways, int splits, int clusters, int M, int N, int K, int G, cudaStream_t st) {
     if (M <= 0 || N <= 0 || K <= 0 || bad_group(G) || (add && !out_is_f32)) return RF_ERR_BAD_ARG;

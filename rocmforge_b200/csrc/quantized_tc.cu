@@ -32,10 +32,13 @@ struct TcShape {
     static constexpr int GROUPS = 4, STORED = 8;         // of widening warps; a stage's blocks of 64 columns as they are stored
     static constexpr int WORDS = STORED * 512, SCALES = 512 / G * 32, STAGES = 2;       // bytes of a stage, of a tile of 16 rows
     static constexpr int PLACES = 4, ROWS = BN == 128 ? 4 : 8;          // blocks of 128 columns in tensor memory; of tokens' numbers
-    static constexpr int B = BN * 256, RINGS = ROWS * B + STAGES * 8 * (WORDS + SCALES), BYTES = 1024 + RINGS + 512;      // (alignment, barriers)
+    static constexpr int B = BN * 256, RINGS = ROWS * B + STAGES * 8 * (WORDS + SCALES), NEEDED = 1024 + RINGS + 512;     // (alignment, barriers)
     static constexpr int BUFS = BN == 128 ? 1 : 2, SUMS = 64 * PLACES;  // accumulators and, behind them, the pieces' sum, behind the weights
     static constexpr int SHARE = BN / 4 < 16 ? 16 : BN / 4;             // a widening warp's part of the sums: 32 rows, so many tokens
     static constexpr int PIECE = W4T_PIECE / 128, PIECE_STAGES = PIECE / GROUPS;
+    // A block takes all of an SM's tensor memory.  It asks for so much shared memory that no block of another kernel that wants some fits beside it:
+    // two clusters could otherwise wait for one another's.
+    static constexpr int BYTES = NEEDED > 190 * 1024 ? NEEDED : 190 * 1024;
     static_assert(BYTES <= W4T_MOST_SHARED && RINGS >= BN * W4T_PITCH * 4, "the rings' place holds the sums");
     static_assert(SUMS + (BUFS + 1) * BN <= 512 && PIECE % ROWS == 0, "");
     static_assert(PLACES % GROUPS == 0 && ROWS % GROUPS == 0, "one parity bit tells two phases apart, not three");

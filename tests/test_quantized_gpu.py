@@ -283,6 +283,19 @@ def test_a_row_does_not_depend_on_its_neighbours(kind):
     assert y[2].isnan().all() and torch.equal(y[[0, 1, 3, 4, 5, 6, 7]], whole[[0, 1, 3, 4, 5, 6, 7]])
 
 
+def test_a_row_does_not_depend_on_its_neighbours_on_the_tensor_cores():
+    from rocmforge_b200 import kernels
+    w, _ = weight(300, 5000, 64)
+    x = numbers(120, 5000, dt=BF).to(DEV)
+    whole = kernels.gemm_w4(x, w, out_f32=True)
+    assert torch.equal(kernels.gemm_w4(x[:110], w, out_f32=True), whole[:110])
+    x[2], x[50, 4999], x[119, 0] = float("nan"), float("inf"), -float("inf")
+    y = kernels.gemm_w4(x, w, out_f32=True)
+    bad = [2, 50, 119]
+    rest = [i for i in range(120) if i not in bad]
+    assert torch.equal(y[rest], whole[rest]) and not y[bad].isfinite().any()
+
+
 @pytest.mark.parametrize("M", [1, 40, 300])
 def test_16_bit_rows_any_distance_apart(M):
     from rocmforge_b200 import kernels
