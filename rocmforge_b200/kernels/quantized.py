@@ -313,9 +313,10 @@ W4_FEW_TOKENS = 32
 # to so many (512 x 37,888 x 3,584: 148 us, 165 by the weights written out in 16 bits; 512 x 3,584 x 18,944: 63, 124; 1,024: 317, 257 and 128, 137).
 W4_TC_TOKENS = 17
 W4_TC_MOST = 512
-# 32-bit results of rows longer than SUM_COLUMNS: up to so many, since that other way takes a pass over the result for every such piece (2,048 x
-# 3,584 x 18,944: 288 us against 332; 4,096: 626, 578)
-W4_TC_MOST_F32 = 2048
+# 32-bit results of rows of several SUM_COLUMNS: up to so many with two of them, twice as many with more, since that other way takes a pass over
+# the result for each (1,024 x 4,608 x 3,584: 36 us against 49, 2,048: 70, 66; 2,048 x 3,584 x 18,944: 275, 331; 4,096: 502, 564; 2,048 x 5,120 x
+# 13,824: 282, 311)
+W4_TC_MOST_F32 = 1024
 # Columns that one tensor-core sum runs over where the result is 32-bit: its additions are cut, not rounded, and what is cut adds up
 # (1,999 x 3,584 x 18,944 against 64 bits: one sum 1.1e-5, pieces of 6,315 2.6e-6, of 2,048 5e-7)
 SUM_COLUMNS = 2048
@@ -441,7 +442,8 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
         raise KernelError(f"gemm_w4: rows of {K} columns are too long")
     else:
         rows_fit = at % 16 == 0 and ld % 8 == 0 and ld >= K             # the kernels copy whole 16 bytes
-        if M > (W4_TC_MOST_F32 if f32 and K > SUM_COLUMNS else W4_TC_MOST) and rows_fit and tc.supported(M, N, K, tc.STORE):
+        most = W4_TC_MOST_F32 * (2 if K > 2 * SUM_COLUMNS else 1) if f32 and K > SUM_COLUMNS else W4_TC_MOST
+        if M > most and rows_fit and tc.supported(M, N, K, tc.STORE):
             return _gemm_by_16_bits(x, w, bias, out, accumulate)
         if not rows_fit:                                 # (64 x 37,888 x 3,583 by rf_gemm_w4, which would take them: 100 us)
             x, rows = torch.empty(M, (K + 7) // 8 * 8, dtype=dt, device=x.device), x

@@ -221,7 +221,7 @@ def test_every_tile_on_the_tensor_cores(monkeypatch, M, bn, splits, N, K, G):
     kernels.tensor_core.check_status(torch.device(DEV))
 
 
-@pytest.mark.parametrize("M,K", [(513, 256), (600, 2104), (2049, 2104), (2049, 2103), (5000, 72)])
+@pytest.mark.parametrize("M,K", [(513, 256), (600, 2104), (1025, 2104), (2049, 2103), (2049, 4200), (1030, 4200), (5000, 72)])
 def test_many_tokens(M, K):
     """Where the weights are written out in 16 bits for the 16-bit product, in pieces of the columns for 32-bit results, and next to it."""
     from rocmforge_b200 import kernels
