@@ -723,8 +723,8 @@ static int launch_add_rmsnorm_q8(float* h, const void* pending, int kind, int n_
     return 0;
 }
 
-// f(group, rows, eights, tiles a warp) with the constants and types of a product's kernel; false: there is none (more than sixteen 16-bit rows
-// are the tensor cores' kernel's)
+// f(group, rows, eights, tiles a warp) with the constants and types of a product's kernel; false: there is none (where four eights of 16-bit rows
+// would pay, the tensor cores' kernel takes less)
 template <typename F>
 static bool with_product(int x_kind, int G, int eights, int pair, F f) {
     using One = std::integral_constant<int, 1>;

@@ -1,4 +1,4 @@
-// Products of bfloat16 rows with 4-bit weights on the 5th-generation tensor cores, from 17 tokens on.
+// Products of bfloat16 rows with 4-bit weights on the 5th-generation tensor cores, from some 17 tokens on.
 //
 // Weights are the accumulator's rows, tokens its columns.  128 rows' weights come as they are stored, by TMA, four blocks of 128 columns a stage,
 // ahead and before the wait for the kernel before.  Four groups of four warps have every fourth block each: a lane reads a row's (whatever the

@@ -309,9 +309,8 @@ def swiglu_q8(gu: torch.Tensor, group: int = 128, activation: str = "silu") -> Q
 # Products of up to so many tokens take rows in 8 bits where a step may choose (32 x 37,888 x 3,584: 22.0 us against 27.8 of 16-bit rows; 64 tokens:
 # 34.7, 29.3; 64 x 3,584 x 18,944: 30.6, 19.7).
 W4_FEW_TOKENS = 32
-# 16-bit rows: from so many tokens on the tensor cores' kernel (16 x 37,888 x 3,584: rf_gemm_w4 21.3 us, rf_gemm_w4_tc 27.6; 24 tokens: 31.4, 27.7), up
-# to so many (512 x 37,888 x 3,584: 148 us, 165 by the weights written out in 16 bits; 512 x 3,584 x 18,944: 63, 124; 1,024: 317, 257 and 128, 137).
-W4_TC_TOKENS = 17
+# 16-bit rows straight from the 4 bits: up to so many tokens (512 x 37,888 x 3,584: 148 us, 165 by the weights written out in 16 bits; 512 x 3,584 x
+# 18,944: 63, 124; 1,024: 317, 257 and 128, 137).
 W4_TC_MOST = 512
 # 32-bit results of rows of several SUM_COLUMNS: up to so many with two of them, twice as many with more, since that other way takes a pass over
 # the result for each (1,024 x 4,608 x 3,584: 36 us against 49, 2,048: 70, 66; 2,048 x 3,584 x 18,944: 275, 331; 4,096: 502, 564; 2,048 x 5,120 x
@@ -339,10 +338,9 @@ W4_COST = {(True, 1, 1): 0.3, (True, 2, 1): 0.55, (True, 2, 2): 0.9, (True, 4, 1
            (False, 1, 1): 0.4, (False, 2, 1): 0.5, (False, 2, 2): 1.05}
 
 
-@functools.lru_cache(4096)
-def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
-    """(eights of tokens, tiles a warp, warps a tile, splits, clusters): how ``rf_gemm_w4`` shares out a product, chosen from sizes alone by
-    what the busiest warp takes; None where no way fits into shared memory."""
+def _w4_few(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
+    """(cost, eights of tokens, tiles a warp, warps a tile, splits, clusters): how ``rf_gemm_w4`` shares out a product, by what the busiest
+    warp takes; None where no way fits into shared memory."""
     units, rows16 = (padded_columns(K, group) // 64 + 1) // 2, (N + 15) // 16
     # tokens at once: fewer than there are only where longer rows leave no room, or (above 16) where that is faster
     for some in ((1,),) if M <= 8 else ((2,), (1,)) if M <= 16 or not q8 else ((2, 4), (1,)):
@@ -363,7 +361,7 @@ def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
                         if best is None or cost < best[0]:
                             best = cost, eights, pair, ways, splits, used
         if best is not None:
-            return best[1:]
+            return best
     return None
 
 
@@ -371,9 +369,8 @@ def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
 W4_TC_COST = {32: (1.48, 3.2), 64: (1.5, 3.8), 128: (1.5, 7.5)}
 
 
-@functools.lru_cache(4096)
-def w4_tc_launch(M: int, N: int, K: int, group: int, clusters_of):
-    """(tokens of a tile, splits): how ``rf_gemm_w4_tc`` shares out a product of 16-bit rows, chosen from sizes alone."""
+def _w4_tc(M: int, N: int, K: int, group: int, clusters_of):
+    """(us, tokens of a tile, splits): how ``rf_gemm_w4_tc`` shares out a product of 16-bit rows."""
     stages, rows, best = (padded_columns(K, group) + 511) // 512, (N + 127) // 128, None
     for bn, (stage, beside) in W4_TC_COST.items():
         tiles = rows * ((M + bn - 1) // bn)
@@ -382,7 +379,20 @@ def w4_tc_launch(M: int, N: int, K: int, group: int, clusters_of):
             cost = rounds * ((stages + splits - 1) // splits * stage + beside) + 0.5 * (splits > 1)
             if best is None or cost < best[0]:
                 best = cost, bn, splits
-    return best[1:]
+    return best
+
+
+@functools.lru_cache(4096)
+def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
+    """How a product is shared out, chosen from sizes alone: five numbers for ``rf_gemm_w4`` (``_w4_few``), two for ``rf_gemm_w4_tc``
+    (``_w4_tc``), None where neither takes it.  16-bit rows go where less time is expected, ``rf_gemm_w4``'s cost being 1.3 us after 2.5
+    (16 x 37,888 x 3,584: 21.5 us there, 28.6 on the tensor cores; 32: 38.9, 28.8; 32 x 4,608 x 3,584: 8.3, 9.5; 64: 12.5, 10.1; 32 x 896 x
+    4,864: 6.2, 6.7; 128: 10.7, 8.2).  Above 128 tokens only the tensor cores are looked at."""
+    few = _w4_few(q8, M, N, K, group, clusters_of) if q8 or M <= 128 else None
+    if q8:
+        return few and few[1:]
+    tiled = _w4_tc(M, N, K, group, clusters_of)
+    return tiled[1:] if few is None or 2.5 + 1.3 * few[0] > tiled[0] else few[1:]
 
 
 @functools.lru_cache(None)
@@ -434,12 +444,12 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
     if code == 0 and not q8:
         return _gemm_by_16_bits(x, w, bias, out, accumulate)
     on = _clusters_on(here)
-    plan = w4_launch(q8, M, N, K, w.group, on) if q8 or M < W4_TC_TOKENS else None
-    if plan is not None:
+    plan = w4_launch(q8, M, N, K, w.group, on)
+    if plan is None:
+        raise KernelError(f"gemm_w4: rows of {K} columns are too long")
+    if len(plan) == 5:
         done = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales_at if q8 else None, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
                                 *plan, M, N, K, w.group, stream())
-    elif q8:
-        raise KernelError(f"gemm_w4: rows of {K} columns are too long")
     else:
         rows_fit = at % 16 == 0 and ld % 8 == 0 and ld >= K             # the kernels copy whole 16 bytes
         most = W4_TC_MOST_F32 * (2 if K > 2 * SUM_COLUMNS else 1) if f32 and K > SUM_COLUMNS else W4_TC_MOST
@@ -450,7 +460,7 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
             x[:, :K] = rows
             at, ld = x.data_ptr(), x.stride(0)
         done = _f("rf_gemm_w4_tc")(at, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
-                                   *w4_tc_launch(M, N, K, w.group, on), M, N, K, w.group, tc.status_word(w.packed.device).data_ptr(), stream())
+                                   *plan, M, N, K, w.group, tc.status_word(w.packed.device).data_ptr(), stream())
     check(done, "gemm_w4" if done == 0 else f"gemm_w4 ({M}x{N}x{K}, groups of {w.group})")
     return out
 

@@ -109,27 +109,23 @@ def clusters(splits):
 
 @pytest.mark.parametrize("q8", [True, False])
 @pytest.mark.parametrize("N,K", [(1, 1), (16, 64), (1003, 1100), (896, 896), (4608, 3584), (37888, 3584), (3584, 18944), (152064, 8192), (64, 70000)])
-def test_how_products_of_few_tokens_are_shared_out(q8, N, K):
-    """Every plan fits into shared memory, has a kernel, and its clusters run at once."""
+def test_how_products_are_shared_out(q8, N, K):
+    """Every plan fits into shared memory, has a kernel, and its clusters run at once; no block of a cluster is left without a stage."""
     from rocmforge_b200.kernels import quantized
     for group in (32, 64, 128):
-        for M in (1, 8, 9, 16) + ((17, 32, 33, 64, 200, 5000) if q8 else ()):
+        for M in (1, 8, 9, 16, 17, 32, 33, 64, 100, 128, 129, 200, 2000, 100000):
             plan = quantized.w4_launch(q8, M, N, K, group, clusters)
             if plan is None:
-                assert K == 70000 and not (q8 and M <= 8)
-                continue
-            eights, pair, ways, splits, used = plan
-            assert (q8, eights, pair) in quantized.W4_COST and ways in (1, 2, 4, 8, 16) and 1 <= splits <= 8
-            assert quantized._f("rf_gemm_w4_shared")(0 if q8 else 1, M, N, K, group, *plan) <= quantized.W4_MOST_SHARED
-            assert used >= 1 and (used == 1 or used * ((M + 8 * eights - 1) // (8 * eights)) <= clusters(splits))
-            assert eights * 8 >= min(M, 16) or K > 18944
-
-
-def test_how_products_on_the_tensor_cores_are_shared_out():
-    from rocmforge_b200.kernels import quantized
-    for M, N, K in ((17, 1, 1), (32, 37888, 3584), (64, 37888, 3584), (128, 37888, 3584), (192, 37888, 3584), (64, 3584, 18944), (2000, 3584, 18944), (100000, 64, 64)):
-        bn, splits = quantized.w4_tc_launch(M, N, K, 128, clusters)
-        assert bn in (32, 64, 128) and 1 <= splits <= 8
-        assert splits == 1 or splits <= (K + 511) // 512
-    assert quantized.w4_tc_launch(32, 37888, 3584, 128, clusters) == (32, 1)
-    assert quantized.w4_tc_launch(64, 3584, 18944, 128, clusters) == (64, 4)
+                assert q8 and K == 70000 and M > 8
+            elif len(plan) == 2:
+                bn, splits = plan
+                assert not q8 and (M > 8 or K == 70000) and bn in (32, 64, 128) and 1 <= splits <= min(8, (K + 511) // 512)
+            else:
+                eights, pair, ways, splits, used = plan
+                assert (q8, eights, pair) in quantized.W4_COST and ways in (1, 2, 4, 8, 16) and 1 <= splits <= 8 and (q8 or M <= 128)
+                assert quantized._f("rf_gemm_w4_shared")(0 if q8 else 1, M, N, K, group, *plan) <= quantized.W4_MOST_SHARED
+                assert used >= 1 and (used == 1 or used * ((M + 8 * eights - 1) // (8 * eights)) <= clusters(splits))
+                assert eights * 8 >= min(M, 16) or K > 18944
+    assert quantized.w4_launch(False, 16, 37888, 3584, 128, clusters) == (2, 1, 1, 1, 148)
+    assert quantized.w4_launch(False, 32, 37888, 3584, 128, clusters) == (32, 1)
+    assert quantized.w4_launch(False, 64, 3584, 18944, 128, clusters) == (64, 4)

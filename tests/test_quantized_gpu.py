@@ -189,9 +189,8 @@ def test_every_way_to_share_out_a_product(monkeypatch, M, eights, pair, ways, cl
     from rocmforge_b200 import kernels
     from rocmforge_b200.kernels import quantized
     if kind == "bf16" and eights == 4:
-        pytest.skip("more than sixteen 16-bit rows are the tensor cores' kernel's")
+        pytest.skip("there is no such kernel")
     monkeypatch.setattr(quantized, "w4_launch", lambda *a: (eights, pair, ways, splits, clusters))
-    monkeypatch.setattr(quantized, "W4_TC_TOKENS", 1000)
     x, x64, w, full = product_case(kind, M, N, K, G)
     x64, full = x64.to(DEV), full.to(DEV)
     h = numbers(M, N, seed=9)
@@ -210,8 +209,7 @@ def test_every_tile_on_the_tensor_cores(monkeypatch, M, bn, splits, N, K, G):
     """Tiles of tokens that are not full, rows of weights that end inside a tile, shares of the columns that are empty."""
     from rocmforge_b200 import kernels
     from rocmforge_b200.kernels import quantized
-    monkeypatch.setattr(quantized, "w4_tc_launch", lambda *a: (bn, splits))
-    monkeypatch.setattr(quantized, "W4_TC_TOKENS", 1)
+    monkeypatch.setattr(quantized, "w4_launch", lambda *a: (bn, splits))
     x, x64, w, full = product_case("bf16", M, N, K, G)
     x64, full = x64.to(DEV), full.to(DEV)
     b, h = numbers(N, seed=2), numbers(M, N, seed=9)
@@ -283,8 +281,11 @@ def test_a_row_does_not_depend_on_its_neighbours(kind):
     assert y[2].isnan().all() and torch.equal(y[[0, 1, 3, 4, 5, 6, 7]], whole[[0, 1, 3, 4, 5, 6, 7]])
 
 
-def test_a_row_does_not_depend_on_its_neighbours_on_the_tensor_cores():
+def test_a_row_does_not_depend_on_its_neighbours_on_the_tensor_cores(monkeypatch):
+    """... as long as the product is shared out in the same way, which goes by how many rows there are."""
     from rocmforge_b200 import kernels
+    from rocmforge_b200.kernels import quantized
+    monkeypatch.setattr(quantized, "w4_launch", lambda *a: (128, 3))
     w, _ = weight(300, 5000, 64)
     x = numbers(120, 5000, dt=BF).to(DEV)
     whole = kernels.gemm_w4(x, w, out_f32=True)
