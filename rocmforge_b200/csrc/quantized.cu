@@ -448,10 +448,8 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint
             for (int r = 0; r < RT; ++r) {
                 copy16(ask_to + r * W4_SLOT, pw[r], true);
                 copy16(ask_to + r * W4_SLOT + 512, second ? pw[r] + 32 : pw[r], second);
-                if (t < GROUPS) {
-                    const bool there = second || 2 * t < GROUPS;
-                    copy4(ask_to + r * W4_SLOT + scale_at, there ? ps[r] : w1, there);
-                }
+                const bool there = second || 2 * t < GROUPS;
+                copy4_if(ask_to + r * W4_SLOT + scale_at, there ? ps[r] : w1, there, t < GROUPS);
                 pw[r] += 64;
                 ps[r] += 8 * GROUPS;
             }
@@ -620,6 +618,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint
             continue;
         }
         if (splits > 1 && round > 0) {
+            __syncwarp();
             asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
             write_round(round - 1);
         }
@@ -639,6 +638,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint
                 }
         if (splits > 1) {
             // two sets of sums in turn: who writes a set for the second time knows, by the barrier between, that all have read the first
+            __syncwarp();                                // (the lanes wrote the round before in loops of different lengths)
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         } else {
             __syncthreads();
@@ -646,9 +646,11 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_product_kernel(const uint
         }
     }
     if (splits > 1) {
+        __syncwarp();
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         write_round(rounds - 1);
         // a CTA's shared memory stays until its peers have read it
+        __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
 }

@@ -15,6 +15,14 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there
 __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
+// ... by the lanes with `mine` alone (a predicate, no branch: the warp stays together for the matrix instructions behind it)
+__device__ __forceinline__ void copy4_if(uint32_t to, const void* from, bool there, bool mine) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %3, 0;\n\t"
+        "@p cp.async.ca.shared.global [%0], [%1], 4, %2;\n\t}"
+        ::"r"(to), "l"(from), "r"(there ? 4 : 0), "r"((uint32_t)mine) : "memory");
+}
 
 struct W4Out {
     void* out;               // [M, N] float32 if is_f32, else bfloat16; add: float32, added into

@@ -77,6 +77,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
+// An arrival of the lanes with `mine` (a predicate, no branch: the warp stays together for the reads and writes of tensor memory behind it).
+__device__ __forceinline__ void at_arrive_if(uint32_t bar, bool mine) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}"
+        ::"r"(bar), "r"((uint32_t)mine) : "memory");
+}
 __device__ __forceinline__ uint2 shared8(uint32_t at) {
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
@@ -127,7 +135,7 @@ __device__ __noinline__ bool add_piece(uint32_t tmem, uint32_t sum_full, int pie
     }
     tcgen05_fence_before();
     __syncwarp();
-    if ((threadIdx.x & 31) == 0) at_arrive(sum_full + 8 * (S::BUFS + buf));
+    at_arrive_if(sum_full + 8 * (S::BUFS + buf), (threadIdx.x & 31) == 0);
     return true;
 }
 
@@ -146,6 +154,7 @@ __device__ __noinline__ void write_16(uint32_t last_sum, uint32_t sum_before, bo
 #pragma unroll
         for (int j = 0; j < 16; ++j) old[j] = there && c + j < live ? reinterpret_cast<const float*>(o.out)[to + (size_t)j * o.N] : 0.f;
     }
+    __syncwarp();                                        // (rows that are not there have read nothing)
     tcgen05_wait_ld();
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -157,6 +166,7 @@ __device__ __noinline__ void write_16(uint32_t last_sum, uint32_t sum_before, bo
             else reinterpret_cast<__nv_bfloat16*>(o.out)[to + (size_t)j * o.N] = __float2bfloat16_rn(v + bias);
         }
     }
+    __syncwarp();                                        // (... nor written anything: the next sixteen tokens' reads need the whole warp)
 }
 
 template <int BN, int G>
@@ -299,7 +309,7 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
                 }
                 if (h == 1) {
                     __syncwarp();                        // all have read the stage
-                    if (lane == 0) at_arrive(bars + W_EMPTY + 8 * at);
+                    at_arrive_if(bars + W_EMPTY + 8 * at, lane == 0);
                 } else if (i > 0) {
                     const int before = number - S::PLACES;
                     ok = __all_sync(0xffffffffu, wait_for(bars + DONE + before % S::ROWS * 8, before / S::ROWS & 1, &abort_flag));
@@ -312,7 +322,7 @@ __global__ void __launch_bounds__(W4T_THREADS, 1) w4_tc_kernel(const __grid_cons
             tcgen05_wait_st();
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) at_arrive(bars + A_FULL + 8 * group);
+            at_arrive_if(bars + A_FULL + 8 * group, lane == 0);
         }
         for (; ok && summed < last; ++summed) ok = add_piece<BN, G>(tmem, bars + S_FULL, summed, &abort_flag);
     }
