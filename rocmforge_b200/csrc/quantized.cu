@@ -163,8 +163,8 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_q8_kernel(float* __restrict_
     pdl_trigger();
     __shared__ float red[34];
     const int r = blockIdx.x;
+    pdl_wait(pending, rows);                             // (rows may be what the kernel before has just chosen)
     const int t = rows ? min(max(rows[r], 0), n_h - 1) : r;             // (a row that is not there is never read)
-    pdl_wait(pending);
     float* hrow = h + (size_t)t * H;
     float v[NV][4];
     float ss = 0.f;

@@ -1,0 +1,35 @@
+"""Edges of the 4-bit weight path on the device, against plain forms in 64 bits."""
+import pytest
+import torch
+
+from test_quantized_gpu import BF, DEV, F32, check_rows, close, numbers, stands_for, weight
+
+pytestmark = pytest.mark.gpu
+
+
+def test_norm_of_rows_that_the_kernel_before_has_chosen():
+    """The rows' indices come from a kernel of this library launched right before (in a graph too, where its successor starts early)."""
+    from rocmforge_b200 import kernels
+    T, H, G = 64, 896, 64
+    h, w = numbers(T, H).to(DEV), torch.ones(H, device=DEV)
+    logits = torch.zeros(200, T, device=DEV)
+    ids = torch.zeros(200, dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        def body():
+            kernels.argmax(logits, out=ids)
+            return kernels.add_rmsnorm_q8(h, w, 1e-6, BF, G, rows=ids)
+        body()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = body()
+        x = h.cpu().double()
+        want = x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt()
+        for seed in (1, 2, 3):
+            logits.copy_(numbers(200, T, seed=seed))
+            graph.replay()
+            torch.cuda.synchronize()
+            check_rows(got, want[logits.cpu().argmax(-1)], 60 * 2.0 ** -24)
+            check_rows(body(), want[logits.cpu().argmax(-1)], 60 * 2.0 ** -24)
+    torch.cuda.current_stream().wait_stream(side)
