@@ -33,3 +33,19 @@ def test_norm_of_rows_that_the_kernel_before_has_chosen():
             check_rows(got, want[logits.cpu().argmax(-1)], 60 * 2.0 ** -24)
             check_rows(body(), want[logits.cpu().argmax(-1)], 60 * 2.0 ** -24)
     torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("T,I", [(3, 1), (40, 33), (40, 65), (9, 129), (5, 256)])
+def test_gelu_of_strongly_negative_gates(dt, G, T, I):
+    """Gates of -6 .. -4, where 1 + tanh has lost most of its bits: a group of nothing else gets its scale from values near 1e-8."""
+    from rocmforge_b200 import kernels
+    gu = numbers(T, 2 * I, spread=False)
+    gu[:, ::2] = -4 - 2 * torch.rand(T, I, generator=torch.Generator().manual_seed(I))
+    gu = gu.to(dt)
+    g, u = gu.double()[:, ::2], gu.double()[:, 1::2]
+    twice = 2 * (2 / torch.pi) ** 0.5 * (g + 0.044715 * g ** 3)
+    r = kernels.swiglu_q8(gu.to(DEV), G, activation="gelu_tanh")
+    # the exponent's argument, at most 25, is off by at most seven roundings; the exponential by two units, the sum, quotient and product by a rounding each
+    check_rows(r, g / (1 + torch.exp(-twice)) * u, (7 * 25 + 4 + 3) * 2.0 ** -24)
