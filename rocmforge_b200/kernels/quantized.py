@@ -453,7 +453,7 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
     else:
         rows_fit = at % 16 == 0 and ld % 8 == 0 and ld >= K             # the kernels copy whole 16 bytes
         most = W4_TC_MOST_F32 * (2 if K > 2 * SUM_COLUMNS else 1) if f32 and K > SUM_COLUMNS else W4_TC_MOST
-        if M > most and rows_fit and tc.supported(M, N, K, tc.STORE):
+        if M > most and rows_fit and out.data_ptr() % 16 == 0 and tc.supported(M, N, K, tc.STORE):      # (its results leave by TMA too)
             return _gemm_by_16_bits(x, w, bias, out, accumulate)
         if not rows_fit:                                 # (64 x 37,888 x 3,583 by rf_gemm_w4, which would take them: 100 us)
             x, rows = torch.empty(M, (K + 7) // 8 * 8, dtype=dt, device=x.device), x

@@ -49,3 +49,24 @@ def test_gelu_of_strongly_negative_gates(dt, G, T, I):
     r = kernels.swiglu_q8(gu.to(DEV), G, activation="gelu_tanh")
     # the exponent's argument, at most 25, is off by at most seven roundings; the exponential by two units, the sum, quotient and product by a rounding each
     check_rows(r, g / (1 + torch.exp(-twice)) * u, (7 * 25 + 4 + 3) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("off", [1, 2, 3, 5])
+@pytest.mark.parametrize("M,N,K", [(520, 256, 512), (2100, 1024, 2304), (1100, 384, 72), (40, 256, 512), (3, 256, 512)])
+def test_results_anywhere_in_memory(M, N, K, off):
+    """``out`` on the boundary of its type alone, whatever the number of tokens, and what lies beside it left alone."""
+    from rocmforge_b200 import kernels
+    w, full = weight(N, K, 64)
+    x = numbers(M, K, dt=BF).to(DEV)
+    full, x64 = full.to(DEV), x.double()
+    want, size, terms = x64 @ full.T, x64.abs() @ full.abs().T, 2 * K + 24
+    h = numbers(M, N, seed=9).to(DEV)
+    for dt, kw, more in ((BF, {}, 0), (F32, dict(out_f32=True), 0), (F32, dict(accumulate=True), 1)):
+        memory = torch.full((M * N + 16,), 7.0, dtype=dt, device=DEV)
+        out = memory[off:off + M * N].view(M, N)
+        if more:
+            out.copy_(h)
+        assert kernels.gemm_w4(x, w, out=out, **kw) is out
+        close(out, want + h.double() * more, size + h.double().abs() * more, terms + more, dt)
+        assert (memory[:off] == 7).all() and (memory[off + M * N:] == 7).all()
+    kernels.tensor_core.check_status(torch.device(DEV))
