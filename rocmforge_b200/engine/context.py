@@ -121,7 +121,7 @@ class StepContext:
         if isinstance(w, W4Weight):
             if not isinstance(x, Q8Rows) and self.q8_group(w) and x.shape[0] <= kernels.W4_FEW_TOKENS:
                 x = kernels.quantize_q8(x, w.group)
-            return kernels.gemm_w4(x, w, bias, **kw)
+            return kernels.gemm_w4(x, w, bias, tensor_cores=self.options.tensor_core_gemm, **kw)
         return kernels.gemm_plain(x, w, bias, tensor_cores=self.options.tensor_core_gemm, **kw)
 
     def matmul_rows_or_parts(self, x, w):

@@ -383,13 +383,13 @@ def _w4_tc(M: int, N: int, K: int, group: int, clusters_of):
 
 
 @functools.lru_cache(4096)
-def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of):
+def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of, tensor_cores: bool = True):
     """How a product is shared out, chosen from sizes alone: five numbers for ``rf_gemm_w4`` (``_w4_few``), two for ``rf_gemm_w4_tc``
     (``_w4_tc``), None where neither takes it.  16-bit rows go where less time is expected, ``rf_gemm_w4``'s cost being 1.3 us after 2.5
     (16 x 37,888 x 3,584: 21.5 us there, 28.6 on the tensor cores; 32: 38.9, 28.8; 32 x 4,608 x 3,584: 8.3, 9.5; 64: 12.5, 10.1; 32 x 896 x
-    4,864: 6.2, 6.7; 128: 10.7, 8.2).  Above 128 tokens only the tensor cores are looked at."""
-    few = _w4_few(q8, M, N, K, group, clusters_of) if q8 or M <= 128 else None
-    if q8:
+    4,864: 6.2, 6.7; 128: 10.7, 8.2).  Above 128 tokens only the tensor cores are looked at, without ``tensor_cores`` never."""
+    few = _w4_few(q8, M, N, K, group, clusters_of) if q8 or M <= 128 or not tensor_cores else None
+    if q8 or not tensor_cores:
         return few and few[1:]
     tiled = _w4_tc(M, N, K, group, clusters_of)
     return tiled[1:] if few is None or 2.5 + 1.3 * few[0] > tiled[0] else few[1:]
@@ -401,11 +401,12 @@ def _clusters_on(device: int):
 
 
 def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tensor | None = None, out_f32: bool = False,
-            accumulate: bool = False) -> torch.Tensor:
+            accumulate: bool = False, tensor_cores: bool = True) -> torch.Tensor:
     """y = x @ w.T (+ bias) with 4-bit weights, 32-bit sums.
 
     ``x``: ``Q8Rows`` of the weight's K and group (products inside a group are exact, in whole numbers), or a tensor [M, K] in bfloat16
-    or float32.  out_f32: the result is float32 whatever the rows; accumulate: added into ``out`` (float32)."""
+    or float32.  out_f32: the result is float32 whatever the rows; accumulate: added into ``out`` (float32); tensor_cores: whether the
+    tcgen05 kernels may take it (as in ``gemm_plain``)."""
     q8 = type(x) is Q8Rows
     if not (q8 or isinstance(x, torch.Tensor)) or type(w) is not W4Weight:
         raise KernelError("gemm_w4: x must be Q8Rows or a tensor, w a W4Weight")
@@ -442,10 +443,12 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
     if M == 0:
         return out
     if code == 0 and not q8:
-        return _gemm_by_16_bits(x, w, bias, out, accumulate)
+        return _gemm_by_wide_weights(x, w, bias, out, accumulate, tensor_cores)
     on = _clusters_on(here)
-    plan = w4_launch(q8, M, N, K, w.group, on)
+    plan = w4_launch(q8, M, N, K, w.group, on, tensor_cores)
     if plan is None:
+        if not q8:
+            return _gemm_by_wide_weights(x, w, bias, out, accumulate, tensor_cores)
         raise KernelError(f"gemm_w4: rows of {K} columns are too long")
     if len(plan) == 5:
         done = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales_at if q8 else None, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
@@ -454,7 +457,7 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
         rows_fit = at % 16 == 0 and ld % 8 == 0 and ld >= K             # the kernels copy whole 16 bytes
         most = W4_TC_MOST_F32 * (2 if K > 2 * SUM_COLUMNS else 1) if f32 and K > SUM_COLUMNS else W4_TC_MOST
         if M > most and rows_fit and out.data_ptr() % 16 == 0 and tc.supported(M, N, K, tc.STORE):      # (its results leave by TMA too)
-            return _gemm_by_16_bits(x, w, bias, out, accumulate)
+            return _gemm_by_wide_weights(x, w, bias, out, accumulate)
         if not rows_fit:                                 # (64 x 37,888 x 3,583 by rf_gemm_w4, which would take them: 100 us)
             x, rows = torch.empty(M, (K + 7) // 8 * 8, dtype=dt, device=x.device), x
             x[:, :K] = rows
@@ -465,12 +468,12 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
     return out
 
 
-def _gemm_by_16_bits(x, w, bias, out, accumulate):
+def _gemm_by_wide_weights(x, w, bias, out, accumulate, tensor_cores=True):
     """The product by the weights written out in the rows' dtype (exactly, with scales of five significant bits)."""
     from .basic import gemm_plain
     K = x.shape[1]
-    if x.dtype == torch.float32:
-        return gemm_plain(x, dequantize_w4(w, x.dtype), bias, out=out, accumulate=accumulate)
+    if x.dtype == torch.float32 or not tensor_cores:
+        return gemm_plain(x, dequantize_w4(w, x.dtype), bias, out=out, out_f32=out.dtype == torch.float32, accumulate=accumulate, tensor_cores=tensor_cores)
     m = tc.RESIDUAL if accumulate else tc.F32 if out.dtype == torch.float32 else tc.STORE
     pieces = 1 if m == tc.STORE else (K + SUM_COLUMNS - 1) // SUM_COLUMNS
     step = (K + 64 * pieces - 1) // (64 * pieces) * 64

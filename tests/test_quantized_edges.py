@@ -13,3 +13,20 @@ def test_chosen_rows_are_read_after_the_wait():
     """``add_rmsnorm_q8(rows=...)`` takes indices from anywhere, the kernel launched just before it among them."""
     body = body_of("add_rmsnorm_q8_kernel")
     assert body.index("pdl_wait(pending, rows)") < body.index("rows[")
+
+
+B200_CLUSTERS = (148, 74, 45, 33, 26, 22, 15, 15)         # of 1 .. 8 blocks that run at once
+
+
+def clusters(splits):
+    return B200_CLUSTERS[splits - 1]
+
+
+@pytest.mark.parametrize("M", [1, 17, 64, 129, 700, 5000])
+@pytest.mark.parametrize("N,K", [(16, 64), (37888, 3584), (3584, 18944), (64, 200000)])
+def test_plans_without_the_tcgen05_kernels(M, N, K):
+    from rocmforge_b200.kernels import quantized
+    plan = quantized.w4_launch(False, M, N, K, 64, clusters, False)
+    assert (plan is None) == (K == 200000) or len(plan) == 5
+    if plan is not None:
+        assert quantized._f("rf_gemm_w4_shared")(1, M, N, K, 64, *plan) <= quantized.W4_MOST_SHARED and (False, *plan[:2]) in quantized.W4_COST

@@ -70,3 +70,53 @@ def test_results_anywhere_in_memory(M, N, K, off):
         close(out, want + h.double() * more, size + h.double().abs() * more, terms + more, dt)
         assert (memory[:off] == 7).all() and (memory[off + M * N:] == 7).all()
     kernels.tensor_core.check_status(torch.device(DEV))
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """The names of the launchers that are called from here on."""
+    from rocmforge_b200.kernels import basic, latent, layernorm, quantized, tensor_core
+    names = []
+    for module in (basic, quantized, tensor_core):
+        for look in [n for n in ("_f", "_fc") if hasattr(module, n)]:
+            def spy(*a, real=getattr(module, look)):
+                names.extend(x for x in a if isinstance(x, str) and x.startswith("rf_"))
+                return real(*a)
+            monkeypatch.setattr(module, look, spy)
+    return names
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("M,N,K", [(1, 48, 100), (20, 300, 2176), (64, 4608, 896), (200, 130, 1100), (1030, 130, 2304), (3, 40, 70016)])
+def test_products_without_the_tcgen05_kernels(launched, dt, M, N, K):
+    from rocmforge_b200 import kernels
+    w, full = weight(N, K, 64)
+    x = numbers(M, K, dt=dt).to(DEV)
+    full, x64, b, h = full.to(DEV), x.double(), numbers(N, seed=2).to(DEV), numbers(M, N, seed=9).to(DEV)
+    want, size = x64 @ full.T + b.double(), x64.abs() @ full.abs().T + b.double().abs()
+    del launched[:]
+    close(kernels.gemm_w4(x, w, b, tensor_cores=False), want, size, 2 * K + 25, dt)
+    close(kernels.gemm_w4(x, w, b, out_f32=True, tensor_cores=False), want, size, 2 * K + 25, F32)
+    close(kernels.gemm_w4(x, w, b, out=h.clone(), accumulate=True, tensor_cores=False), want + h.double(), size + h.double().abs(), 2 * K + 26, F32)
+    assert launched and not [n for n in launched if "_tc" in n], launched
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("row_bits", [8, 16])
+def test_the_engine_without_the_tcgen05_kernels(folders, launched, dtype, row_bits):
+    """``Options(tensor_core_gemm=False)`` holds for products with 4-bit weights as well, in prompts of few and of many tokens and in single steps."""
+    import rocmforge_b200 as rf
+    from helpers import random_tokens
+    from test_quantized_engine_gpu import TORCH, assert_both_close, run_both
+    make = lambda on: rf.Model.from_folder(folders("D", dtype), dtype=TORCH[dtype],  # noqa: E731
+                                           options=rf.Options(weight_bits=4, weight_group=32, row_bits=row_bits, tensor_core_gemm=on, tcgen05_attention=on))
+    off, on = make(False), make(True)
+    for lens in ((5,), (17, 100), (600,)):
+        del launched[:]
+        prompts = [random_tokens(off.spec.vocab_size, n, n) for n in lens]
+        a, _ = run_both(off, off, prompts, off.spec.vocab_size)
+        # (32-bit rows that stay what they are go by the weights written out)
+        assert ("rf_dequantize_w4" if (dtype, row_bits) == ("float32", 16) else "rf_gemm_w4") in launched
+        assert not [n for n in launched if "_tc" in n and "attention" not in n], sorted(set(launched))
+        b, _ = run_both(on, on, prompts, on.spec.vocab_size)
+        assert_both_close(a, b, dtype, f"{dtype} {lens}")
