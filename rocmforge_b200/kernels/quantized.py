@@ -395,6 +395,12 @@ def w4_launch(q8: bool, M: int, N: int, K: int, group: int, clusters_of, tensor_
     return tiled[1:] if few is None or 2.5 + 1.3 * few[0] > tiled[0] else few[1:]
 
 
+def q8_rows_at_once(M: int, N: int, K: int, group: int, clusters_of):
+    """How many of ``M`` rows in 8 bits one launch takes: all, or where rows are so long that they do not lie in shared memory together
+    (100,000 columns and 32 rows, 140,000 and 8), the most of 16, 8, .. 1 that do; None where one does not (beyond 400,000)."""
+    return next((m for m in (M, 16, 8, 4, 2, 1) if m <= M and w4_launch(True, m, N, K, group, clusters_of)), None)
+
+
 @functools.lru_cache(None)
 def _clusters_on(device: int):
     return functools.partial(w4_clusters, device=device)
@@ -449,7 +455,13 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
     if plan is None:
         if not q8:
             return _gemm_by_wide_weights(x, w, bias, out, accumulate, tensor_cores)
-        raise KernelError(f"gemm_w4: rows of {K} columns are too long")
+        step = q8_rows_at_once(M, N, K, w.group, on)
+        if step is None:
+            raise KernelError(f"gemm_w4: rows of {K} columns are too long")
+        for lo in range(0, M, step):
+            rows = Q8Rows(x.q[lo:lo + step], x.scales[lo:lo + step], K, x.group, dt)
+            gemm_w4(rows, w, bias, out=out[lo:lo + step], out_f32=out_f32, accumulate=accumulate)
+        return out
     if len(plan) == 5:
         done = _f("rf_gemm_w4")(0 if q8 else 1, at, x.scales_at if q8 else None, ld, w.at, w.scales_at, bias_at, bias_f32, out.data_ptr(), f32, accumulate,
                                 *plan, M, N, K, w.group, stream())

@@ -30,3 +30,17 @@ def test_plans_without_the_tcgen05_kernels(M, N, K):
     assert (plan is None) == (K == 200000) or len(plan) == 5
     if plan is not None:
         assert quantized._f("rf_gemm_w4_shared")(1, M, N, K, 64, *plan) <= quantized.W4_MOST_SHARED and (False, *plan[:2]) in quantized.W4_COST
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_long_8_bit_rows_go_a_few_at_a_time(group):
+    """Rows that do not lie in shared memory together have a plan for fewer of them: as many as fit."""
+    from rocmforge_b200.kernels import quantized
+    whole = 0
+    for K in (18944, 70000, 100000, 140000, 300000, 400000):
+        for M in (1, 2, 8, 9, 32, 100):
+            step = quantized.q8_rows_at_once(M, 64, K, group, clusters)
+            assert step is not None and 1 <= step <= M and quantized.w4_launch(True, step, 64, K, group, clusters)
+            whole += step < M
+            assert step == M or quantized.w4_launch(True, M, 64, K, group, clusters) is None
+    assert whole > 0 and quantized.q8_rows_at_once(1, 64, 4000000, group, clusters) is None

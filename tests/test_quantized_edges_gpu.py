@@ -120,3 +120,16 @@ def test_the_engine_without_the_tcgen05_kernels(folders, launched, dtype, row_bi
         assert not [n for n in launched if "_tc" in n and "attention" not in n], sorted(set(launched))
         b, _ = run_both(on, on, prompts, on.spec.vocab_size)
         assert_both_close(a, b, dtype, f"{dtype} {lens}")
+
+
+@pytest.mark.parametrize("M,K,G", [(32, 100000, 32), (32, 100000, 64), (8, 140000, 32), (9, 140001, 64), (8, 140000, 128), (1, 300000, 128)])
+def test_long_8_bit_rows(M, K, G):
+    from rocmforge_b200 import kernels
+    N = 40
+    w, full = weight(N, K, G)
+    r = kernels.quantize_q8(numbers(M, K, dt=BF).to(DEV), G)
+    full, x64, b, h = full.to(DEV), stands_for(r).to(DEV), numbers(N, seed=2).to(DEV), numbers(M, N, seed=9).to(DEV)
+    want, size, terms = x64 @ full.T + b.double(), x64.abs() @ full.abs().T + b.double().abs(), K // 32 + 25
+    close(kernels.gemm_w4(r, w, b), want, size, terms, BF)
+    close(kernels.gemm_w4(r, w, b, out_f32=True), want, size, terms, F32)
+    close(kernels.gemm_w4(r, w, b, out=h.clone(), accumulate=True), want + h.double(), size + h.double().abs(), terms + 1, F32)
