@@ -14,7 +14,7 @@ from .latent import (streams_update, pair_embed, scale_, latent_write, latent_ga
                      attention_latent_prefill_supported, attention_latent_decode, attention_latent_decode_groups)
 from .basic import (silu_columns, row_norm_gate, moe_route_grouped, moe_sort_passive)
 from .quantized import (W4Weight, Q8Rows, quantize_w4, dequantize_w4, quantize_q8, add_rmsnorm_q8, swiglu_q8, gemm_w4, weights_made, W4_GROUPS,
-                        W4_FEW_TOKENS, W4_TC_MOST)
+                        W4_FEW_TOKENS, W4_NORM_MOST, W4_TC_MOST, padded_columns)
 from .layernorm import (stream_update, side_gate, RoutedSum, GatedRows)
 from ._ffi import launch_count
 from . import tensor_core

@@ -252,13 +252,17 @@ def quantize_q8(x: torch.Tensor, group: int = 128) -> Q8Rows:
     return y
 
 
+# Columns, padded, that a row of add_rmsnorm_q8 may have: a block keeps them in registers, 32 a thread.
+W4_NORM_MOST = 32768
+
+
 def add_rmsnorm_q8(h: torch.Tensor, weight: torch.Tensor, eps: float, compute_dtype: torch.dtype, group: int = 128,
                    pending: torch.Tensor | None = None, rows: torch.Tensor | None = None) -> Q8Rows:
     """``add_rmsnorm`` with its result in 8 bits: rmsnorm(h + pending) * weight, from 32 bits straight to groups of ``group`` columns.
 
     ``h`` [T, H] float32 is the residual stream; ``pending`` (None, a float32 stack [S, T, H] of partial sums, or a [T, H] tensor of the
     compute dtype or float32) is added into it in place.  With ``rows`` (int32 indices) only those rows are normalised and ``h`` is left
-    untouched."""
+    untouched.  H up to ``W4_NORM_MOST``."""
     _need_here("add_rmsnorm_q8", h, weight, pending, rows)
     _need_group(group, "add_rmsnorm_q8")
     need(h.dtype == torch.float32 and h.dim() == 2 and h.is_contiguous(), "add_rmsnorm_q8: h must be [T,H] float32")

@@ -59,8 +59,10 @@ class RMSNorm(Norm):
         return y
 
     def forward_q8(self, ctx, stream, group: int):
-        """The norm of all rows in 8 bits, groups of ``group`` (``kernels.Q8Rows``), unless whoever updated the stream has run it already."""
-        if stream.prepared is not None and stream.prepared[0] is self and stream.pending is None:
+        """The norm of all rows in 8 bits, groups of ``group`` (``kernels.Q8Rows``), unless whoever updated the stream has run it already or
+        rows are wider than that kernel takes (the product that reads them then makes 8 bits of them)."""
+        if (stream.prepared is not None and stream.prepared[0] is self and stream.pending is None
+                or kernels.padded_columns(self.size, group) > kernels.W4_NORM_MOST):
             return self.forward(ctx, stream)
         stream.prepared = None
         y = kernels.add_rmsnorm_q8(stream.h, self.weight, self.eps, self.compute_dtype, group, pending=stream.pending)

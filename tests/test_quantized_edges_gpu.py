@@ -133,3 +133,26 @@ def test_long_8_bit_rows(M, K, G):
     close(kernels.gemm_w4(r, w, b), want, size, terms, BF)
     close(kernels.gemm_w4(r, w, b, out_f32=True), want, size, terms, F32)
     close(kernels.gemm_w4(r, w, b, out=h.clone(), accumulate=True), want + h.double(), size + h.double().abs(), terms + 1, F32)
+
+
+@pytest.mark.parametrize("H", [32768, 32769, 40000])
+def test_a_wide_norm_hands_on_what_it_can(H):
+    """The 8-bit norm takes 32,768 columns; a part with more gets the norm's ordinary rows, and its product makes 8 bits of them."""
+    from rocmforge_b200 import kernels
+    from rocmforge_b200.engine.stream import ResidualStream
+    from rocmforge_b200.parts.norm import RMSNorm
+    norm = RMSNorm(H, 1e-6)
+    norm.bind({"weight": torch.ones(H, device=DEV)}, BF)
+    h, p = numbers(3, H), numbers(2, 3, H, seed=4)
+    stream = ResidualStream(h.to(DEV))
+    stream.add_pending(p.to(DEV))
+    y = norm.forward_q8(None, stream, 64)
+    new = h + p[0] + p[1]
+    assert stream.pending is None and torch.equal(stream.h.cpu(), new)
+    x = new.double()
+    want = x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt()
+    if H <= 32768:
+        check_rows(y, want, 60 * 2.0 ** -24)
+    else:
+        assert y.dtype == BF and ((y.cpu().double() - want).abs() <= (2.0 ** -8 + 60 * 2.0 ** -24) * want.abs()).all()
+        check_rows(kernels.quantize_q8(y, 64), y.cpu().double(), 0)
