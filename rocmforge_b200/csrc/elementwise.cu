@@ -628,6 +628,37 @@ __global__ void swiglu_kernel(const T* __restrict__ gu, T* __restrict__ a, size_
     }
 }
 
+// The same from 32-bit sums, rounded once, to bfloat16 (ACT 3: the unit with clamped halves): gate and up lie beside each other, so the numbers
+// of the result lie where the pairs do and rows do not matter.  VEC: four results a thread, on boundaries of their size.  gelu by tanh as
+// g / (1 + exp(-2 u)), which keeps its bits where a gate is far below zero.  128 x 18,944 4.9 us, 5.0 TB/s, 512 15.2, 6.4 TB/s (swiglu_kernel
+// from bfloat16 9.3 and 32.5: a 64-bit division for every number); 1 x 18,944 1.3: a launch.
+template <int ACT, bool VEC>
+__global__ void __launch_bounds__(256) gated_round_kernel(const float* gu, __nv_bfloat16* __restrict__ a, size_t n, float limit, float alpha) {
+    pdl_trigger();
+    pdl_wait(gu);
+    auto unit = [&](float g, float u) {
+        if constexpr (ACT == 0) return g / (1.f + expf(-g)) * u;
+        else if constexpr (ACT == 1) return fmaxf(g, 0.f) * u;
+        else if constexpr (ACT == 2) return g / (1.f + expf(-1.5957691216057308f * (g + 0.044715f * g * g * g))) * u;
+        else {
+            g = fminf(g, limit);
+            u = fminf(fmaxf(u, -limit), limit);
+            return g / (1.f + expf(-alpha * g)) * (u + 1.f);
+        }
+    };
+    const size_t step = (size_t)gridDim.x * blockDim.x;
+    size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if constexpr (VEC) {
+        for (; i < n / 4; i += step) {
+            const float4 x = reinterpret_cast<const float4*>(gu)[2 * i], y = reinterpret_cast<const float4*>(gu)[2 * i + 1];
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(unit(x.x, x.y), unit(x.z, x.w)), hi = __floats2bfloat162_rn(unit(y.x, y.y), unit(y.z, y.w));
+            reinterpret_cast<uint2*>(a)[i] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        }
+    } else {
+        for (; i < n; i += step) a[i] = __float2bfloat16_rn(unit(gu[2 * i], gu[2 * i + 1]));
+    }
+}
+
 // ---------------------------------------------------------------- squared ReLU
 // a = max(x, 0)^2, evaluated in 32-bit.
 template <typename T>
@@ -1525,6 +1556,17 @@ static int launch_swiglu(const void* gu, void* a, int T_, int I, cudaStream_t st
 }
 
 
+template <int ACT>
+static int launch_gated_round(const float* gu, __nv_bfloat16* a, size_t n, float limit, float alpha, cudaStream_t st) {
+    const bool vec = n % 4 == 0 && !(reinterpret_cast<uintptr_t>(gu) & 15) && !(reinterpret_cast<uintptr_t>(a) & 7);
+    const size_t threads = vec ? n / 4 : n, want = (threads + 255) / 256;
+    const dim3 grid((unsigned)(want < 148 * 16 ? want : 148 * 16));
+    if (vec) rf_launch(gated_round_kernel<ACT, true>, grid, dim3(256), 0, st, gu, a, n, limit, alpha);
+    else rf_launch(gated_round_kernel<ACT, false>, grid, dim3(256), 0, st, gu, a, n, limit, alpha);
+    RF_LAUNCH_CHECK();
+    return 0;
+}
+
 template <typename T>
 static int launch_relu2(const void* x, void* a, long long n, cudaStream_t st) {
     if (n <= 0) return 0;
@@ -1663,6 +1705,16 @@ int rf_reglu(int dtype, const void* gu, void* a, int T_, int I, cudaStream_t st)
 }
 int rf_geglu(int dtype, const void* gu, void* a, int T_, int I, cudaStream_t st) {
     return dtype == 0 ? launch_swiglu<float, 2>(gu, a, T_, I, st) : launch_swiglu<__nv_bfloat16, 2>(gu, a, T_, I, st);
+}
+// gu float32 [T, 2 I] -> a bfloat16 [T, I]; act 0: silu, 1: relu, 2: gelu by tanh, 3: clamped halves (limit, alpha)
+int rf_gated_round(int act, const void* gu, void* a, int T_, int I, float limit, float alpha, cudaStream_t st) {
+    if (T_ < 0 || I < 0 || act < 0 || act > 3) return RF_ERR_BAD_ARG;
+    const size_t n = (size_t)T_ * I;
+    if (n == 0) return 0;
+    const float* x = (const float*)gu;
+    __nv_bfloat16* y = (__nv_bfloat16*)a;
+    return act == 0 ? launch_gated_round<0>(x, y, n, limit, alpha, st) : act == 1 ? launch_gated_round<1>(x, y, n, limit, alpha, st)
+         : act == 2 ? launch_gated_round<2>(x, y, n, limit, alpha, st) : launch_gated_round<3>(x, y, n, limit, alpha, st);
 }
 int rf_relu2(int dtype, const void* x, void* a, long long n, cudaStream_t st) {
     return dtype == 0 ? launch_relu2<float>(x, a, n, st) : launch_relu2<__nv_bfloat16>(x, a, n, st);

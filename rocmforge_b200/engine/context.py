@@ -202,11 +202,13 @@ class StepContext:
         w = gate_up.weight
         if isinstance(w, W4Weight):
             if y.shape[0] <= kernels.W4_TC_MOST or self.compute_dtype != torch.bfloat16:
-                gu = self.matmul(y, w, gate_up.bias)
+                # (32-bit sums, as the 16-bit product's epilogue has them: the unit is rounded once)
+                gu = self.matmul(y, w, gate_up.bias, out_f32=True)
                 if activation == "clamped_glu":
-                    return kernels.clamped_glu(gu, limit, alpha)
+                    return kernels.clamped_glu(gu, limit, alpha, dtype=self.compute_dtype)
                 group = self.q8_group(reader)
-                return kernels.swiglu_q8(gu, group, activation) if group else kernels.swiglu(gu, activation=activation)
+                return (kernels.swiglu_q8(gu, group, activation, dtype=self.compute_dtype) if group
+                        else kernels.swiglu(gu, activation=activation, dtype=self.compute_dtype))
             w = kernels.dequantize_w4(w, self.compute_dtype)         # many tokens: the 16-bit product with the unit in its epilogue
         mode = {"silu": tc.SWIGLU, "relu": tc.REGLU, "gelu_tanh": tc.GEGLU, "clamped_glu": tc.CLAMPGLU}[activation]
         glu = dict(limit=limit, alpha=alpha) if mode == tc.CLAMPGLU else {}

@@ -72,14 +72,18 @@ def round_rows(h: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
-def clamped_glu(gu: torch.Tensor, limit: float, alpha: float, row_scale: torch.Tensor | None = None) -> torch.Tensor:
+def clamped_glu(gu: torch.Tensor, limit: float, alpha: float, row_scale: torch.Tensor | None = None,
+                dtype: torch.dtype | None = None) -> torch.Tensor:
     """a[t, j] = g sigmoid(alpha g) (u + 1) with g = min(s gu[t, 2j], limit), u = clamp(s gu[t, 2j+1], -limit, limit) and
-    s = row_scale[t] (float32 [T]; 1 without), evaluated in 32-bit."""
+    s = row_scale[t] (float32 [T]; 1 without), evaluated in 32-bit.  ``dtype``: as for ``swiglu``."""
     need_cuda(gu, row_scale)
     need(gu.dim() == 2 and gu.is_contiguous() and gu.shape[1] % 2 == 0, "clamped_glu: input must be [T, 2I]")
     T, I2 = gu.shape
     need(row_scale is None or (row_scale.dtype == torch.float32 and row_scale.numel() >= T and row_scale.is_contiguous()),
          "clamped_glu: row_scale must be float32 [T]")
+    if dtype is not None and dtype != gu.dtype:
+        need(row_scale is None, "clamped_glu: row_scale does not go with another dtype")
+        return _gated_round(gu, 3, dtype, "clamped_glu", float(limit), float(alpha))
     out = torch.empty((T, I2 // 2), dtype=gu.dtype, device=gu.device)
     f = _f("elementwise", "rf_clamped_glu", c_int, c_void_p, c_void_p, c_int, c_int, c_float, c_float, c_void_p, c_void_p)
     check(f(dtype_code(gu.dtype), ptr(gu), ptr(out), T, I2 // 2, float(limit), float(alpha), ptr(row_scale), stream()), "clamped_glu")
@@ -204,16 +208,29 @@ def rope_kv_write(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: in
 _GATED_UNITS = {"silu": "rf_swiglu", "relu": "rf_reglu", "gelu_tanh": "rf_geglu"}
 
 
-def swiglu(gu: torch.Tensor, out: torch.Tensor | None = None, activation: str = "silu") -> torch.Tensor:
-    """a[t, j] = silu(gu[t, 2j]) * gu[t, 2j+1] (``activation`` "relu", "gelu_tanh": that function instead of silu)."""
+def swiglu(gu: torch.Tensor, out: torch.Tensor | None = None, activation: str = "silu", dtype: torch.dtype | None = None) -> torch.Tensor:
+    """a[t, j] = silu(gu[t, 2j]) * gu[t, 2j+1] (``activation`` "relu", "gelu_tanh": that function instead of silu).  ``dtype``: of the
+    result, where it is not gu's: bfloat16 from float32, rounded once."""
     need(activation in _GATED_UNITS, f"swiglu: activation {activation!r} (known: {sorted(_GATED_UNITS)})")
     need_cuda(gu)
     need(gu.dim() == 2 and gu.is_contiguous() and gu.shape[1] % 2 == 0, "swiglu: input must be [T, 2I]")
     T, I2 = gu.shape
+    if dtype is not None and dtype != gu.dtype:
+        need(out is None, "swiglu: out does not go with another dtype")
+        return _gated_round(gu, list(_GATED_UNITS).index(activation), dtype, "swiglu")
     if out is None:
         out = torch.empty((T, I2 // 2), dtype=gu.dtype, device=gu.device)
     f = _f("elementwise", _GATED_UNITS[activation], c_int, c_void_p, c_void_p, c_int, c_int, c_void_p)
     check(f(dtype_code(gu.dtype), ptr(gu), ptr(out), T, I2 // 2, stream()), "swiglu")
+    return out
+
+
+def _gated_round(gu, act, dtype, what, limit=0.0, alpha=0.0):
+    need(gu.dtype == torch.float32 and dtype == torch.bfloat16, f"{what}: from {gu.dtype} to {dtype} (known: from float32 to bfloat16)")
+    T, I2 = gu.shape
+    out = torch.empty((T, I2 // 2), dtype=dtype, device=gu.device)
+    f = _f("elementwise", "rf_gated_round", c_int, c_void_p, c_void_p, c_int, c_int, c_float, c_float, c_void_p)
+    check(f(act, ptr(gu), ptr(out), T, I2 // 2, limit, alpha, stream()), what)
     return out
 
 

@@ -295,8 +295,9 @@ def add_rmsnorm_q8(h: torch.Tensor, weight: torch.Tensor, eps: float, compute_dt
 _ACTIVATIONS = {"silu": 0, "relu": 1, "gelu_tanh": 2}
 
 
-def swiglu_q8(gu: torch.Tensor, group: int = 128, activation: str = "silu") -> Q8Rows:
-    """``swiglu`` with its result in 8 bits: act(gu[t, 2j]) * gu[t, 2j+1], from 32 bits straight to groups of ``group`` columns."""
+def swiglu_q8(gu: torch.Tensor, group: int = 128, activation: str = "silu", dtype: torch.dtype | None = None) -> Q8Rows:
+    """``swiglu`` with its result in 8 bits: act(gu[t, 2j]) * gu[t, 2j+1], from 32 bits straight to groups of ``group`` columns.  ``dtype``:
+    that of the rows they stand for, where it is not gu's.  (A gate that is no number counts as 0 for "relu", as in ``swiglu``.)"""
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise KernelError(f"swiglu_q8: activation {activation!r} (known: {sorted(_ACTIVATIONS)})")
@@ -304,8 +305,9 @@ def swiglu_q8(gu: torch.Tensor, group: int = 128, activation: str = "silu") -> Q
     _need_group(group, "swiglu_q8")
     need(gu.dim() == 2 and gu.is_contiguous() and gu.shape[1] % 2 == 0 and gu.shape[1] > 0, "swiglu_q8: input must be [T, 2I]")
     T, I = gu.shape[0], gu.shape[1] // 2
-    code = dtype_code(gu.dtype)
-    y = Q8Rows.empty(T, I, group, gu.dtype, gu.device)
+    code, dtype = dtype_code(gu.dtype), dtype or gu.dtype
+    dtype_code(dtype)
+    y = Q8Rows.empty(T, I, group, dtype, gu.device)
     check(_f("rf_swiglu_q8")(code, gu.data_ptr(), act, y.at, y.scales_at, T, I, group, stream()), "swiglu_q8")
     return y
 

@@ -156,3 +156,75 @@ def test_a_wide_norm_hands_on_what_it_can(H):
     else:
         assert y.dtype == BF and ((y.cpu().double() - want).abs() <= (2.0 ** -8 + 60 * 2.0 ** -24) * want.abs()).all()
         check_rows(kernels.quantize_q8(y, 64), y.cpu().double(), 0)
+
+
+def step_context(T, dtype, **options):
+    """A StepContext as far as products and gated units look at it."""
+    from rocmforge_b200.engine.context import Options, StepContext
+    ctx = object.__new__(StepContext)
+    ctx.options, ctx.compute_dtype, ctx.T = Options(weight_bits=4, **options), dtype, T
+    return ctx
+
+
+def unit(activation, g, u):
+    if activation == "clamped_glu":
+        g, u = g.clamp_max(3), u.clamp(-3, 3)
+        return g * torch.sigmoid(1.702 * g) * (u + 1)
+    return dict(silu=lambda: g * torch.sigmoid(g), relu=lambda: g.clamp_min(0),
+                gelu_tanh=lambda: g / (1 + torch.exp(-2 * (2 / torch.pi) ** 0.5 * (g + 0.044715 * g ** 3))))[activation]() * u
+
+
+@pytest.mark.parametrize("row_bits", [8, 16])
+@pytest.mark.parametrize("activation", ["silu", "relu", "gelu_tanh", "clamped_glu"])
+@pytest.mark.parametrize("T", [1, 5, 32, 40, 300, 600])
+def test_the_unit_is_formed_from_32_bit_sums(T, activation, row_bits):
+    """Gate and up are whole numbers of 2^-10, exact in 32 bits and not in 16; the unit of them is rounded once, to the rows' dtype or to 8 bits."""
+    from rocmforge_b200 import kernels
+    from rocmforge_b200.parts.linear import Linear
+    K, I, G = 256, 136, 64
+    gen = torch.Generator().manual_seed(T)
+    q = torch.randint(-8, 8, (2 * I, K), generator=gen, dtype=torch.int8)
+    w = kernels.W4Weight.from_quantized(q.to(DEV), torch.full((2 * I, K // G), 2.0 ** -10, device=DEV), G)
+    x = torch.randint(-8, 9, (T, K), generator=gen).to(BF).to(DEV)
+    gu = (x.double() @ q.to(DEV).double().T / 1024).cpu()
+    want = unit(activation, gu[:, ::2], gu[:, 1::2])
+    linear = object.__new__(Linear)
+    linear.weight, linear.bias, linear.N, linear.K = w, None, 2 * I, K
+    ctx = step_context(T, BF, row_bits=row_bits)
+    # whole numbers in 8 bits: the scale of a group is its largest / 127, so the rows are made by hand
+    y = x
+    if row_bits == 8 and T <= 32:
+        full = torch.zeros(T, K, dtype=torch.int8, device=DEV)
+        full[:] = x.to(torch.int8)
+        y = kernels.Q8Rows(full, torch.ones(T, K // G, device=DEV), K, G, BF)
+    kw = dict(limit=3.0, alpha=1.702) if activation == "clamped_glu" else {}
+    got = ctx.gated_activation(y, linear, activation, reader=w, **kw)
+    assert got.dtype == BF and tuple(got.shape) == (T, I)
+    # the unit in 32 bits: an argument of at most 25 off by seven roundings, an exponential by two units, three more roundings; 1 + u rounds as well
+    rel = (7 * 25 + 8) * 2.0 ** -24
+    if isinstance(got, kernels.Q8Rows):
+        check_rows(got, want, rel)
+    else:
+        got = got.cpu().double()
+        bound = (2.0 ** -8 + 2 * rel) * want.abs() + 1e-30
+        assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("activation", ["silu", "relu", "gelu_tanh", "clamped_glu"])
+@pytest.mark.parametrize("T,I,off", [(0, 8, 0), (1, 1, 0), (3, 101, 0), (7, 64, 1), (130, 1000, 2), (700, 640, 0)])
+def test_units_of_32_bit_sums_rounded_once(activation, T, I, off):
+    """``swiglu`` and ``clamped_glu`` with a result in bfloat16 from float32, on any boundary."""
+    from rocmforge_b200 import kernels
+    memory = torch.zeros(2 * T * I + 4, device=DEV)
+    gu = memory[off:off + 2 * T * I].view(T, 2 * I)
+    gu.copy_(2 * numbers(T, 2 * I, spread=False))
+    want = unit(activation, gu.cpu().double()[:, ::2], gu.cpu().double()[:, 1::2])
+    got = (kernels.clamped_glu(gu, 3.0, 1.702, dtype=BF) if activation == "clamped_glu" else kernels.swiglu(gu, activation=activation, dtype=BF))
+    assert got.dtype == BF and got.shape == (T, I)
+    # the exponential's argument: seven roundings of at most 80 where the exponential is not yet 2^-110 (what is left there is below 2^-100)
+    bound = (2.0 ** -8 + (7 * 80 + 8) * 2.0 ** -24) * want.abs() + 2.0 ** -100
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+    with pytest.raises(kernels.KernelError):
+        kernels.swiglu(gu.to(BF), dtype=F32)
+    with pytest.raises(kernels.KernelError):
+        kernels.clamped_glu(gu.to(BF), 3.0, 1.0, dtype=F32)
