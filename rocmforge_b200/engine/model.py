@@ -125,18 +125,20 @@ class Model:
             raise RuntimeError("rocmforge_b200 models run on a CUDA device only (there is no CPU fallback)")
         self.options = options or Options()
         build.ensure_built(spec.cuda_modules(compute_dtype) + (["quantized", "quantized_tc"] if self.options.weight_bits == 4 else []))
+        self.weight_bytes = sum(t.nbytes for t in {t.data_ptr(): t for t in params.values()}.values())
         for prefix, part in spec.named_parts().items():
-            local = {name[len(prefix):]: t for name, t in params.items()
-                     if name.startswith(prefix) and name[len(prefix):] in part.param_specs()}
+            specs = part.param_specs()
+            local = {name[len(prefix):]: t for name, t in params.items() if name.startswith(prefix) and name[len(prefix):] in specs}
             part.bind(local, compute_dtype)
+            if part.linears():                           # (a fused weight may hold rows of zeros that no tensor has)
+                self.weight_bytes += (sum(linear.weight.nbytes for linear in part.linears())
+                                      - sum(t.nbytes for name, t in local.items() if specs[name].kind == "matrix"))
         self._tables = {}                  # name -> builder of a host table that a part wants with every step
         for part in spec.named_parts().values():
             for name in part.step_table_names():
                 self._tables.setdefault(name, (lambda batch, part=part, name=name: part.step_table(name, batch)))
         self._desc = DeviceDescriptor(self.device)
         self._scratch: Dict[tuple, torch.Tensor] = {}
-        self.weight_bytes = sum(t.numel() * t.element_size()
-                                for t in {t.data_ptr(): t for t in params.values()}.values())
         if self.options.weight_bits == 4:
             with torch.cuda.device(self.device):
                 for part in spec.named_parts().values():

@@ -228,3 +228,25 @@ def test_units_of_32_bit_sums_rounded_once(activation, T, I, off):
         kernels.swiglu(gu.to(BF), dtype=F32)
     with pytest.raises(kernels.KernelError):
         kernels.clamped_glu(gu.to(BF), 3.0, 1.0, dtype=F32)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["D", "FA", "FC", "FD", "RA"])
+def test_weight_bytes_are_what_the_products_hold(folders, name, dtype):
+    """Zero rows that a part adds to a fused weight lie on the device too, in 16 bits as in 4 (FA, FC and FD have some)."""
+    import rocmforge_b200 as rf
+    from rocmforge_b200 import kernels
+    from rocmforge_b200.weights.loader import load_folder
+    from test_quantized_engine_gpu import TORCH
+    for bits in (16, 4):
+        m = rf.Model.from_folder(folders(name, dtype), dtype=TORCH[dtype], options=rf.Options(weight_bits=bits, weight_group=32))
+        params = load_folder(folders(name, dtype), m.spec.param_specs(), TORCH[dtype], "cpu")
+        others, held = {}, 0                             # (tied tensors count once)
+        for prefix, part in m.spec.named_parts().items():
+            for local, spec in part.param_specs().items():
+                if not (part.linears() and spec.kind == "matrix") and prefix + local in params:
+                    others[params[prefix + local].data_ptr()] = params[prefix + local].nbytes
+            for linear in part.linears():
+                assert isinstance(linear.weight, kernels.W4Weight) == (bits == 4)
+                held += linear.weight.nbytes
+        assert m.weight_bytes == held + sum(others.values())
