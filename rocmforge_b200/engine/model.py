@@ -9,6 +9,7 @@ earlier from the cache, and returns float32 logits for the wanted rows.
 """
 from __future__ import annotations
 
+from collections import Counter
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence
 
@@ -126,24 +127,36 @@ class Model:
         self.options = options or Options()
         build.ensure_built(spec.cuda_modules(compute_dtype) + (["quantized", "quantized_tc"] if self.options.weight_bits == 4 else []))
         self.weight_bytes = sum(t.nbytes for t in {t.data_ptr(): t for t in params.values()}.values())
+        # 4 bits: part after part (``params`` may lie on the host), so that the weights are never on the device in 16 bits all at once
+        names, moved = Counter((t.data_ptr(), t.shape) for t in params.values()), {}
         for prefix, part in spec.named_parts().items():
             specs = part.param_specs()
-            local = {name[len(prefix):]: t for name, t in params.items() if name.startswith(prefix) and name[len(prefix):] in specs}
+            local = {name[len(prefix):]: self._here(t, names, moved) for name, t in params.items()
+                     if name.startswith(prefix) and name[len(prefix):] in specs}
             part.bind(local, compute_dtype)
             if part.linears():                           # (a fused weight may hold rows of zeros that no tensor has)
                 self.weight_bytes += (sum(linear.weight.nbytes for linear in part.linears())
                                       - sum(t.nbytes for name, t in local.items() if specs[name].kind == "matrix"))
+            del local
+            if self.options.weight_bits == 4:
+                with torch.cuda.device(self.device):
+                    for linear in part.linears():
+                        self.weight_bytes -= linear.to_4_bits(self.options.weight_group)
         self._tables = {}                  # name -> builder of a host table that a part wants with every step
         for part in spec.named_parts().values():
             for name in part.step_table_names():
                 self._tables.setdefault(name, (lambda batch, part=part, name=name: part.step_table(name, batch)))
         self._desc = DeviceDescriptor(self.device)
         self._scratch: Dict[tuple, torch.Tensor] = {}
-        if self.options.weight_bits == 4:
-            with torch.cuda.device(self.device):
-                for part in spec.named_parts().values():
-                    for linear in part.linears():
-                        self.weight_bytes -= linear.to_4_bits(self.options.weight_group)
+
+    def _here(self, t: torch.Tensor, names: Counter, moved: Dict[tuple, torch.Tensor]) -> torch.Tensor:
+        """``t`` on the model's device; what several names share is moved once."""
+        key = (t.data_ptr(), t.shape)
+        if names[key] == 1:
+            return t.to(self.device)
+        if key not in moved:
+            moved[key] = t.to(self.device)
+        return moved[key]
 
     # ---------------------------------------------------------------- construction
     @classmethod
@@ -151,7 +164,8 @@ class Model:
         from ..config import load_config
         arch, config = load_config(folder)
         spec = arch.build(config)
-        params = load_folder(folder, spec.param_specs(), dtype, device)
+        few = options is not None and options.weight_bits == 4         # (the model moves them as it makes 4 bits of them)
+        params = load_folder(folder, spec.param_specs(), dtype, "cpu" if few else device)
         return cls(spec, params, dtype, device, options)
 
     @classmethod

@@ -250,3 +250,26 @@ def test_weight_bytes_are_what_the_products_hold(folders, name, dtype):
                 assert isinstance(linear.weight, kernels.W4Weight) == (bits == 4)
                 held += linear.weight.nbytes
         assert m.weight_bytes == held + sum(others.values())
+
+
+@pytest.mark.parametrize("tied", [False, True])
+def test_a_model_in_4_bits_never_lies_on_the_device_in_16(tmp_path, tied):
+    """Loaded part after part: the most memory that is held at once is the 4-bit model and one part in 16 bits (with its fused copy)."""
+    import rocmforge_b200 as rf
+    from helpers import CONFIGS, write_tiny
+    cfg = dict(CONFIGS["D"], num_hidden_layers=12, hidden_size=512, intermediate_size=2048, num_attention_heads=8, num_key_value_heads=2, head_dim=64,
+               tie_word_embeddings=tied)
+    write_tiny(cfg, str(tmp_path), "bfloat16")
+    make = lambda bits: rf.Model.from_folder(str(tmp_path), options=rf.Options(weight_bits=bits))  # noqa: E731
+    sixteen = make(16).weight_bytes
+    m = make(4)                                          # (everything is built and allocated that stays)
+    m.new_cache(max_tokens=64)
+    four = m.weight_bytes
+    del m
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    m = make(4)
+    held, peak = torch.cuda.memory_allocated() - before, torch.cuda.max_memory_allocated() - before
+    part = 2 * 3 * 512 * 2048                            # the feed-forward, the largest part: its tensors, two of them fused once more
+    assert four <= held <= four + 2 ** 20 and peak <= four + 2 * part + 2 ** 20 and peak < 0.6 * sixteen
