@@ -44,3 +44,26 @@ def test_long_8_bit_rows_go_a_few_at_a_time(group):
             whole += step < M
             assert step == M or quantized.w4_launch(True, M, 64, K, group, clusters) is None
     assert whole > 0 and quantized.q8_rows_at_once(1, 64, 4000000, group, clusters) is None
+
+
+@pytest.mark.parametrize("name,parts", [("RA", {"GQAAttention", "SquaredReluMLP"}), ("RB", {"GQAAttention", "SquaredReluMLP"}), ("FA", {"GQAAttention", "GatedMLP"}),
+                                        ("VA", {"GQAAttention"}), ("GA", {"GatedMLP"}), ("DC", {"GQAAttention", "GatedMLP"})])
+def test_products_of_every_kind_of_part(folders, name, parts):
+    """Which products the parts of other designs offer for 4 bits, bound: all that their matrices go into, the one that alone reads the input first."""
+    from rocmforge_b200.config import load_config
+    from rocmforge_b200.weights import load_folder
+    folder = folders(name, "bfloat16")
+    arch, config = load_config(folder)
+    spec = arch.build(config)
+    params, offering = load_folder(folder, spec.param_specs(), torch.bfloat16, "cpu"), set()
+    for prefix, part in spec.named_parts().items():
+        specs = part.param_specs()
+        if type(part).__name__ not in parts:
+            continue
+        part.bind({k[len(prefix):]: t for k, t in params.items() if k.startswith(prefix) and k[len(prefix):] in specs}, torch.bfloat16)
+        offering.add(type(part).__name__)
+        linears = part.linears()
+        matrices = [s for s in specs.values() if s.kind == "matrix"]
+        assert len(linears) == 2 and part.input_weight() is linears[0].weight
+        assert sum(a.weight.numel() for a in linears) >= sum(s.shape[0] * s.shape[1] for s in matrices) and linears[0].K == part.hidden == linears[1].N
+    assert offering == parts

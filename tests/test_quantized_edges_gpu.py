@@ -273,3 +273,103 @@ def test_a_model_in_4_bits_never_lies_on_the_device_in_16(tmp_path, tied):
     held, peak = torch.cuda.memory_allocated() - before, torch.cuda.max_memory_allocated() - before
     part = 2 * 3 * 512 * 2048                            # the feed-forward, the largest part: its tensors, two of them fused once more
     assert four <= held <= four + 2 ** 20 and peak <= four + 2 * part + 2 ** 20 and peak < 0.6 * sixteen
+
+
+# ---------------------------------------------------------------- sums of whole numbers, exact in 32 bits in whatever order
+def whole(kind, M, N, K, G, seed=0):
+    """Rows, a weight and the product, all whole numbers (scales are 1), every partial sum below 2^24."""
+    from rocmforge_b200 import kernels
+    gen = torch.Generator().manual_seed(seed + M + N + K)
+    q = torch.randint(-8, 8, (N, K), generator=gen, dtype=torch.int8).to(DEV)
+    x = torch.randint(-9, 10, (M, K), generator=gen, dtype=torch.int8).to(DEV)
+    assert 9 * 8 * K < 2 ** 24
+    w = kernels.W4Weight.from_quantized(q, torch.ones(N, (K + G - 1) // G, device=DEV), G)
+    want = (x.double() @ q.double().T).float()
+    if kind != "q8":
+        return x.to(BF if kind == "bf16" else F32), w, want
+    Kp = kernels.padded_columns(K, G)
+    full = torch.zeros(M, Kp, dtype=torch.int8, device=DEV)
+    full[:, :K] = x
+    return kernels.Q8Rows(full, torch.ones(M, Kp // G, device=DEV), K, G, BF), w, want
+
+
+@pytest.mark.parametrize("kind", ["q8", "bf16", "f32"])
+@pytest.mark.parametrize("M", [1, 5, 16, 31, 64, 130, 530])
+@pytest.mark.parametrize("N,K,G", [(48, 19001, 32), (130, 19008, 64), (200, 18944, 128), (1003, 1100, 32), (17, 65, 128)])
+def test_every_column_counts_once(kind, M, N, K, G):
+    """Equal to the last bit: a column left out or counted twice, or a number in the wrong place, shows at any length."""
+    from rocmforge_b200 import kernels
+    x, w, want = whole(kind, M, N, K, G)
+    b, h = torch.arange(N, device=DEV, dtype=F32) - 7, torch.arange(M * N, device=DEV, dtype=F32).view(M, N) % 1000
+    assert torch.equal(kernels.gemm_w4(x, w, b, out_f32=True), want + b)
+    assert torch.equal(kernels.gemm_w4(x, w, out=h.clone(), accumulate=True), want + h)
+    assert torch.equal(kernels.gemm_w4(x, w), want if kind == "f32" else want.to(BF))
+    assert torch.equal(kernels.gemm_w4(x, w, b, out_f32=True, tensor_cores=False), want + b)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 5, 8])
+@pytest.mark.parametrize("kind,plan", [("q8", (1, 1, 1)), ("q8", (1, 1, 16)), ("q8", (2, 1, 4)), ("q8", (2, 2, 2)), ("q8", (4, 1, 8)), ("q8", (4, 2, 4)),
+                                       ("bf16", (1, 1, 1)), ("bf16", (1, 1, 8)), ("bf16", (2, 1, 2)), ("bf16", (2, 2, 4)), ("bf16", (32,)), ("bf16", (64,)), ("bf16", (128,))])
+def test_every_column_counts_once_in_every_plan(monkeypatch, kind, plan, splits):
+    from rocmforge_b200 import kernels
+    from rocmforge_b200.kernels import quantized
+    for M, N, K, G in ((33, 300, 4228, 32), (8, 96, 2050, 64), (17, 450, 6400, 128)):
+        clusters = 3
+        monkeypatch.setattr(quantized, "w4_launch", lambda *a: (*plan, splits) if len(plan) == 1 else (*plan, splits, clusters))
+        if len(plan) == 3:
+            fits = quantized._f("rf_gemm_w4_shared")(0 if kind == "q8" else 1, M, N, K, G, *plan, splits, clusters) <= quantized.W4_MOST_SHARED
+            if not fits:
+                continue
+        x, w, want = whole(kind, M, N, K, G)
+        h = torch.arange(M * N, device=DEV, dtype=F32).view(M, N) % 1000
+        assert torch.equal(kernels.gemm_w4(x, w, out=h.clone(), accumulate=True), want + h)
+        assert torch.equal(kernels.gemm_w4(x, w), want.to(BF))
+
+
+# ---------------------------------------------------------------- the engine
+@pytest.mark.parametrize("row_bits", [8, 16])
+def test_sequences_go_on_alike_in_graphs_and_out_of_them(folders, row_bits):
+    """Decode graphs of one, two and three sequences, replayed in turn with steps outside graphs between them: token by token what the same
+    batches give without any graph."""
+    import rocmforge_b200 as rf
+    from helpers import random_tokens
+    make = lambda graphs: rf.LLM(folders("D", "bfloat16"), options=rf.Options(weight_bits=4, weight_group=64, row_bits=row_bits, decode_graphs=graphs))  # noqa: E731
+    graphs, plain = make(True), make(False)
+    prompts = [random_tokens(300, n, n) for n in (40, 21, 33)]
+    for batch in (prompts[:1], prompts[:2], prompts, prompts[1:], prompts[:2], prompts[:1]):
+        runner = graphs.engine and graphs.engine.decode_runner
+        before = runner.replays if runner else 0
+        got = [r.tokens for r in graphs.generate(batch, max_tokens=12, temperature=0.0, stop_token_ids=[])]
+        assert graphs.engine.decode_runner.replays > (before if graphs.engine.decode_runner is runner else 0)
+        want = [r.tokens for r in plain.generate(batch, max_tokens=12, temperature=0.0, stop_token_ids=[])]
+        assert plain.engine.decode_runner is None and got == want and all(len(t) == 12 for t in got)
+
+
+@pytest.mark.parametrize("row_bits", ["8", "16"])
+def test_the_command_line_passes_its_options_on(folders, monkeypatch, row_bits):
+    """The options reach the model, and the ids that the command prints are those of a model made with the same ones."""
+    import os
+    import subprocess
+    import sys
+
+    import rocmforge_b200 as rf
+    from helpers import ROOT
+    from rocmforge_b200 import cli, kernels
+    from rocmforge_b200.engine import model
+    seen, real = [], model.Model.__init__
+
+    def init(self, *a, **kw):
+        real(self, *a, **kw)
+        seen.append(self)
+    argv = ["--model", folders("D", "bfloat16"), "--prompt-ids", "1,2,3,4,5", "--max-tokens", "8", "--temperature", "0", "--stop-ids", "",
+            "--weight-bits", "4", "--weight-group", "32", "--row-bits", row_bits]
+    monkeypatch.setattr(model.Model, "__init__", init)
+    assert cli.main(argv) == 0
+    options = seen[0].options
+    assert (options.weight_bits, options.weight_group, options.row_bits) == (4, 32, int(row_bits))
+    assert all(isinstance(a.weight, kernels.W4Weight) and a.weight.group == 32 for p in seen[0].spec.named_parts().values() for a in p.linears())
+    run = subprocess.run([sys.executable, os.path.join(ROOT, "bin", "rocmforge"), *argv, "--debug"], capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr
+    got = [int(line.split("token_id=")[1]) for line in run.stderr.splitlines() if line.startswith("[Generated]")]
+    llm = rf.LLM(folders("D", "bfloat16"), options=rf.Options(weight_bits=4, weight_group=32, row_bits=int(row_bits), decode_graphs=False))
+    assert got == llm.generate([[1, 2, 3, 4, 5]], max_tokens=8, temperature=0.0, stop_token_ids=[])[0].tokens
