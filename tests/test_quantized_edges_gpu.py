@@ -373,3 +373,75 @@ def test_the_command_line_passes_its_options_on(folders, monkeypatch, row_bits):
     got = [int(line.split("token_id=")[1]) for line in run.stderr.splitlines() if line.startswith("[Generated]")]
     llm = rf.LLM(folders("D", "bfloat16"), options=rf.Options(weight_bits=4, weight_group=32, row_bits=int(row_bits), decode_graphs=False))
     assert got == llm.generate([[1, 2, 3, 4, 5]], max_tokens=8, temperature=0.0, stop_token_ids=[])[0].tokens
+
+
+OTHERS = ["RC", "VB", "VC", "VE", "FB", "FD", "LB", "LD", "GB", "GC", "GD", "GF", "DB", "DD"]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", OTHERS)
+def test_the_other_designs(folders, name, dtype):
+    """The variants of each design that the engine's tests of 4-bit weights leave out, by the same bounds."""
+    from helpers import random_tokens
+    from test_quantized_engine_gpu import assert_both_close, pair, run_both
+    four, full = pair(folders, name, dtype, 32, 16)
+    V = four.spec.vocab_size
+    longest = min(100, four.spec.max_position - 8)
+    for lens in ((5, 17), (longest, min(51, longest))):
+        a, b = run_both(four, full, [random_tokens(V, n, n) for n in lens], V)
+        assert_both_close(a, b, dtype, f"{name} {dtype} {lens}")
+
+
+def to_8_bits(y, G, dtype):
+    """``Q8Rows`` of numbers in 64 bits."""
+    from rocmforge_b200 import kernels
+    T, K = y.shape
+    p = torch.zeros(T, kernels.padded_columns(K, G), dtype=torch.float64, device=y.device)
+    p[:, :K] = y
+    p = p.view(T, -1, G)
+    a = p.abs().amax(-1, keepdim=True) / 127
+    q = torch.where(a > 0, p / a, 0.0).round().to(torch.int8)
+    return kernels.Q8Rows(q.view(T, -1), a.float().view(T, -1), K, G, dtype)
+
+
+def plain_gemm_w4(x, w, bias=None, *, out=None, out_f32=False, accumulate=False, tensor_cores=True):
+    from rocmforge_b200 import kernels
+    x64 = (x.q.double() * x.scales.double().repeat_interleave(x.group, 1))[:, :x.K] if type(x) is kernels.Q8Rows else x.double()
+    y = x64 @ kernels.dequantize_w4(w, F32).double().T + (0 if bias is None else bias.double())
+    return out.copy_(out.double() + y) if accumulate else y.to(F32 if out_f32 else x.dtype)
+
+
+def plain_add_rmsnorm_q8(h, weight, eps, dtype, group=128, pending=None, rows=None):
+    if pending is not None:
+        h.add_(pending.sum(0) if pending.dim() == 3 else pending.float())
+    x = h.double()
+    return to_8_bits(x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * weight.double(), group, dtype)
+
+
+def plain_swiglu_q8(gu, group=128, activation="silu", dtype=None):
+    return to_8_bits(unit(activation, gu.double()[:, ::2], 1) * gu.double()[:, 1::2], group, dtype or gu.dtype)
+
+
+@pytest.mark.parametrize("name", ["A", "B", "C", "D", "E", "RA", "RB", "VA", "VD", "FA", "FC", "LA", "LC", "GA", "GE", "DA", "DC", *OTHERS])
+def test_8_bit_rows_in_the_engine_are_those_of_the_formulas(folders, monkeypatch, name):
+    """Every design in 32 bits with 8-bit rows, against itself with the operators in 64 bits: the same numbers to 32-bit accuracy.  A number that lies
+    on the border between two steps may fall to either side, which shows in the logits after it and in no others; what is wrong shows in all."""
+    import rocmforge_b200 as rf
+    from helpers import random_tokens
+    from rocmforge_b200 import kernels
+    m = rf.Model.from_folder(folders(name, "float32"), dtype=F32, options=rf.Options(weight_bits=4, weight_group=32))
+    V, out, used = m.spec.vocab_size, [], set()
+    for plain in (False, True):
+        if plain:
+            for f in (plain_gemm_w4, plain_add_rmsnorm_q8, plain_swiglu_q8):
+                monkeypatch.setattr(kernels, f.__name__[6:], lambda *a, f=f, **kw: (used.add(f.__name__), f(*a, **kw))[1])
+            monkeypatch.setattr(kernels, "quantize_q8", lambda x, group=128: to_8_bits(x.double(), group, x.dtype))
+        cache = m.new_cache(max_tokens=64 * 24, max_slots=4)
+        slots = [cache.alloc_slot() for _ in (5, 17)]
+        got = [m.step(cache, [rf.StepRequest(s, p, [0, len(p) - 1]) for s, p in zip(slots, [random_tokens(V, n, n) for n in (5, 17)])])]
+        for d in range(3):
+            got.append(m.step(cache, [rf.StepRequest(s, [random_tokens(V, 1, 10 * d + i)[0]], [0]) for i, s in enumerate(slots)]))
+        out.append(torch.cat(got).cpu().double())
+    assert "plain_gemm_w4" in used
+    off = (out[0] - out[1]).norm(dim=1) / out[1].norm(dim=1)
+    assert torch.isfinite(out[0]).all() and int((off < 1e-5).sum()) >= 3, off
