@@ -668,6 +668,9 @@ def main():
     ap.add_argument("--fused-norm-max", type=int, default=None,
                     help="--only runs: most tokens of a step for which products prepare the norm that follows them")
     ap.add_argument("--dtype", choices=["bf16", "fp32"], default="bf16", help="--only decode / prefill: the bfloat16 or the true 32-bit path")
+    ap.add_argument("--weight-bits", type=int, choices=[4, 16], default=16, help="--only decode / prefill: 4, the model with weights in 4 bits")
+    ap.add_argument("--weight-group", type=int, choices=[32, 64, 128], default=128, help="--only decode / prefill: columns that share a 4-bit weight's scale")
+    ap.add_argument("--row-bits", type=int, choices=[8, 16], default=8, help="--only decode / prefill: what products of few tokens with 4-bit weights read")
     ap.add_argument("--prefill-tokens", type=int, default=PREFILL_TOKENS, help="--only prefill: tokens of the prompt")
     ap.add_argument("--seed", type=int, default=0)
     args = ap.parse_args()
@@ -726,7 +729,8 @@ def main():
         raw["num_hidden_layers"] = args.layers
     cfg = Qwen2Config.from_dict(raw)
     V = cfg.vocab_size
-    model = rf.Model.random(cfg, seed=args.seed, dtype=torch.float32 if (args.only and args.dtype == "fp32") else torch.bfloat16)
+    options = rf.Options(weight_bits=args.weight_bits, weight_group=args.weight_group, row_bits=args.row_bits) if args.only in ("decode", "prefill") else None
+    model = rf.Model.random(cfg, seed=args.seed, dtype=torch.float32 if (args.only and args.dtype == "fp32") else torch.bfloat16, options=options)
     if args.only and args.fused_norm:
         model.options.fused_norm = True
     if args.only and args.fused_norm_max is not None:

@@ -72,7 +72,7 @@ struct Place {
 };
 
 // ---------------------------------------------------------------- rows to 8 bits
-// A lane has four columns.  (64 x 3,584 1.6 us: a launch; 2,048 x 3,584 9.9, floor 3.4: a group's two divisions and shuffles in every lane.)
+// A lane has four columns.  (64 x 3,584 1.6 us: a launch; 2,048 x 3,584 10.8, floor 3.4: a group's two divisions and shuffles in every lane.)
 template <typename T, int G, bool VEC>
 __global__ void __launch_bounds__(256) quantize_q8_kernel(const T* x, long long ldx, int8_t* __restrict__ q, float* __restrict__ scales,
                                                           int T_, int K, int Kp) {
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256) quantize_q8_kernel(const T* x, long long 
     }
 }
 
-// ... and the numbers that 8-bit rows stand for, eight (rows of whole eights, on 16-byte boundaries: 2,048 x 3,584 5.5 us, by fours 9.2) or four
+// ... and the numbers that 8-bit rows stand for, eight (rows of whole eights, on 16-byte boundaries: 2,048 x 3,584 5.9 us, by fours 9.2) or four
 // columns a thread.
 template <typename T, int EACH>
 __global__ void __launch_bounds__(256) dequantize_q8_kernel(const int8_t* q, const float* scales, T* __restrict__ y, int T_, int K, int Kp, int G) {
@@ -156,8 +156,8 @@ __global__ void __launch_bounds__(256) swiglu_q8_kernel(const T* gu, int8_t* __r
 // ---------------------------------------------------------------- add + RMSNorm to 8 bits
 // v = h[row] + sum_s pending[s][row];  y = v rsqrt(mean(v^2) + eps) w, to 8 bits from 32.  The kinds of pending and of rows are those
 // of add_rmsnorm (elementwise.cu).  A block has a row, a lane four columns at a time, in registers: one pass over the stream and what is added to
-// it.  2,048 x 3,584 after a 16-bit update 16.6 us, 4.9 TB/s (the norm with a 16-bit result 21.1); 64 x 5,120 after five sums 4.6 and 1 x 896 after
-// four 2.0: a chain of trips to L2 and of the block's sum.
+// it.  2,048 x 3,584 after a 16-bit update 17.4 us, 4.7 TB/s (the norm with a 16-bit result 21.1); 64 x 5,120 after five sums 4.7 and 1 x 896 after
+// four 2.1: a chain of trips to L2 and of the block's sum.
 template <typename T, int G, int NV, bool VEC>
 __global__ void __launch_bounds__(1024) add_rmsnorm_q8_kernel(float* __restrict__ h, const void* pending, int kind, int n_pending,
                                                               size_t pstride, const void* w, int w_is_f32, float eps,
@@ -227,7 +227,8 @@ __device__ __forceinline__ float w4_scale(float m) {
     u += 0x3ffffu + (u >> 19 & 1u);                      // to the nearest of five significant bits, ties to even
     return __uint_as_float(u & 0xfff80000u);
 }
-// A warp makes the tiles of a group's columns: lane 4 g + t holds the eight columns of its two rows and two halves, 32 numbers a tile.
+// A warp makes the tiles of a group's columns: lane 4 g + t holds the eight columns of its two rows and two halves, 32 numbers a tile, read one by
+// one (rows start anywhere).  37,888 x 3,584 150 us from float32, 4.1 TB/s, 179 from bfloat16: loads; it runs once, when a model is made.
 template <typename T, int G>
 __global__ void __launch_bounds__(256) quantize_w4_kernel(const T* weight, long long ldw, uint4* __restrict__ packed, __nv_bfloat16* __restrict__ scales,
                                                           int N, int K, int Kp) {
@@ -281,7 +282,8 @@ __global__ void __launch_bounds__(256) quantize_w4_kernel(const T* weight, long 
     }
 }
 
-// The weights as numbers, columns lo .. hi - 1 (lo a multiple of 64): a warp writes a tile, a lane four runs of eight columns.
+// The weights as numbers, columns lo .. hi - 1 (lo a multiple of 64): a warp writes a tile, a lane four runs of eight columns.  37,888 x 3,584 to
+// bfloat16 56 us, 6.1 TB/s, to float32 134 us, 4.6 TB/s: what it writes.
 template <typename T, int G>
 __global__ void __launch_bounds__(256) dequantize_w4_kernel(const uint4* packed, const __nv_bfloat16* scales, T* __restrict__ out, int N, int Kp, int lo, int hi) {
     pdl_wait(packed, scales);

@@ -417,8 +417,12 @@ def gemm_w4(x, w: W4Weight, bias: torch.Tensor | None = None, *, out: torch.Tens
     """y = x @ w.T (+ bias) with 4-bit weights, 32-bit sums.
 
     ``x``: ``Q8Rows`` of the weight's K and group (products inside a group are exact, in whole numbers), or a tensor [M, K] in bfloat16
-    or float32.  out_f32: the result is float32 whatever the rows; accumulate: added into ``out`` (float32); tensor_cores: whether the
-    tcgen05 kernels may take it (as in ``gemm_plain``)."""
+    or float32.  out_f32: the result is float32 whatever the rows; accumulate: added into ``out`` (float32, apart from ``x``);
+    tensor_cores: whether the tcgen05 kernels may take it (as in ``gemm_plain``).
+
+    8-bit rows stay what they are for any number of them, though from some 40 on bfloat16 rows take less time (``W4_FEW_TOKENS``).  Few
+    bfloat16 rows: a group's sum is formed before its scale, so numbers of 2^118 and more may overflow where the scaled sum would not.
+    float32 rows multiply weights written out in float32: a buffer of that size for the call, and its time (37,888 x 3,584 239 us)."""
     q8 = type(x) is Q8Rows
     if not (q8 or isinstance(x, torch.Tensor)) or type(w) is not W4Weight:
         raise KernelError("gemm_w4: x must be Q8Rows or a tensor, w a W4Weight")
