@@ -383,10 +383,11 @@ __device__ __forceinline__ unsigned long long fma_two(unsigned long long a, unsi
 // at 1.5 2^23 as a float's bits, so that its bits are that float plus the sum (below 2^22: 128 columns of 16 * 8 * 127), and no conversion is
 // needed.  16-bit rows: the halves of bytes become bfloat16 numbers and a group's sum is a float.
 // What bounds it, and what it took (device time in a chain of launches over weights larger than L2): 1 to 8 8-bit rows x 37,888 x 3,584 12.9 to
-// 13.1 us, 5.5 TB/s: the weights' stream; 1 x 4,608 x 3,584 4.4 us, 1 x 896 x 896 2.4: a launch, one trip to memory and the warps' sums.  16 rows
-// 14.4 us, 32 21.4, 64 35.2 (in groups of 32 columns 59), 64 x 3,584 x 18,944 in groups of 64 33.2: instructions; at 64 x 37,888 x 3,584 the
-// schedulers issue in 60 % of cycles and the tensor cores are busy in 38 %.  16-bit rows: 1 x 37,888 x
-// 3,584 19 us, 16 x 27,648 x 5,120 26.7: widening the weights, whatever the tokens.
+// 13.0 us, 5.4 TB/s: the weights' stream; 1 x 4,608 x 3,584 4.3 us, 1 x 896 x 896 2.4: a launch, one trip to memory and the warps' sums.  16 rows
+// 14.0 us, 32 22.1, 64 39.2 (in groups of 32 columns 63; four eights of tokens by two tiles a warp, which the cost rule misses here, 34.5),
+// 64 x 3,584 x 18,944 in groups of 64 32.8: instructions; at 64 x 37,888 x 3,584 the
+// schedulers issue in 61 % of cycles and the tensor cores are busy in 39 %.  16-bit rows: 1 x 37,888 x
+// 3,584 19 us, 16 x 27,648 x 5,120 27.0: widening the weights, whatever the tokens.
 #define W4_WARPS 16
 #define W4_SLOT (1024 + 128)                             // a unit's weights, and its scales [group][16 rows]
 #define W4_SUMS(rt) (16 * (rt) * W4_WARPS + 4)           // pitch of the warps' sums [token][16 rt rows a warp]

@@ -11,8 +11,8 @@
 // 1.1e-5 off, pieces of 6,315 columns 2.6e-6).  For 32-bit results a sum runs over W4T_PIECE columns at most: the widening warps add it to a
 // second one beside it, rounded, while the next piece goes into another accumulator (tiles of 128 tokens: into the same one, after a wait).
 //
-// What it took (32-bit results, device time in a chain of launches over weights larger than L2): 32 x 37,888 x 3,584 27.8 us, 64 29.2, 128 37.6 (the
-// 16-bit product of as many tokens 44, 47, 56), 64 x 3,584 x 18,944 19.6 (105), 128 x 4,608 x 3,584 11.5 (21.8), 512 x 3,584 x 18,944 66 (94).
+// What it took (32-bit results, device time in a chain of launches over weights larger than L2): 32 x 37,888 x 3,584 28.5 us, 64 30.2, 128 38.5 (the
+// 16-bit product of as many tokens 42, 44, 49), 64 x 3,584 x 18,944 20.2 (81), 128 x 4,608 x 3,584 11.7 (22.4), 512 x 3,584 x 18,944 68 (94).
 // What bounds it: up to 128 tokens the widening, 1.5 us for 512 columns of 128 rows (15 instructions a lane for 8 weights; the schedulers issue in
 // 56 to 60 % of cycles, waits between its parts), and what comes before and after a block's loop, 3 us and, with 128 tokens, 7; many tokens: widening
 // beside MMAs that would take 1.1 us.

@@ -312,15 +312,15 @@ def swiglu_q8(gu: torch.Tensor, group: int = 128, activation: str = "silu", dtyp
     return y
 
 
-# Products of up to so many tokens take rows in 8 bits where a step may choose (32 x 37,888 x 3,584: 22.0 us against 27.8 of 16-bit rows; 64 tokens:
-# 34.7, 29.3; 64 x 3,584 x 18,944: 30.6, 19.7).
+# Products of up to so many tokens take rows in 8 bits where a step may choose (32 x 37,888 x 3,584: 22.1 us against 28.5 of 16-bit rows; 64 tokens:
+# 39.2, 30.2; 64 x 3,584 x 18,944: 28.0, 20.2).
 W4_FEW_TOKENS = 32
-# 16-bit rows straight from the 4 bits: up to so many tokens (512 x 37,888 x 3,584: 148 us, 165 by the weights written out in 16 bits; 512 x 3,584 x
-# 18,944: 63, 124; 1,024: 317, 257 and 128, 137).
+# 16-bit rows straight from the 4 bits: up to so many tokens (512 x 37,888 x 3,584: 147 us, 155 by the weights written out in 16 bits; 512 x 3,584 x
+# 18,944: 59, 123; 1,024: 289, 239 and 120, 142).
 W4_TC_MOST = 512
 # 32-bit results of rows of several SUM_COLUMNS: up to so many with two of them, twice as many with more, since that other way takes a pass over
-# the result for each (1,024 x 4,608 x 3,584: 36 us against 49, 2,048: 70, 66; 2,048 x 3,584 x 18,944: 275, 331; 4,096: 502, 564; 2,048 x 5,120 x
-# 13,824: 282, 311)
+# the result for each (1,024 x 4,608 x 3,584: 40 us against 51, 2,048: 74, 68; 2,048 x 3,584 x 18,944: 273, 338; 4,096: 488, 586; 2,048 x 5,120 x
+# 13,824: 260, 326)
 W4_TC_MOST_F32 = 1024
 # Columns that one tensor-core sum runs over where the result is 32-bit: its additions are cut, not rounded, and what is cut adds up
 # (1,999 x 3,584 x 18,944 against 64 bits: one sum 1.1e-5, pieces of 6,315 2.6e-6, of 2,048 5e-7)
